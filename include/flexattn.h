@@ -328,6 +328,107 @@ int fa_bwd_dq(const fa_params *p, const void *q, const void *k, const void *v, c
               const float *lse, const float *delta, void *dq, void *stream);
 
 /*
+ * Around a KV cache: rotary positions, appends and decode over a cache in 8
+ * bits.  No reference counterpart (its roadmap lists a decode kernel).
+ *
+ * Rotary positions: the first 2 * pairs elements of a head are rotated in
+ * pairs by pos * inv_freq[i] radians and multiplied by scale, the others
+ * copied.  Pair i is elements (i, i + pairs), or with interleaved (2 i, 2 i + 1).
+ * The angles are computed in 64 bits: any position keeps fp32 accuracy.
+ */
+typedef struct fa_rotary {
+  const double *inv_freq; /* (pairs) radians per position, device */
+  int32_t pairs, interleaved;
+  float scale;
+} fa_rotary;
+
+/* A (B, heads, T, D) tensor with element strides of its first three
+ * dimensions (a projection's (B, T, heads, D) output is read in place); the
+ * last one is dense. */
+typedef struct fa_strided {
+  const void *data;
+  int64_t stride_b, stride_h, stride_t;
+  int32_t heads;
+} fa_strided;
+
+/* out[i] (B, heads, T, D) dense = rotated in[i], i < count <= 2 (queries and
+ * keys in one launch), bf16 or float32; with inverse the transposed rotation
+ * (the gradient).  Token t of row b is at positions[b * positions_stride + t]
+ * (int32, or int64 with positions_64), or at offset + t where positions is
+ * null.  Any even 2 * pairs <= D <= 1024, any strides and alignment (16-byte accesses
+ * where 2 * pairs and D are multiples of 16 and every row is aligned).  The
+ * outputs must not overlap the inputs. */
+typedef struct fa_rotary_call {
+  int32_t abi_version, dtype; /* FA_ABI_VERSION; FA_DTYPE_BF16 or FA_DTYPE_F32 */
+  int32_t B, T, D, inverse;
+  fa_rotary rotary;
+  int32_t count;
+  fa_strided in[2];
+  void *out[2];
+  const void *positions;
+  int32_t positions_64;
+  int64_t positions_stride, offset;
+} fa_rotary_call;
+int fa_apply_rotary(const fa_rotary_call *c, void *stream);
+
+/* A paged cache in e4m3: k, v (num_pages, Hkv, page_size, D); each run of 32
+ * tokens of a page and head has one scale, a power of two in [2^-126, 2^127],
+ * k_scale, v_scale (num_pages, Hkv, page_size / 32): the value is code x scale
+ * (only the scale's exponent is read).  page_size is a multiple of 32. */
+enum { FA_KV_RUN = 32 };
+
+/* Appends T new tokens per batch row: token t < new_lens[b] (null: T; the rest
+ * of a padded row is left out) goes to position kv_lens[b] + t, i.e. to row
+ * pos % page_size of page page_table[b * max_pages + pos / page_size] (page
+ * table null: page b is row b's).  Tokens whose position lies past max_pages
+ * pages, or whose page id is outside [0, num_pages), are dropped; everything
+ * else in the cache is left as it was.  Keys are rotated to their positions
+ * first (rotary.pairs 0: not).  The pages that a call writes belong to one
+ * batch row each.
+ * cache_dtype FA_DTYPE_BF16: k_cache, v_cache bf16 (fa_fwd_kvcache's layout).
+ * FA_DTYPE_FP8_E4M3: codes; a run's scale is 2^e with e the smallest integer in
+ * [-126, 127] such that 448 2^e >= the largest finite |x| of its tokens, from the float32
+ * rotated keys (one rounding, to nearest even; NaN and infinities become the
+ * NaN code).  A run that the call finds begun keeps its scale, or where the
+ * new tokens need a larger one takes that, its older codes moved to it.
+ * query (heads 0: none): (B, heads, T, D) rotated like the keys into query_out,
+ * padded tokens too.  bf16 inputs with 16-byte aligned rows, D = 32, 64 or 128,
+ * 2 * pairs a multiple of 16. */
+typedef struct fa_kv_append_call {
+  int32_t abi_version, cache_dtype;
+  int32_t B, T, D, page_size, max_pages, num_pages;
+  fa_strided key, value, query;
+  void *query_out;
+  void *k_cache, *v_cache;
+  float *k_scale, *v_scale;
+  const int32_t *page_table, *kv_lens, *new_lens;
+  fa_rotary rotary;
+} fa_kv_append_call;
+int fa_kv_append(const fa_kv_append_call *c, void *stream);
+
+/* Decode over a paged cache in e4m3 (p->dtype = FA_DTYPE_FP8_E4M3; q, o bf16,
+ * lse float32; D = 32, 64 or 128).  Row b has kv_lens[b] keys (null: p->Skv, the
+ * tokens of its page table) and its queries are the newest of them: query i of
+ * q_lens[b] (null: Sq) sits at position kv_lens[b] - q_lens[b] + i, which is
+ * what p's window and ALiBi refer to; queries i >= q_lens[b] give o = 0 and
+ * lse = -inf, as do queries that see no key.  Page ids outside the cache read
+ * as zero keys.  Document ids and block tables are refused.  Workgroups take
+ * equal shares of all rows' tiles of 32 keys; the partial results of items
+ * that several of them share are joined in a fixed order by a second launch.
+ * The workspace is 16-byte aligned, of the size that the other function gives
+ * (0 where a call would be refused); calls that overlap in time need one each. */
+typedef struct fa_fp8_cache {
+  const void *k, *v;
+  const float *k_scale, *v_scale;
+  const int32_t *page_table; /* (B, max_pages) or NULL: page b is row b's */
+  int32_t page_size, max_pages, num_pages;
+  const int32_t *kv_lens, *q_lens; /* (B) or NULL */
+} fa_fp8_cache;
+size_t fa_fwd_kvcache_fp8_workspace_bytes(const fa_params *p, const fa_fp8_cache *kv);
+int fa_fwd_kvcache_fp8(const fa_params *p, const fa_fp8_cache *kv, const void *q, void *o, float *lse,
+                       void *workspace, size_t workspace_bytes, void *stream);
+
+/*
  * Block-mask construction on the device (create_block_mask, block_mask.py:54-129)
  * for the mask semantics of fa_params: the window (window_left, window_right)
  * and, optionally, document ids shared by queries and keys (token t of table

@@ -15,6 +15,7 @@ CSRC = os.path.join(HERE, "csrc")
 # the tile-kernel instantiations and is compiled once per head dim and
 # direction, so the objects build in parallel.
 UNITS = [(os.path.join(CSRC, "capi.hip"), [], "capi"), (os.path.join(CSRC, "kernels_fp8.hip"), [], "kernels_fp8"),
+         (os.path.join(CSRC, "kernels_cache.hip"), [], "kernels_cache"),
          (os.path.join(CSRC, "host.cpp"), [], "host")] + [
     (os.path.join(CSRC, "kernels.hip"), [f"-DFA_KERNELS_D={d}", f"-DFA_KERNELS_BWD={bwd}"],
      f"kernels_d{d}_{'bwd' if bwd else 'fwd'}")

@@ -1,0 +1,199 @@
+// Argument checks and kernel arguments of the C ABI calls around a KV cache
+// (included by capi.hip inside its anonymous namespace).
+
+bool aligned(const void* p, int bytes) { return (reinterpret_cast<uintptr_t>(p) & (bytes - 1)) == 0; }
+
+// Rows of a strided tensor start at multiples of 16 bytes.
+bool rows16(const fa_strided& t, int es) {
+  const long long m = 16 / es - 1;
+  return aligned(t.data, 16) && !(t.stride_b & m) && !(t.stride_h & m) && !(t.stride_t & m);
+}
+
+// Heads that one thread takes its angles through: as many as leave every
+// compute unit eight workgroups of 256 threads (the angles of 8 pairs cost as much as
+// about ten heads' arithmetic, but only few tokens leave too few threads).
+int heads_per_thread(long long threads, int heads) {
+  const long long full = 8ll * 256 * device_cus();
+  long long groups = full / (threads > 0 ? threads : 1);
+  if (groups < 1) groups = 1;
+  if (groups > heads) groups = heads;
+  return (int)((heads + groups - 1) / groups);
+}
+
+int rotary_geometry(fa::RotaryArgs* a, bool vec) {
+  const int pairs = (a->n + 7) / 8;
+  a->units = vec ? a->D / 16 : pairs + (a->D - 2 * a->n + 15) / 16;
+  const int heads = a->t[0].heads + a->t[1].heads;
+  const long long tokens = (long long)a->B * a->T * a->units;
+  a->per = heads_per_thread(tokens, heads);
+  a->groups = cdiv(heads, a->per);
+  // (one thread index; the last workgroup's included)
+  return tokens * a->groups > 0x7fffff00ll ? FA_ERR_SHAPE : FA_OK;
+}
+
+int rotary_args(const fa_rotary_call* c, fa::RotaryArgs* a, bool* vec) {
+  if (!c) return FA_ERR_NULL;
+  if (c->abi_version != FA_ABI_VERSION) return FA_ERR_VERSION;
+  if (c->dtype != FA_DTYPE_BF16 && c->dtype != FA_DTYPE_F32) return FA_ERR_DTYPE;
+  if (c->B < 1 || c->T < 1 || c->D < 1 || c->D > 1024 || c->count < 1 || c->count > 2) return FA_ERR_SHAPE;
+  if (c->rotary.pairs < 1 || 2 * (long long)c->rotary.pairs > c->D) return FA_ERR_SHAPE;
+  if (!c->rotary.inv_freq) return FA_ERR_NULL;
+  if (!aligned(c->rotary.inv_freq, 8) || !aligned(c->positions, c->positions_64 ? 8 : 4)) return FA_ERR_SHAPE;
+  *a = fa::RotaryArgs{};
+  const int es = c->dtype == FA_DTYPE_F32 ? 4 : 2;
+  *vec = c->rotary.pairs % 8 == 0 && c->D % 16 == 0;
+  for (int i = 0; i < c->count; ++i) {
+    const fa_strided& t = c->in[i];
+    if (!t.data || !c->out[i]) return FA_ERR_NULL;
+    if (t.heads < 1 || !aligned(t.data, es) || !aligned(c->out[i], es)) return FA_ERR_SHAPE;
+    *vec = *vec && rows16(t, es) && aligned(c->out[i], 16);
+    a->t[i] = {t.data, c->out[i], t.stride_b, t.stride_h, t.stride_t, t.heads};
+  }
+  a->B = c->B;
+  a->T = c->T;
+  a->D = c->D;
+  a->freq = c->rotary.inv_freq;
+  a->n = c->rotary.pairs;
+  a->interleaved = c->rotary.interleaved != 0;
+  a->inverse = c->inverse != 0;
+  a->scale = c->rotary.scale;
+  a->positions = c->positions;
+  a->pos64 = c->positions_64 != 0;
+  a->pos_stride = c->positions_stride;
+  a->offset = c->offset;
+  return rotary_geometry(a, *vec);
+}
+
+int append_args(const fa_kv_append_call* c, fa::AppendArgs* a) {
+  if (!c) return FA_ERR_NULL;
+  if (c->abi_version != FA_ABI_VERSION) return FA_ERR_VERSION;
+  if (c->cache_dtype != FA_DTYPE_BF16 && c->cache_dtype != FA_DTYPE_FP8_E4M3) return FA_ERR_DTYPE;
+  const bool fp8 = c->cache_dtype == FA_DTYPE_FP8_E4M3;
+  if (c->D != 32 && c->D != 64 && c->D != 128) return FA_ERR_UNSUPPORTED;
+  const int Hkv = c->key.heads;
+  if (c->B < 1 || c->T < 1 || Hkv < 1 || c->value.heads != Hkv || c->query.heads < 0) return FA_ERR_SHAPE;
+  if (c->page_size < FA_KV_RUN || c->page_size % FA_KV_RUN || c->num_pages < 1 || c->max_pages < 1) return FA_ERR_SHAPE;
+  if (!c->page_table && (c->max_pages != 1 || c->num_pages < c->B)) return FA_ERR_SHAPE;
+  if (!c->key.data || !c->value.data || !c->k_cache || !c->v_cache || !c->kv_lens) return FA_ERR_NULL;
+  if (fp8 && (!c->k_scale || !c->v_scale)) return FA_ERR_NULL;
+  if (!rows16(c->key, 2) || !rows16(c->value, 2) || !aligned16({c->k_cache, c->v_cache})) return FA_ERR_SHAPE;
+  const bool turn = c->rotary.pairs != 0;
+  if (turn) {
+    if (!c->rotary.inv_freq) return FA_ERR_NULL;
+    if (c->rotary.pairs < 0 || 2 * (long long)c->rotary.pairs > c->D || !aligned(c->rotary.inv_freq, 8)) return FA_ERR_SHAPE;
+    if (c->rotary.pairs % 8) return FA_ERR_UNSUPPORTED;
+  }
+  *a = fa::AppendArgs{};
+  a->k = c->key.data;
+  a->v = c->value.data;
+  a->ksb = c->key.stride_b, a->ksh = c->key.stride_h, a->kst = c->key.stride_t;
+  a->vsb = c->value.stride_b, a->vsh = c->value.stride_h, a->vst = c->value.stride_t;
+  a->kc = c->k_cache;
+  a->vc = c->v_cache;
+  a->ks = c->k_scale;
+  a->vs = c->v_scale;
+  a->page_table = c->page_table;
+  a->page_size = c->page_size;
+  a->max_pages = c->max_pages;
+  a->num_pages = c->num_pages;
+  a->kv_lens = c->kv_lens;
+  a->new_lens = c->new_lens;
+  a->B = c->B;
+  a->Hkv = Hkv;
+  a->T = c->T;
+  if (turn) {
+    a->freq = c->rotary.inv_freq;
+    a->n = c->rotary.pairs;
+    a->interleaved = c->rotary.interleaved != 0;
+    a->scale = c->rotary.scale;
+  }
+  const long long runs = ((long long)c->T + FA_KV_RUN - 2) / FA_KV_RUN + 1;
+  const long long token_threads = runs * FA_KV_RUN * c->B * (c->D / 16);
+  a->per = heads_per_thread(token_threads, Hkv);
+  a->groups = cdiv(Hkv, a->per);
+  const long long blocks = runs * c->B * a->groups;
+  if (blocks > 0x7fffffll) return FA_ERR_SHAPE;
+  a->runs = (int)runs;
+  a->kv_blocks = (int)blocks;
+  if (c->query.heads > 0) {
+    if (!turn) return FA_ERR_SHAPE;  // nothing to do for the queries
+    if (!c->query.data || !c->query_out) return FA_ERR_NULL;
+    if (!rows16(c->query, 2) || !aligned(c->query_out, 16)) return FA_ERR_SHAPE;
+    fa::RotaryArgs& q = a->q;
+    q.t[0] = {c->query.data, c->query_out, c->query.stride_b, c->query.stride_h, c->query.stride_t, c->query.heads};
+    q.B = c->B;
+    q.T = c->T;
+    q.D = c->D;
+    q.freq = a->freq;
+    q.n = a->n;
+    q.interleaved = a->interleaved;
+    q.scale = a->scale;
+    q.kv_lens = c->kv_lens;
+    return rotary_geometry(&q, true);
+  }
+  return FA_OK;
+}
+
+struct DecodeLayout {
+  int nq;               // 16-row query blocks per work item
+  size_t part, ml, bytes;
+};
+
+int decode_args(const fa_params* p, const fa_fp8_cache* kv, int cus, fa::DecodeArgs* a, DecodeLayout* L) {
+  if (!p || !kv) return FA_ERR_NULL;
+  if (p->abi_version != FA_ABI_VERSION) return FA_ERR_VERSION;
+  if (p->dtype != FA_DTYPE_FP8_E4M3) return FA_ERR_DTYPE;
+  if (p->D != 32 && p->D != 64 && p->D != 128) return FA_ERR_UNSUPPORTED;
+  if (p->B < 1 || p->Hq < 1 || p->Hkv < 1 || p->Hq % p->Hkv || p->Sq < 1 || p->Skv < 1) return FA_ERR_SHAPE;
+  if (!(p->softcap >= 0.f) || !(p->scale >= 0.f)) return FA_ERR_SHAPE;
+  if (p->q_doc_ids || p->kv_doc_ids || p->doc_start || p->doc_end || p->kv_num_blocks || p->kv_indices ||
+      p->full_kv_num_blocks || p->full_kv_indices)
+    return FA_ERR_UNSUPPORTED;
+  if (kv->page_size < FA_KV_RUN || kv->page_size % FA_KV_RUN || kv->num_pages < 1 || kv->max_pages < 1) return FA_ERR_SHAPE;
+  if (!kv->page_table && (kv->max_pages != 1 || kv->num_pages < p->B)) return FA_ERR_SHAPE;
+  if ((long long)kv->max_pages * kv->page_size < p->Skv) return FA_ERR_SHAPE;
+  const long long runs = (long long)kv->num_pages * p->Hkv * (kv->page_size / FA_KV_RUN);
+  if (runs > 0x7fffffffll) return FA_ERR_SHAPE;  // run indices are 32 bits (2^36 token rows)
+  if (!kv->k || !kv->v || !kv->k_scale || !kv->v_scale) return FA_ERR_NULL;
+  if (!aligned16({kv->k, kv->v})) return FA_ERR_SHAPE;
+  *a = fa::DecodeArgs{};
+  const int g = p->Hq / p->Hkv;
+  const long long rows = (long long)g * p->Sq;
+  if (rows * p->B * p->Hkv > 0x7ffffffll) return FA_ERR_SHAPE;
+  L->nq = rows <= 16 ? 1 : rows <= 32 ? 2 : 4;
+  const long long rt = (rows + 16 * L->nq - 1) / (16 * L->nq);
+  const long long items = p->B * (long long)p->Hkv * rt;
+  const long long tiles = (p->Skv + fa::kTileKeys - 1) / fa::kTileKeys;
+  if (items * tiles > 0x7fffffffll - (1 << 20)) return FA_ERR_SHAPE;  // tile numbers of a call are 32 bits
+  a->k = static_cast<const uint8_t*>(kv->k);
+  a->v = static_cast<const uint8_t*>(kv->v);
+  a->ks = kv->k_scale;
+  a->vs = kv->v_scale;
+  a->page_table = kv->page_table;
+  a->kv_lens = kv->kv_lens;
+  a->q_lens = kv->q_lens;
+  a->B = p->B;
+  a->Hq = p->Hq;
+  a->Hkv = p->Hkv;
+  a->Sq = p->Sq;
+  a->g = g;
+  a->page_runs = kv->page_size / FA_KV_RUN;
+  a->max_pages = kv->max_pages;
+  a->num_pages = kv->num_pages;
+  a->cap = p->Skv;
+  a->win_left = p->window_left < 0 ? -1 : p->window_left;
+  a->win_right = p->window_right < 0 ? -1 : p->window_right;
+  a->scale = p->scale == 0.f ? 1.0f / sqrtf((float)p->D) : p->scale;
+  a->scale_log2 = a->scale * fa::kLog2e;
+  a->softcap = p->softcap;
+  a->alibi = p->alibi_slopes;
+  a->rt = (int)rt;
+  a->least = 16;
+  const long long most = (items * tiles + a->least - 1) / a->least;  // workgroups with a chunk of their own
+  a->wgs = (int)(most < 2ll * cus ? most : 2ll * cus);
+  const size_t slots = 2 * (size_t)a->wgs * 16 * L->nq;
+  L->part = (((size_t)p->B + 2) * sizeof(int) + 255) & ~(size_t)255;
+  L->ml = L->part + slots * p->D * sizeof(float);
+  L->bytes = L->ml + slots * 2 * sizeof(float);
+  return FA_OK;
+}

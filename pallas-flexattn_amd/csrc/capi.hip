@@ -280,6 +280,7 @@ int fwd_fp8_launch(const fa_params* p, const fa_fp8_inputs* in, bool q16, void* 
 }
 
 #include "user_mods.h"
+#include "cache_calls.h"
 
 }  // namespace
 
@@ -644,6 +645,47 @@ int fa_mods_bwd_dq(const fa_mods* m, const fa_params* p, const void* const* bufs
   a.delta = const_cast<float*>(delta);
   a.dq = dq;
   return mods_bwd_stages(m, p, bufs, nbufs, a, kStageDq, static_cast<hipStream_t>(stream));
+}
+
+int fa_apply_rotary(const fa_rotary_call* c, void* stream) {
+  fa::RotaryArgs a;
+  bool vec;
+  const int rc = rotary_args(c, &a, &vec);
+  if (rc) return rc;
+  return fa::launch_rotary(a, c->dtype == FA_DTYPE_F32, vec, static_cast<hipStream_t>(stream));
+}
+
+int fa_kv_append(const fa_kv_append_call* c, void* stream) {
+  fa::AppendArgs a;
+  const int rc = append_args(c, &a);
+  if (rc) return rc;
+  return fa::launch_append(a, c->D, c->cache_dtype == FA_DTYPE_FP8_E4M3, static_cast<hipStream_t>(stream));
+}
+
+size_t fa_fwd_kvcache_fp8_workspace_bytes(const fa_params* p, const fa_fp8_cache* kv) {
+  fa::DecodeArgs a;
+  DecodeLayout L;
+  return decode_args(p, kv, device_cus(), &a, &L) == FA_OK ? L.bytes : 0;
+}
+
+int fa_fwd_kvcache_fp8(const fa_params* p, const fa_fp8_cache* kv, const void* q, void* o, float* lse,
+                       void* workspace, size_t workspace_bytes, void* stream) {
+  fa::DecodeArgs a;
+  DecodeLayout L;
+  const int rc = decode_args(p, kv, device_cus(), &a, &L);
+  if (rc) return rc;
+  if (!q || !o || !lse) return FA_ERR_NULL;
+  if (!aligned16({q, o})) return FA_ERR_SHAPE;
+  if (!workspace || workspace_bytes < L.bytes || !aligned16({workspace})) return FA_ERR_WORKSPACE;
+  a.q = q;
+  a.o = o;
+  a.lse = lse;
+  char* ws = static_cast<char*>(workspace);
+  a.head = reinterpret_cast<int*>(ws);
+  a.part = reinterpret_cast<float*>(ws + L.part);
+  a.part_ml = reinterpret_cast<float*>(ws + L.ml);
+  return fa::launch_decode_fp8(a, p->D, L.nq, p->alibi_slopes != nullptr || p->softcap > 0.f,
+                               static_cast<hipStream_t>(stream));
 }
 
 size_t fa_mask_build_workspace_bytes(const fa_mask_build* m) {

@@ -1,0 +1,63 @@
+// Instantiations and launches of the kernels around a KV cache: rotary
+// positions, appends, and decode over an e4m3 cache.
+#include "launch.h"
+
+namespace fa {
+
+static unsigned rotary_threads(const RotaryArgs& a) { return (unsigned)a.B * a.groups * a.units * a.T; }
+
+int launch_rotary(const RotaryArgs& a, bool f32, bool vec, hipStream_t s) {
+  const dim3 grid((rotary_threads(a) + 255) / 256);
+  if (f32) {
+    if (vec) hipLaunchKernelGGL((rotary_kernel<float, true>), grid, dim3(256), 0, s, a);
+    else hipLaunchKernelGGL((rotary_kernel<float, false>), grid, dim3(256), 0, s, a);
+  } else {
+    if (vec) hipLaunchKernelGGL((rotary_kernel<uint16_t, true>), grid, dim3(256), 0, s, a);
+    else hipLaunchKernelGGL((rotary_kernel<uint16_t, false>), grid, dim3(256), 0, s, a);
+  }
+  return launch_status();
+}
+
+template <int D>
+static void run_append(const AppendArgs& a, bool fp8, hipStream_t s) {
+  const unsigned turns = a.q.units ? (rotary_threads(a.q) + 2 * D - 1) / (2 * D) : 0;
+  const dim3 grid(a.kv_blocks + turns), block(2 * D);
+  if (fp8) hipLaunchKernelGGL((kv_append_kernel<D, true>), grid, block, 0, s, a);
+  else hipLaunchKernelGGL((kv_append_kernel<D, false>), grid, block, 0, s, a);
+}
+
+int launch_append(const AppendArgs& a, int D, bool fp8, hipStream_t s) {
+  switch (D) {
+    case 32: run_append<32>(a, fp8, s); break;
+    case 64: run_append<64>(a, fp8, s); break;
+    case 128: run_append<128>(a, fp8, s); break;
+    default: return FA_ERR_UNSUPPORTED;
+  }
+  return launch_status();
+}
+
+template <int D, int NQ, bool M>
+static void run_decode(const DecodeArgs& a, hipStream_t s) {
+  hipLaunchKernelGGL((decode_fp8_kernel<D, NQ, M>), dim3(a.wgs), dim3(256), 0, s, a);
+}
+
+template <int D, bool M>
+static void decode_nq(const DecodeArgs& a, int nq, hipStream_t s) {
+  if (nq == 1) run_decode<D, 1, M>(a, s);
+  else if (nq == 2) run_decode<D, 2, M>(a, s);
+  else run_decode<D, 4, M>(a, s);
+  const int rows = a.B * a.Hkv * a.g * a.Sq;
+  hipLaunchKernelGGL((decode_fp8_merge<D>), dim3(cdiv(rows, 4)), dim3(256), 0, s, a, 16 * nq);
+}
+
+int launch_decode_fp8(const DecodeArgs& a, int D, int nq, bool mods, hipStream_t s) {
+  switch (D) {
+    case 32: mods ? decode_nq<32, true>(a, nq, s) : decode_nq<32, false>(a, nq, s); break;
+    case 64: mods ? decode_nq<64, true>(a, nq, s) : decode_nq<64, false>(a, nq, s); break;
+    case 128: mods ? decode_nq<128, true>(a, nq, s) : decode_nq<128, false>(a, nq, s); break;
+    default: return FA_ERR_UNSUPPORTED;
+  }
+  return launch_status();
+}
+
+}  // namespace fa

@@ -7,8 +7,10 @@
 
 #include "../../include/flexattn.h"
 #include "bwd.h"
+#include "decode_fp8.h"
 #include "fwd.h"
 #include "fwd_fp8.h"
+#include "kv_append.h"
 #include "problem.h"
 
 namespace fa {
@@ -31,5 +33,12 @@ int launch_delta(const BwdArgs& a, hipStream_t s);  // Delta = rowsum(dO * O)
 // quantiser (kernels_fp8.hip); q16: Q is bf16, quantised in the kernel
 int launch_fwd_fp8(const Fp8FwdArgs& a, int D, bool mods, bool q16, hipStream_t s);
 int launch_quant_fp8(const QuantArgs& a, hipStream_t s);
+
+// Around a KV cache (kernels_cache.hip): rotary positions (f32 or bf16; vec:
+// 16-byte accesses), appends (D = 32, 64 or 128) and decode over e4m3 pages
+// (nq: 16-row query blocks per work item, 1, 2 or 4)
+int launch_rotary(const RotaryArgs& a, bool f32, bool vec, hipStream_t s);
+int launch_append(const AppendArgs& a, int D, bool fp8, hipStream_t s);
+int launch_decode_fp8(const DecodeArgs& a, int D, int nq, bool mods, hipStream_t s);
 
 }  // namespace fa

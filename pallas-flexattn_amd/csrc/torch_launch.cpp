@@ -4,6 +4,9 @@
 // conversions for every pointer.  Host code only; the C ABI's entry points are
 // handed over by address (bind), so it links against torch alone.
 //
+// The calls around a KV cache (rotary, append, decode over e4m3 pages) are checked here
+// too: their struct arguments are filled from the tensors' own shapes and strides.
+//
 // Why: a small training step is bound by the host.  At B2 H4 S300 D64 the
 // Python form of these two calls took 13 us (forward) and 18 us (backward; about
 // 34 on the autograd engine's thread) of a 136 us step whose kernels take 40.
@@ -13,6 +16,8 @@
 #include <ATen/ATen.h>
 
 #include <cstdint>
+
+#include "../../include/flexattn.h"
 
 namespace {
 
@@ -122,10 +127,383 @@ PyObject* py_bwd(PyObject*, PyObject* const* a, Py_ssize_t n) {
   END_HANDLE_TH_ERRORS
 }
 
+// ------------------------------------------------------ around a KV cache ----
+decltype(&fa_apply_rotary) g_rotary = nullptr;
+decltype(&fa_kv_append) g_append = nullptr;
+decltype(&fa_fwd_kvcache_fp8) g_decode = nullptr;
+decltype(&fa_fwd_kvcache_fp8_workspace_bytes) g_decode_ws = nullptr;
+
+// bind_cache(fa_apply_rotary, fa_kv_append, fa_fwd_kvcache_fp8, fa_fwd_kvcache_fp8_workspace_bytes)
+PyObject* py_bind_cache(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  if (n != 4) {
+    PyErr_SetString(PyExc_TypeError, "bind_cache takes 4 addresses");
+    return nullptr;
+  }
+  g_rotary = reinterpret_cast<decltype(g_rotary)>(address(a[0]));
+  g_append = reinterpret_cast<decltype(g_append)>(address(a[1]));
+  g_decode = reinterpret_cast<decltype(g_decode)>(address(a[2]));
+  g_decode_ws = reinterpret_cast<decltype(g_decode_ws)>(address(a[3]));
+  if (PyErr_Occurred()) return nullptr;
+  Py_RETURN_NONE;
+}
+
+#define REFUSE(type, text)          \
+  do {                              \
+    PyErr_SetString(type, text);    \
+    return nullptr;                 \
+  } while (0)
+
+// A tensor argument, or a null pointer for None; false with an exception set otherwise.
+bool optional(PyObject* x, const at::Tensor** t) {
+  *t = nullptr;
+  if (x == Py_None) return true;
+  return (*t = tensor(x)) != nullptr;
+}
+
+// (B, H, T, D) with rows that the kernels' 16-byte accesses can take as they
+// are, else a dense copy.
+bool rows_ok(const at::Tensor& t) {
+  const int64_t m = 16 / t.element_size() - 1;
+  if (t.stride(3) != 1 || (reinterpret_cast<uintptr_t>(t.const_data_ptr()) & 15)) return false;
+  for (int i = 0; i < 3; ++i)
+    if (t.size(i) > 1 && (t.stride(i) & m)) return false;
+  return true;
+}
+fa_strided strided(const at::Tensor& t) {
+  fa_strided s{};
+  s.data = t.const_data_ptr();
+  // (strides of dimensions of size one are never used: they may be anything)
+  s.stride_b = t.size(0) > 1 ? t.stride(0) : 0;
+  s.stride_h = t.size(1) > 1 ? t.stride(1) : 0;
+  s.stride_t = t.size(2) > 1 ? t.stride(2) : 0;
+  s.heads = static_cast<int32_t>(t.size(1));
+  return s;
+}
+constexpr int64_t kMaxSize = 0x7fffffff;
+bool sizes_fit(const at::Tensor& t) {
+  for (int64_t d : t.sizes())
+    if (d > kMaxSize) return false;
+  return true;
+}
+
+const char* const kFreqText = "inv_freq must be a dense float64 vector with at most head_dim / 2 entries";
+bool freq_ok(const at::Tensor& f, int64_t D) {
+  return f.dim() == 1 && f.scalar_type() == at::kDouble && f.is_contiguous() && f.size(0) >= 1 && 2 * f.size(0) <= D;
+}
+
+// A vector of one int per batch row as int32 on dev.
+at::Tensor row_ints(const at::Tensor& t, const at::Device& dev) {
+  if (t.scalar_type() == at::kInt && t.device() == dev && t.is_contiguous()) return t;
+  return t.to(dev, at::kInt).contiguous();
+}
+
+// rotary(q, k | None, inv_freq, interleaved, scale, positions | None, offset, inverse, stream)
+// -> (status, q'[, k'])
+PyObject* py_rotary(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  if (n != 9 || !g_rotary) REFUSE(PyExc_TypeError, "rotary takes 9 arguments, after bind_cache");
+  const at::Tensor *q = tensor(a[0]), *k, *pos;
+  if (!q || !optional(a[1], &k)) return nullptr;
+  const at::Tensor* f = tensor(a[2]);
+  if (!f || !optional(a[5], &pos)) return nullptr;
+  const int interleaved = PyObject_IsTrue(a[3]), inverse = PyObject_IsTrue(a[7]);
+  const double scale = PyFloat_AsDouble(a[4]);
+  const long long offset = PyLong_AsLongLong(a[6]);
+  void* stream = address(a[8]);
+  if (PyErr_Occurred()) return nullptr;
+  if (q->dim() != 4 || (k && k->dim() != 4)) REFUSE(PyExc_ValueError, "query and key must be (B, H, T, D)");
+  if (q->scalar_type() != at::kBFloat16 && q->scalar_type() != at::kFloat)
+    REFUSE(PyExc_TypeError, "apply_rotary takes bfloat16 or float32 tensors");
+  if (k && k->scalar_type() != q->scalar_type()) REFUSE(PyExc_TypeError, "query and key must share a dtype");
+  const int64_t B = q->size(0), T = q->size(2), D = q->size(3);
+  if (k && (k->size(0) != B || k->size(2) != T || k->size(3) != D))
+    REFUSE(PyExc_ValueError, "batch, length and head dim of query and key must match");
+  if (!freq_ok(*f, D)) REFUSE(PyExc_ValueError, kFreqText);
+  if (D > 1024 || !sizes_fit(*q) || (k && !sizes_fit(*k))) REFUSE(PyExc_ValueError, "head dim at most 1024, other sizes below 2^31");
+  if (pos) {
+    if (pos->scalar_type() != at::kInt && pos->scalar_type() != at::kLong)
+      REFUSE(PyExc_TypeError, "positions must be int32 or int64");
+    const bool row = pos->dim() == 1 && pos->size(0) == T;
+    if (!row && !(pos->dim() == 2 && pos->size(1) == T && (pos->size(0) == B || pos->size(0) == 1)))
+      REFUSE(PyExc_ValueError, "positions must be (T,), (1, T) or (B, T)");
+  }
+  const at::Device dev = q->device();
+  if (!dev.is_cuda()) REFUSE(PyExc_ValueError, "query and key must be GPU tensors");
+  if ((k && k->device() != dev) || f->device() != dev || (pos && pos->device() != dev))
+    REFUSE(PyExc_ValueError, "query, key, inv_freq and positions must be on one device");
+  const at::Tensor* in[2] = {q, k};
+  at::Tensor src[2], out[2], p;
+  fa_rotary_call c{};
+  c.abi_version = FA_ABI_VERSION;
+  c.dtype = q->scalar_type() == at::kFloat ? FA_DTYPE_F32 : FA_DTYPE_BF16;
+  c.B = static_cast<int32_t>(B);
+  c.T = static_cast<int32_t>(T);
+  c.D = static_cast<int32_t>(D);
+  c.inverse = inverse;
+  c.rotary.inv_freq = f->const_data_ptr<double>();
+  c.rotary.pairs = static_cast<int32_t>(f->size(0));
+  c.rotary.interleaved = interleaved;
+  c.rotary.scale = static_cast<float>(scale);
+  for (int i = 0; i < (k ? 2 : 1); ++i) {
+    out[i] = at::empty(in[i]->sizes(), in[i]->options());
+    if (in[i]->numel() == 0) continue;
+    src[i] = in[i]->stride(3) == 1 || D == 1 ? *in[i] : in[i]->contiguous();
+    c.in[c.count] = strided(src[i]);
+    c.out[c.count++] = out[i].mutable_data_ptr();
+  }
+  if (pos) {
+    p = pos->size(-1) <= 1 || pos->stride(-1) == 1 ? *pos : pos->contiguous();
+    c.positions = p.const_data_ptr();
+    c.positions_64 = p.scalar_type() == at::kLong;
+    c.positions_stride = p.dim() == 2 && p.size(0) > 1 ? p.stride(0) : 0;
+  }
+  c.offset = offset;
+  int rc = FA_OK;
+  if (c.count) {
+    Py_BEGIN_ALLOW_THREADS
+    rc = g_rotary(&c, stream);
+    Py_END_ALLOW_THREADS
+  }
+  if (!k) return Py_BuildValue("iN", rc, THPVariable_Wrap(out[0]));
+  return Py_BuildValue("iNN", rc, THPVariable_Wrap(out[0]), THPVariable_Wrap(out[1]));
+  END_HANDLE_TH_ERRORS
+}
+
+// The checks that append and decode share: the cache's tensors and tables.
+// `v8`: e4m3 with scales; sets an exception and returns false where refused.
+bool cache_ok(const at::Tensor& k, const at::Tensor& v, const at::Tensor* ks, const at::Tensor* vs, const at::Tensor* table,
+              int64_t B, int64_t D) {
+  PyObject* value = PyExc_ValueError;
+  const char* bad = nullptr;
+  const auto type = ks ? at::kFloat8_e4m3fn : at::kBFloat16;
+  if (k.scalar_type() != type || v.scalar_type() != type) {
+    value = PyExc_TypeError;
+    bad = ks ? "the cache's key and value must be float8_e4m3fn" : "the cache's key and value must be bfloat16";
+  } else if (k.dim() != 4 || k.sizes() != v.sizes()) {
+    bad = "the cache's key and value must both be (num_pages, Hkv, page_size, D)";
+  } else if (k.size(0) < 1 || k.size(1) < 1 || k.size(2) < FA_KV_RUN || k.size(2) % FA_KV_RUN) {
+    bad = "page_size must be a multiple of 32, with at least one page and head";
+  } else if (k.size(3) != D || (D != 32 && D != 64 && D != 128)) {
+    bad = "the head dim must be 32, 64 or 128, the cache's and the tokens' the same";
+  } else if (!k.is_contiguous() || !v.is_contiguous()) {
+    bad = "the cache's tensors must be contiguous";
+  } else if (!sizes_fit(k)) {
+    bad = "the cache's sizes must be below 2^31";
+  } else if (ks) {
+    const at::IntArrayRef s = ks->sizes();
+    if (ks->scalar_type() != at::kFloat || vs->scalar_type() != at::kFloat) {
+      value = PyExc_TypeError;
+      bad = "the cache's scales must be float32";
+    } else if (s.size() != 3 || s[0] != k.size(0) || s[1] != k.size(1) || s[2] != k.size(2) / FA_KV_RUN ||
+               vs->sizes() != s || !ks->is_contiguous() || !vs->is_contiguous()) {
+      bad = "the cache's scales must be dense (num_pages, Hkv, page_size / 32)";
+    }
+  }
+  if (!bad) {
+    if (!table) {
+      if (k.size(0) < B) bad = "without a page_table the cache has a page for every batch row";
+    } else if (table->dim() != 2 || table->size(0) != B || table->size(1) < 1) {
+      bad = "page_table must be (B, max_pages)";
+    } else if (table->scalar_type() != at::kInt && table->scalar_type() != at::kLong) {
+      value = PyExc_TypeError;
+      bad = "page_table must be int32 or int64";
+    }
+  }
+  if (bad) PyErr_SetString(value, bad);
+  return !bad;
+}
+bool lens_ok(const at::Tensor* t, int64_t B, const char* shape_text) {
+  if (!t) return true;
+  if (t->scalar_type() != at::kInt && t->scalar_type() != at::kLong) {
+    PyErr_SetString(PyExc_TypeError, "lengths must be int32 or int64");
+    return false;
+  }
+  if (t->dim() != 1 || t->size(0) != B) {
+    PyErr_SetString(PyExc_ValueError, shape_text);
+    return false;
+  }
+  return true;
+}
+
+// append(k cache, v cache, k scale | None, v scale | None, key, value, kv_lens, table | None, new_lens | None,
+//        inv_freq | None, interleaved, scale, query | None, stream) -> (status, query' | None)
+PyObject* py_append(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  if (n != 14 || !g_append) REFUSE(PyExc_TypeError, "append takes 14 arguments, after bind_cache");
+  const at::Tensor *kc = tensor(a[0]), *vc, *ks, *vs, *k, *v, *lens, *table, *fresh, *f, *q;
+  if (!kc || !(vc = tensor(a[1])) || !optional(a[2], &ks) || !optional(a[3], &vs) || !(k = tensor(a[4])) ||
+      !(v = tensor(a[5])) || !(lens = tensor(a[6])) || !optional(a[7], &table) || !optional(a[8], &fresh) ||
+      !optional(a[9], &f) || !optional(a[12], &q))
+    return nullptr;
+  const int interleaved = PyObject_IsTrue(a[10]);
+  const double scale = PyFloat_AsDouble(a[11]);
+  void* stream = address(a[13]);
+  if (PyErr_Occurred()) return nullptr;
+  if (k->dim() != 4 || k->sizes() != v->sizes() || (q && q->dim() != 4))
+    REFUSE(PyExc_ValueError, "key and value must both be (B, Hkv, T, D), query (B, Hq, T, D)");
+  if (k->scalar_type() != at::kBFloat16 || v->scalar_type() != at::kBFloat16 || (q && q->scalar_type() != at::kBFloat16))
+    REFUSE(PyExc_TypeError, "append_kv_cache takes bfloat16 query, key and value");
+  const int64_t B = k->size(0), T = k->size(2), D = k->size(3);
+  if (q && (q->size(0) != B || q->size(2) != T || q->size(3) != D))
+    REFUSE(PyExc_ValueError, "batch, length and head dim of query and key must match");
+  if (q && !f) REFUSE(PyExc_ValueError, "query is rotated with the keys: it needs rotary");
+  if (!cache_ok(*kc, *vc, ks, vs, table, B, D)) return nullptr;
+  if (k->size(1) != kc->size(1)) REFUSE(PyExc_ValueError, "head counts of key and cache do not match");
+  if (!lens_ok(lens, B, "kv_lens must have one entry per batch row") ||
+      !lens_ok(fresh, B, "new_lens must have one entry per batch row"))
+    return nullptr;
+  if (f && !freq_ok(*f, D)) REFUSE(PyExc_ValueError, kFreqText);
+  if (f && f->size(0) % 8) REFUSE(PyExc_ValueError, "append_kv_cache takes a rotary_dim that is a multiple of 16");
+  if (!sizes_fit(*k) || (q && !sizes_fit(*q))) REFUSE(PyExc_ValueError, "sizes must be below 2^31");
+  const at::Device dev = kc->device();
+  if (!dev.is_cuda()) REFUSE(PyExc_ValueError, "the cache must be on the GPU");
+  if (vc->device() != dev || (ks && (ks->device() != dev || vs->device() != dev)) || k->device() != dev ||
+      v->device() != dev || (q && q->device() != dev) || (f && f->device() != dev))
+    REFUSE(PyExc_ValueError, "cache, tokens and inv_freq must be on one device");
+  at::Tensor out;
+  if (q) out = at::empty(q->sizes(), q->options());
+  int rc = FA_OK;
+  if (k->numel() || (q && q->numel())) {
+    const at::Tensor kk = rows_ok(*k) ? *k : dense16(*k), vv = rows_ok(*v) ? *v : dense16(*v);
+    const at::Tensor ll = row_ints(*lens, dev);
+    at::Tensor tt, nn, qq;
+    fa_kv_append_call c{};
+    c.abi_version = FA_ABI_VERSION;
+    c.cache_dtype = ks ? FA_DTYPE_FP8_E4M3 : FA_DTYPE_BF16;
+    c.B = static_cast<int32_t>(B);
+    c.T = static_cast<int32_t>(T);
+    c.D = static_cast<int32_t>(D);
+    c.num_pages = static_cast<int32_t>(kc->size(0));
+    c.page_size = static_cast<int32_t>(kc->size(2));
+    c.max_pages = 1;
+    c.key = strided(kk);
+    c.value = strided(vv);
+    if (q && q->numel()) {
+      qq = rows_ok(*q) ? *q : dense16(*q);
+      c.query = strided(qq);
+      c.query_out = out.mutable_data_ptr();
+    }
+    c.k_cache = kc->mutable_data_ptr();
+    c.v_cache = vc->mutable_data_ptr();
+    if (ks) {
+      c.k_scale = ks->mutable_data_ptr<float>();
+      c.v_scale = vs->mutable_data_ptr<float>();
+    }
+    if (table) {
+      tt = row_ints(*table, dev);
+      c.page_table = tt.const_data_ptr<int32_t>();
+      c.max_pages = static_cast<int32_t>(tt.size(1));
+    }
+    c.kv_lens = ll.const_data_ptr<int32_t>();
+    if (fresh) {
+      nn = row_ints(*fresh, dev);
+      c.new_lens = nn.const_data_ptr<int32_t>();
+    }
+    if (f) {
+      c.rotary.inv_freq = f->const_data_ptr<double>();
+      c.rotary.pairs = static_cast<int32_t>(f->size(0));
+      c.rotary.interleaved = interleaved;
+      c.rotary.scale = static_cast<float>(scale);
+    }
+    Py_BEGIN_ALLOW_THREADS
+    rc = g_append(&c, stream);
+    Py_END_ALLOW_THREADS
+  }
+  if (!q) return Py_BuildValue("iO", rc, Py_None);
+  return Py_BuildValue("iN", rc, THPVariable_Wrap(out));
+  END_HANDLE_TH_ERRORS
+}
+
+// decode(q, k, v, k scale, v scale, kv_lens | None, table | None, q_lens | None, left, right, slopes | None,
+//        softcap, scale, gqa, stream) -> (status, o, lse)
+PyObject* py_decode(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  if (n != 15 || !g_decode) REFUSE(PyExc_TypeError, "decode takes 15 arguments, after bind_cache");
+  const at::Tensor *q = tensor(a[0]), *k, *v, *ks, *vs, *lens, *table, *ql, *slopes;
+  if (!q || !(k = tensor(a[1])) || !(v = tensor(a[2])) || !(ks = tensor(a[3])) || !(vs = tensor(a[4])) ||
+      !optional(a[5], &lens) || !optional(a[6], &table) || !optional(a[7], &ql) || !optional(a[10], &slopes))
+    return nullptr;
+  const long left = PyLong_AsLong(a[8]), right = PyLong_AsLong(a[9]);
+  const double softcap = PyFloat_AsDouble(a[11]), scale = PyFloat_AsDouble(a[12]);
+  const int gqa = PyObject_IsTrue(a[13]);
+  void* stream = address(a[14]);
+  if (PyErr_Occurred()) return nullptr;
+  if (q->dim() != 4) REFUSE(PyExc_ValueError, "query must be (B, Hq, Sq, D)");
+  if (q->scalar_type() != at::kBFloat16) REFUSE(PyExc_TypeError, "flex_decode_fp8 takes bfloat16 queries");
+  const int64_t B = q->size(0), Hq = q->size(1), Sq = q->size(2), D = q->size(3);
+  if (!cache_ok(*k, *v, ks, vs, table, B, D)) return nullptr;
+  const int64_t Hkv = k->size(1);
+  if (Hq != Hkv && !gqa) REFUSE(PyExc_ValueError, "query and cache head counts differ: pass enable_gqa=True for grouped-query attention");
+  if (Hq % Hkv) REFUSE(PyExc_ValueError, "number of q heads must be a multiple of the number of kv heads");
+  if (!lens_ok(lens, B, "kv_lens must have one entry per batch row") ||
+      !lens_ok(ql, B, "query_lens must have one entry per batch row"))
+    return nullptr;
+  if (slopes && (slopes->scalar_type() != at::kFloat || slopes->dim() != 1 || slopes->size(0) != Hq))
+    REFUSE(PyExc_ValueError, "ALiBi needs one slope per q head");
+  if (!(scale >= 0.0) || !(softcap >= 0.0)) REFUSE(PyExc_ValueError, "scale must be positive");
+  const int64_t pages = table ? table->size(1) : 1, cap = pages * k->size(2);
+  if (!sizes_fit(*q) || cap > kMaxSize) REFUSE(PyExc_ValueError, "sizes must be below 2^31");
+  const at::Device dev = q->device();
+  if (!dev.is_cuda()) REFUSE(PyExc_ValueError, "query and cache must be on the GPU");
+  if (k->device() != dev || v->device() != dev || ks->device() != dev || vs->device() != dev ||
+      (slopes && slopes->device() != dev))
+    REFUSE(PyExc_ValueError, "query and cache must be on one device");
+  const at::Tensor qq = dense16(*q);
+  at::Tensor o = at::empty(qq.sizes(), qq.options());
+  at::Tensor lse = at::empty(qq.sizes().slice(0, 3), qq.options().dtype(at::kFloat));
+  int rc = FA_OK;
+  if (qq.numel()) {
+    at::Tensor ll, tt, qn;
+    fa_params p{};
+    p.abi_version = FA_ABI_VERSION;
+    p.dtype = FA_DTYPE_FP8_E4M3;
+    p.B = static_cast<int32_t>(B);
+    p.Hq = static_cast<int32_t>(Hq);
+    p.Hkv = static_cast<int32_t>(Hkv);
+    p.Sq = static_cast<int32_t>(Sq);
+    p.Skv = static_cast<int32_t>(cap);
+    p.D = static_cast<int32_t>(D);
+    p.scale = static_cast<float>(scale);
+    p.window_left = static_cast<int32_t>(left);
+    p.window_right = static_cast<int32_t>(right);
+    p.alibi_slopes = slopes ? slopes->const_data_ptr<float>() : nullptr;
+    p.softcap = static_cast<float>(softcap);
+    fa_fp8_cache c{};
+    c.k = k->const_data_ptr();
+    c.v = v->const_data_ptr();
+    c.k_scale = ks->const_data_ptr<float>();
+    c.v_scale = vs->const_data_ptr<float>();
+    c.page_size = static_cast<int32_t>(k->size(2));
+    c.num_pages = static_cast<int32_t>(k->size(0));
+    c.max_pages = static_cast<int32_t>(pages);
+    if (table) c.page_table = (tt = row_ints(*table, dev)).const_data_ptr<int32_t>();
+    if (lens) c.kv_lens = (ll = row_ints(*lens, dev)).const_data_ptr<int32_t>();
+    if (ql) c.q_lens = (qn = row_ints(*ql, dev)).const_data_ptr<int32_t>();
+    const size_t bytes = g_decode_ws(&p, &c);
+    at::Tensor ws = at::empty({static_cast<int64_t>(bytes < 256 ? 256 : bytes)}, qq.options().dtype(at::kByte));
+    const void* qp = qq.const_data_ptr();
+    void *op = o.mutable_data_ptr(), *wp = ws.mutable_data_ptr();
+    float* lp = lse.mutable_data_ptr<float>();
+    Py_BEGIN_ALLOW_THREADS
+    rc = g_decode(&p, &c, qp, op, lp, wp, bytes, stream);
+    Py_END_ALLOW_THREADS
+  }
+  return Py_BuildValue("iNN", rc, THPVariable_Wrap(o), THPVariable_Wrap(lse));
+  END_HANDLE_TH_ERRORS
+}
+
+PyCFunction fast(PyObject* (*f)(PyObject*, PyObject* const*, Py_ssize_t)) {
+  return reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)(void)>(f));
+}
+
 PyMethodDef methods[] = {
     {"bind", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)(void)>(py_bind)), METH_FASTCALL, nullptr},
     {"fwd", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)(void)>(py_fwd)), METH_FASTCALL, nullptr},
     {"bwd", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)(void)>(py_bwd)), METH_FASTCALL, nullptr},
+    {"bind_cache", fast(py_bind_cache), METH_FASTCALL, nullptr},
+    {"rotary", fast(py_rotary), METH_FASTCALL, nullptr},
+    {"append", fast(py_append), METH_FASTCALL, nullptr},
+    {"decode", fast(py_decode), METH_FASTCALL, nullptr},
     {nullptr, nullptr, 0, nullptr}};
 
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_launch", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};

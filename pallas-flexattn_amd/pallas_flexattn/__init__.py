@@ -39,6 +39,8 @@ from pallas_flexattn.block_mask import (
     create_sliding_window_block_mask,
 )
 from pallas_flexattn.fp8 import Fp8Tensor, dequantize_fp8, flex_attention_fp8, quantize_fp8
+from pallas_flexattn.rotary import Rotary, apply_rotary, rotary_embedding
+from pallas_flexattn.kv_cache import Fp8KVCache, append_kv_cache, create_fp8_kv_cache, flex_decode_fp8
 from pallas_flexattn.kernel_tuner import (
     get_optimal_params,
     get_kernel_config,
@@ -71,6 +73,13 @@ __all__ = [
     "quantize_fp8",
     "dequantize_fp8",
     "Fp8Tensor",
+    "Rotary",
+    "rotary_embedding",
+    "apply_rotary",
+    "Fp8KVCache",
+    "create_fp8_kv_cache",
+    "append_kv_cache",
+    "flex_decode_fp8",
     "flash_attention_bwd_preprocess",
     "flash_attention_bwd_dkv",
     "flash_attention_bwd_dq",

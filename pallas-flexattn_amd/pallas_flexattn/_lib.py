@@ -72,6 +72,41 @@ class FaFp8Inputs(ctypes.Structure):
                 ("q_scale", _pf), ("k_scale", _pf), ("v_scale", _pf)]
 
 
+class FaRotary(ctypes.Structure):
+    """Mirror of ``struct fa_rotary`` (include/flexattn.h)."""
+    _fields_ = [("inv_freq", ctypes.c_void_p), ("pairs", _i32), ("interleaved", _i32), ("scale", ctypes.c_float)]
+
+
+class FaStrided(ctypes.Structure):
+    """Mirror of ``struct fa_strided`` (include/flexattn.h)."""
+    _fields_ = [("data", ctypes.c_void_p), ("stride_b", ctypes.c_int64), ("stride_h", ctypes.c_int64),
+                ("stride_t", ctypes.c_int64), ("heads", _i32)]
+
+
+class FaRotaryCall(ctypes.Structure):
+    """Mirror of ``struct fa_rotary_call`` (include/flexattn.h)."""
+    _fields_ = [("abi_version", _i32), ("dtype", _i32), ("B", _i32), ("T", _i32), ("D", _i32), ("inverse", _i32),
+                ("rotary", FaRotary), ("count", _i32), ("in_", FaStrided * 2), ("out", ctypes.c_void_p * 2),
+                ("positions", ctypes.c_void_p), ("positions_64", _i32), ("positions_stride", ctypes.c_int64),
+                ("offset", ctypes.c_int64)]
+
+
+class FaKvAppendCall(ctypes.Structure):
+    """Mirror of ``struct fa_kv_append_call`` (include/flexattn.h)."""
+    _fields_ = [("abi_version", _i32), ("cache_dtype", _i32), ("B", _i32), ("T", _i32), ("D", _i32),
+                ("page_size", _i32), ("max_pages", _i32), ("num_pages", _i32), ("key", FaStrided),
+                ("value", FaStrided), ("query", FaStrided), ("query_out", ctypes.c_void_p),
+                ("k_cache", ctypes.c_void_p), ("v_cache", ctypes.c_void_p), ("k_scale", _pf), ("v_scale", _pf),
+                ("page_table", _pi32), ("kv_lens", _pi32), ("new_lens", _pi32), ("rotary", FaRotary)]
+
+
+class FaFp8Cache(ctypes.Structure):
+    """Mirror of ``struct fa_fp8_cache`` (include/flexattn.h)."""
+    _fields_ = [("k", ctypes.c_void_p), ("v", ctypes.c_void_p), ("k_scale", _pf), ("v_scale", _pf),
+                ("page_table", _pi32), ("page_size", _i32), ("max_pages", _i32), ("num_pages", _i32),
+                ("kv_lens", _pi32), ("q_lens", _pi32)]
+
+
 EXPORTED = ("fa_fwd", "fa_fwd_fp8", "fa_fwd_fp8_q16", "fa_quantize_fp8", "fa_quantize_fp8_kv", "fa_fwd_host", "fa_bwd_preprocess_host", "fa_bwd_dkdv_host",
             "fa_bwd_dq_host", "fa_bwd_host", "fa_fwd_splitkv", "fa_fwd_splitkv_workspace_bytes", "fa_fwd_kvcache",
             "fa_fwd_kvcache_workspace_bytes", "fa_bwd", "fa_bwd_workspace_bytes", "fa_bwd_split",
@@ -79,7 +114,8 @@ EXPORTED = ("fa_fwd", "fa_fwd_fp8", "fa_fwd_fp8_q16", "fa_quantize_fp8", "fa_qua
             "fa_bwd_noalloc", "fa_bwd_noalloc_max_rows", "fa_bwd_preprocess", "fa_bwd_dkdv", "fa_bwd_dq",
             "fa_mask_build_workspace_bytes", "fa_build_block_mask", "fa_strerror", "fa_abi_version",
             "fa_mods_compile", "fa_mods_free_blob", "fa_mods_load", "fa_mods_unload", "fa_mods_fwd", "fa_mods_bwd",
-            "fa_mods_bwd_dkdv", "fa_mods_bwd_dq", "fa_mods_source_hash")
+            "fa_mods_bwd_dkdv", "fa_mods_bwd_dq", "fa_mods_source_hash",
+            "fa_apply_rotary", "fa_kv_append", "fa_fwd_kvcache_fp8", "fa_fwd_kvcache_fp8_workspace_bytes")
 
 MODS_MASK, MODS_SCORE, MODS_BUILTIN_SCORE, MODS_GENERAL = 1, 2, 4, 8
 
@@ -170,6 +206,15 @@ def load():
     lib.fa_mods_bwd_dkdv.restype = i
     lib.fa_mods_bwd_dq.argtypes = [v, P, v, i, v, v, v, v, v, v, v, v]
     lib.fa_mods_bwd_dq.restype = i
+    lib.fa_apply_rotary.argtypes = [ctypes.POINTER(FaRotaryCall), v]
+    lib.fa_apply_rotary.restype = i
+    lib.fa_kv_append.argtypes = [ctypes.POINTER(FaKvAppendCall), v]
+    lib.fa_kv_append.restype = i
+    FC = ctypes.POINTER(FaFp8Cache)
+    lib.fa_fwd_kvcache_fp8.argtypes = [P, FC, v, v, v, v, ctypes.c_size_t, v]
+    lib.fa_fwd_kvcache_fp8.restype = i
+    lib.fa_fwd_kvcache_fp8_workspace_bytes.argtypes = [P, FC]
+    lib.fa_fwd_kvcache_fp8_workspace_bytes.restype = ctypes.c_size_t
     lib.fa_strerror.argtypes = [ctypes.c_int]
     lib.fa_strerror.restype = ctypes.c_char_p
     lib.fa_mods_source_hash.argtypes = []
@@ -202,6 +247,8 @@ def launcher():
                                 f"(pallas-flexattn_amd/build.py): {e}") from e
         ext.bind(*(ctypes.cast(f, ctypes.c_void_p).value for f in (lib.fa_fwd, lib.fa_bwd_split,
                                                                             lib.fa_bwd_split_workspace_bytes)))
+        ext.bind_cache(*(ctypes.cast(f, ctypes.c_void_p).value for f in (
+            lib.fa_apply_rotary, lib.fa_kv_append, lib.fa_fwd_kvcache_fp8, lib.fa_fwd_kvcache_fp8_workspace_bytes)))
         _launch = ext
     return _launch
 
