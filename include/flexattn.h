@@ -406,8 +406,8 @@ typedef struct fa_kv_append_call {
 } fa_kv_append_call;
 int fa_kv_append(const fa_kv_append_call *c, void *stream);
 
-/* Decode over a paged cache in e4m3 (p->dtype = FA_DTYPE_FP8_E4M3; q, o bf16,
- * lse float32; D = 32, 64 or 128).  Row b has kv_lens[b] keys (null: p->Skv, the
+/* Decode over a paged cache in e4m3 (p->dtype = FA_DTYPE_FP8_E4M3; q bf16 with
+ * 16-byte aligned rows, o bf16 and lse float32 dense; D = 32, 64 or 128).  Row b has kv_lens[b] keys (null: p->Skv, the
  * tokens of its page table) and its queries are the newest of them: query i of
  * q_lens[b] (null: Sq) sits at position kv_lens[b] - q_lens[b] + i, which is
  * what p's window and ALiBi refer to; queries i >= q_lens[b] give o = 0 and
@@ -425,7 +425,7 @@ typedef struct fa_fp8_cache {
   const int32_t *kv_lens, *q_lens; /* (B) or NULL */
 } fa_fp8_cache;
 size_t fa_fwd_kvcache_fp8_workspace_bytes(const fa_params *p, const fa_fp8_cache *kv);
-int fa_fwd_kvcache_fp8(const fa_params *p, const fa_fp8_cache *kv, const void *q, void *o, float *lse,
+int fa_fwd_kvcache_fp8(const fa_params *p, const fa_fp8_cache *kv, const fa_strided *q, void *o, float *lse,
                        void *workspace, size_t workspace_bytes, void *stream);
 
 /*

@@ -136,6 +136,7 @@ int append_args(const fa_kv_append_call* c, fa::AppendArgs* a) {
 
 struct DecodeLayout {
   int nq;               // 16-row query blocks per work item
+  bool stream;          // cache reads past the caches
   size_t part, ml, bytes;
 };
 
@@ -163,7 +164,10 @@ int decode_args(const fa_params* p, const fa_fp8_cache* kv, int cus, fa::DecodeA
   L->nq = rows <= 16 ? 1 : rows <= 32 ? 2 : 4;
   const long long rt = (rows + 16 * L->nq - 1) / (16 * L->nq);
   const long long items = p->B * (long long)p->Hkv * rt;
-  const long long tiles = (p->Skv + fa::kTileKeys - 1) / fa::kTileKeys;
+  // tiles that a row walks at most: all of its keys', or the window's
+  const int left = p->window_left < 0 ? -1 : p->window_left;
+  long long tiles = (p->Skv + fa::kTileKeys - 1) / fa::kTileKeys;
+  if (left >= 0) tiles = std::min(tiles, ((long long)left + p->Sq + fa::kTileKeys - 2) / fa::kTileKeys + 1);
   if (items * tiles > 0x7fffffffll - (1 << 20)) return FA_ERR_SHAPE;  // tile numbers of a call are 32 bits
   a->k = static_cast<const uint8_t*>(kv->k);
   a->v = static_cast<const uint8_t*>(kv->v);
@@ -181,18 +185,38 @@ int decode_args(const fa_params* p, const fa_fp8_cache* kv, int cus, fa::DecodeA
   a->max_pages = kv->max_pages;
   a->num_pages = kv->num_pages;
   a->cap = p->Skv;
-  a->win_left = p->window_left < 0 ? -1 : p->window_left;
+  a->win_left = left;
   a->win_right = p->window_right < 0 ? -1 : p->window_right;
   a->scale = p->scale == 0.f ? 1.0f / sqrtf((float)p->D) : p->scale;
   a->scale_log2 = a->scale * fa::kLog2e;
   a->softcap = p->softcap;
   a->alibi = p->alibi_slopes;
   a->rt = (int)rt;
-  a->least = 16;
-  const long long most = (items * tiles + a->least - 1) / a->least;  // workgroups with a chunk of their own
-  a->wgs = (int)(most < 2ll * cus ? most : 2ll * cus);
-  const size_t slots = 2 * (size_t)a->wgs * 16 * L->nq;
-  L->part = (((size_t)p->B + 2) * sizeof(int) + 255) & ~(size_t)255;
+  // How the walk is cut (csrc/decode_index.h), from the longest walk that the
+  // sizes allow; measured as GPU time per call in replayed graphs, D = 128 unless named,
+  // by item in eight waves / in pieces of four.
+  // One workgroup per item, no second launch, where walks are short (8 items of 16
+  // tiles 7.2 / 10.7 us, 128 of 34 11.4 / 14.8, at 48 about even) or where the items
+  // fill half of the units and none is very long (128 of 96 23.8 / 25.0, of 127 29.5 /
+  // 29.9, 512 of 68 37.5 / 38.8, D = 64 512 of 65 19.9 / 22.3). Pieces beyond: 8 of 126 25.6 / 13.0,
+  // 64 of 127 26.7 / 19.9, 256 rows of mixed lengths to 257 61 / 56; they lose only
+  // on many equal long rows (D = 64 256 of 513 88 / 96).
+  a->by_item = tiles <= 48 || (2 * items >= cus && tiles <= 128);
+  // Pieces of one chunk each fill the GPU with two workgroups per unit; four at D <= 64,
+  // whose tiles are half the bytes (D = 64 256 mixed to 284 42.0 / 40.6, D = 128 64 of 1024 97 / 99).
+  a->pieces = (p->D <= 64 ? 4 : 2) * cus;
+  // At least 16 tiles a piece, four per wave, so that the merge stays short (8 of 500
+  // 16.5 us, with 8 tiles 18.8); 8 where that makes at most 16 pieces (8 of 126 12.4, 11.8).
+  a->least = tiles <= 128 ? 8 : 16;
+  // A call that reads more than fits the 256 MB last-level cache beside other data
+  // reads past it (V of 64 items of 1024 tiles: 107 / 97 us, 256 mixed 61 / 56, at 100 MB
+  // even); smaller ones may find theirs there (D = 64 51 MB 14.3 / 15.2, D = 128 33 MB 14.8 / 15.7).
+  L->stream = 2ll * p->B * p->Hkv * tiles * fa::kTileKeys * p->D > 96ll << 20;
+  const long long grid = a->by_item ? items : fa::decode_grid(items, (int)tiles, a->pieces, a->least);
+  if (grid > 0x7fffffll) return FA_ERR_SHAPE;
+  a->grid = (int)grid;
+  const size_t slots = a->by_item ? 0 : (size_t)fa::decode_slots(grid, a->pieces) * 16 * L->nq;
+  L->part = ((2 * (size_t)p->B + 2) * sizeof(int) + 255) & ~(size_t)255;
   L->ml = L->part + slots * p->D * sizeof(float);
   L->bytes = L->ml + slots * 2 * sizeof(float);
   return FA_OK;

@@ -3,6 +3,7 @@
 #include <hip/hip_runtime.h>
 #include <hip/hiprtc.h>
 
+#include <algorithm>
 #include <cstdlib>
 #include <cstring>
 #include <initializer_list>
@@ -668,23 +669,26 @@ size_t fa_fwd_kvcache_fp8_workspace_bytes(const fa_params* p, const fa_fp8_cache
   return decode_args(p, kv, device_cus(), &a, &L) == FA_OK ? L.bytes : 0;
 }
 
-int fa_fwd_kvcache_fp8(const fa_params* p, const fa_fp8_cache* kv, const void* q, void* o, float* lse,
+int fa_fwd_kvcache_fp8(const fa_params* p, const fa_fp8_cache* kv, const fa_strided* q, void* o, float* lse,
                        void* workspace, size_t workspace_bytes, void* stream) {
   fa::DecodeArgs a;
   DecodeLayout L;
   const int rc = decode_args(p, kv, device_cus(), &a, &L);
   if (rc) return rc;
-  if (!q || !o || !lse) return FA_ERR_NULL;
-  if (!aligned16({q, o})) return FA_ERR_SHAPE;
+  if (!q || !q->data || !o || !lse) return FA_ERR_NULL;
+  if (q->heads != p->Hq || !rows16(*q, 2) || !aligned16({o})) return FA_ERR_SHAPE;
   if (!workspace || workspace_bytes < L.bytes || !aligned16({workspace})) return FA_ERR_WORKSPACE;
-  a.q = q;
+  a.q = q->data;
+  a.qsb = q->stride_b;
+  a.qsh = q->stride_h;
+  a.qst = q->stride_t;
   a.o = o;
   a.lse = lse;
   char* ws = static_cast<char*>(workspace);
   a.head = reinterpret_cast<int*>(ws);
   a.part = reinterpret_cast<float*>(ws + L.part);
   a.part_ml = reinterpret_cast<float*>(ws + L.ml);
-  return fa::launch_decode_fp8(a, p->D, L.nq, p->alibi_slopes != nullptr || p->softcap > 0.f,
+  return fa::launch_decode_fp8(a, p->D, L.nq, p->alibi_slopes != nullptr || p->softcap > 0.f, L.stream,
                                static_cast<hipStream_t>(stream));
 }
 

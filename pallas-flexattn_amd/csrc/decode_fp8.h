@@ -6,7 +6,7 @@
 // Bound by the reads of the cache (2 D + 1/4 bytes per key and kv head), so
 // everything is laid out for those: a wave takes 32-key tiles (4 + 4 KiB at
 // D = 128), its codes go from HBM straight into the registers that feed the
-// matrix cores, one tile ahead of the arithmetic; no LDS and no barrier inside
+// matrix cores, the next tile's as soon as this one's are used; no LDS and no barrier inside
 // the walk.  The g query heads of a kv head and their Sq queries are one block
 // of g Sq rows (rows of a group are contiguous in memory), 16 NQ rows of it per
 // work item, so the cache is read once per group.
@@ -15,12 +15,12 @@
 //   * S^T = K Q^T: A = 16 keys, lane (r, g) holds key r's bytes 64 c + 16 g + [0, 16)
 //     of every 64-byte piece c: the sum over d may run in any order, so a
 //     lane's 16 bytes are two of its k steps; B = Q rows r, the same d.
-//   * the C tile gives lane (r, g) the scores of query r and keys 16 j + 4 g + i
-//     (j: which 16 keys, i = 0..3): eight of the tile's 32 keys.  P stays in
+//   * the C tile gives lane (r, g) the scores of query r and A rows 4 g + i (i =
+//     0..3) of both 16-key halves j; row 4 g + i is key 16 j + 4 i + g.  P stays in
 //     those lanes as the B operand of O^T += V^T P^T, whose k index may name the keys
 //     in that order; the A operand then wants the same eight keys of one d.
 //   * V rows: lane (r, g) loads bytes [DV r, DV r + DV) (DV = D / 16) of its eight
-//     keys; v_perm_b32 pairs two keys' bytes, the conversion to bf16 makes the
+//     keys: an instruction reads four consecutive rows, whole cache lines; v_perm_b32 pairs two keys' bytes, the conversion to bf16 makes the
 //     operand's words.  MFMA t is then rows d = DV r + t, and a lane ends
 //     with 4 DV consecutive d of its query: 16-byte stores.
 // P goes into the product as two bf16 pieces (its value and what that
@@ -34,7 +34,8 @@
 namespace fa {
 
 struct DecodeArgs {
-  const void* q;     // (B, Hq, Sq, D) bf16
+  const void* q;     // (B, Hq, Sq, D) bf16, strides of its first three dimensions
+  long long qsb, qsh, qst;
   const uint8_t *k, *v;  // (num_pages, Hkv, page_size, D)
   const float *ks, *vs;  // (num_pages, Hkv, page_size / 32)
   const int* page_table;  // (B, max_pages); null: page b is row b's
@@ -47,9 +48,11 @@ struct DecodeArgs {
   float scale, scale_log2, softcap;
   const float* alibi;
   int rt;            // query blocks per kv head
-  int wgs, least;    // workgroups of the walk, tiles a chunk has at least
-  // workspace: [chunk, items' first tiles (B + 1)] ints, then the slots' O
-  // (2 wgs, 16 NQ, D) and (m, l) (2 wgs, 16 NQ, 2)
+  int pieces, least; // what decode_chunk takes
+  // by_item: a workgroup takes one whole item, nothing is shared.  Else the
+  // workspace holds the rows' first units and slots (2 (B + 1) ints) and the slots'
+  // O (16 NQ, D) and (m, l) (16 NQ, 2)
+  int by_item, grid;
   int* head;
   float *part, *part_ml;
 };
@@ -77,8 +80,16 @@ __device__ __forceinline__ float quad_sum(float x) {
   return pair_sum(__uint_as_float(r[0]) + __uint_as_float(r[1]));
 }
 
+// Loads of the cache.  kStream: past the caches (non-temporal), where every
+// load instruction reads whole 128-byte lines (V, and K rows of at most 64 bytes).
+template <bool kStream, typename T>
+__device__ __forceinline__ T code_load(const uint8_t* p) {
+  if constexpr (kStream) return __builtin_nontemporal_load(reinterpret_cast<const T*>(p));
+  else return *reinterpret_cast<const T*>(p);
+}
+
 // The codes of one tile, as a lane holds them.
-template <int D>
+template <int D, bool kStream>
 struct CodeTile {
   static constexpr int DV = D / 16;               // V bytes per lane and key
   static constexpr int KC = D >= 64 ? D / 64 : 1; // K pieces per key
@@ -86,386 +97,391 @@ struct CodeTile {
   static constexpr int VW = DV >= 4 ? DV / 4 : 1; // words of a V row piece
   uint32_t k[2][KC][KW];
   uint32_t v[8][VW];
-  __device__ __forceinline__ void load(const uint8_t* kp, const uint8_t* vp, int r, int g) {
+  __device__ __forceinline__ void load_k(const uint8_t* kp, int r, int g) {
 #pragma unroll
     for (int j = 0; j < 2; ++j)
 #pragma unroll
       for (int c = 0; c < KC; ++c) {
-        const uint8_t* p = kp + (16 * j + r) * D + c * 64 + g * (4 * KW);
+        const uint8_t* p = kp + (16 * j + 4 * (r & 3) + (r >> 2)) * D + c * 64 + g * (4 * KW);
         if constexpr (KW == 4) {
-          const u32x4 w = *reinterpret_cast<const u32x4*>(p);
+          const u32x4 w = code_load<kStream && KC == 1, u32x4>(p);
 #pragma unroll
           for (int x = 0; x < 4; ++x) k[j][c][x] = w[x];
         } else {
-          const u32x2 w = *reinterpret_cast<const u32x2*>(p);
+          const u32x2 w = code_load<kStream, u32x2>(p);
 #pragma unroll
           for (int x = 0; x < 2; ++x) k[j][c][x] = w[x];
         }
       }
+  }
+  __device__ __forceinline__ void load_v(const uint8_t* vp, int r, int g) {
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
-      const uint8_t* p = vp + (16 * (e >> 2) + 4 * g + (e & 3)) * D + DV * r;
+      const uint8_t* p = vp + (16 * (e >> 2) + 4 * (e & 3) + g) * D + DV * r;
       if constexpr (DV == 8) {
-        const u32x2 w = *reinterpret_cast<const u32x2*>(p);
+        const u32x2 w = code_load<kStream, u32x2>(p);
         v[e][0] = w[0];
         v[e][1] = w[1];
       } else if constexpr (DV == 4) {
-        v[e][0] = *reinterpret_cast<const uint32_t*>(p);
+        v[e][0] = code_load<kStream, uint32_t>(p);
       } else {
-        v[e][0] = *reinterpret_cast<const uint16_t*>(p);
+        v[e][0] = code_load<kStream, uint16_t>(p);
       }
     }
   }
-  __device__ __forceinline__ void zero() {
+  __device__ __forceinline__ void zero_k() {
 #pragma unroll
     for (int j = 0; j < 2; ++j)
 #pragma unroll
       for (int c = 0; c < KC; ++c)
 #pragma unroll
         for (int x = 0; x < KW; ++x) k[j][c][x] = 0u;
-#pragma unroll
-    for (int e = 0; e < 8; ++e)
-#pragma unroll
-      for (int x = 0; x < VW; ++x) v[e][x] = 0u;
   }
 };
 
-// Prefix sums of the rows' tiles over the batch (every workgroup computes
-// them: B loads and a scan) and the row that tile `pos` lies in.
-struct DecodeWalk {
-  int total, chunk;
-  int b, start;  // row of this workgroup's first tile, that row's first tile
-};
-template <int NT>
-__device__ __forceinline__ DecodeWalk decode_walk(const DecodeArgs& a, int wg, int* sh) {
-  constexpr int NW = NT / 64;
-  const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6;
-  const int per = (a.B + NT - 1) / NT, b0 = min(tid * per, a.B), b1 = min(b0 + per, a.B);
-  const int each = a.Hkv * a.rt;
-  auto tiles = [&](int b) {
-    const int have = a.kv_lens ? clamp_len(a.kv_lens[b], a.cap) : a.cap;
-    const int ql = a.q_lens ? clamp_len(a.q_lens[b], a.Sq) : a.Sq;
-    return decode_span(have, ql, a.win_left).n * each;
-  };
-  int sum = 0;
-  for (int b = b0; b < b1; ++b) sum += tiles(b);
-  int inc = sum;
-#pragma unroll
-  for (int d = 1; d < 64; d <<= 1) {
-    const int o = __shfl_up(inc, d);
-    if (lane >= d) inc += o;
-  }
-  if (lane == 63) sh[w] = inc;
-  __syncthreads();
-  int before = 0, total = 0;
-#pragma unroll
-  for (int i = 0; i < NW; ++i) {
-    const int s = sh[i];
-    before += i < w ? s : 0;
-    total += s;
-  }
-  DecodeWalk r;
-  r.total = total;
-  r.chunk = decode_chunk(total, a.wgs, a.least);
-  const int pos = wg * r.chunk;
-  int first = before + inc - sum;  // first tile of row b0
-  if (wg == 0 && a.head) {         // for the merge
-    if (tid == 0) {
-      a.head[0] = r.chunk;
-      a.head[1 + a.B] = total;
-    }
-    int f = first;
-    for (int b = b0; b < b1; ++b) {
-      a.head[1 + b] = f;
-      f += tiles(b);
-    }
-  }
-  if (pos >= first && pos < first + sum) {
-    int b = b0;
-    for (; b < b1 - 1; ++b) {
-      const int n = tiles(b);
-      if (pos < first + n) break;
-      first += n;
-    }
-    sh[NW] = b;
-    sh[NW + 1] = first;
-  }
-  __syncthreads();
-  r.b = sh[NW];
-  r.start = sh[NW + 1];
-  return r;
+__device__ __forceinline__ int row_keys(const DecodeArgs& a, int b) {
+  return a.kv_lens ? clamp_len(a.kv_lens[b], a.cap) : a.cap;
+}
+__device__ __forceinline__ int row_queries(const DecodeArgs& a, int b) {
+  return a.q_lens ? clamp_len(a.q_lens[b], a.Sq) : a.Sq;
+}
+// inclusive sum over the lanes of a wave (DPP: no LDS round trips)
+__device__ __forceinline__ int wave_scan(int x) {
+  x += __builtin_amdgcn_update_dpp(0, x, 0x111, 0xf, 0xf, false);  // row_shr 1, 2, 4, 8
+  x += __builtin_amdgcn_update_dpp(0, x, 0x112, 0xf, 0xf, false);
+  x += __builtin_amdgcn_update_dpp(0, x, 0x114, 0xf, 0xf, false);
+  x += __builtin_amdgcn_update_dpp(0, x, 0x118, 0xf, 0xf, false);
+  x += __builtin_amdgcn_update_dpp(0, x, 0x142, 0xa, 0xf, false);  // row 0 -> 1, 2 -> 3
+  x += __builtin_amdgcn_update_dpp(0, x, 0x143, 0xc, 0xf, false);  // row 1 -> 2, 3
+  return x;
 }
 
-template <int D, int NQ, bool kMods>
-__global__ __launch_bounds__(256, NQ == 4 ? 1 : 2) void decode_fp8_kernel(DecodeArgs a) {
-  constexpr int NW = 4;
-  using Tile = CodeTile<D>;
+// The piece of work of a workgroup (wave-uniform).
+struct DecodeUnit {
+  int b;                 // batch row; -1: no work left
+  int have, ql;          // its keys and queries
+  int item;              // kv head * rt + query block
+  int t0, nt, slot;      // tiles, and the slot of a part of an item (-1: all of it)
+};
+// Every wave finds its workgroup's unit by itself: the rows' lengths are read
+// by the lanes (consecutive rows per lane), two scans give the chunk and the rows' first units.
+__device__ __forceinline__ DecodeUnit decode_unit(const DecodeArgs& a, int wg, bool first_wave) {
+  const int each = a.Hkv * a.rt;
+  DecodeUnit u;
+  if (a.by_item) {
+    u.b = wg / each;
+    u.item = wg - u.b * each;
+    u.have = a.kv_lens ? clamp_len(scalar_load(a.kv_lens, u.b), a.cap) : a.cap;
+    u.ql = a.q_lens ? clamp_len(scalar_load(a.q_lens, u.b), a.Sq) : a.Sq;
+    const DecodeSpan s = decode_span(u.have, u.ql, a.win_left);
+    u.t0 = s.lo;
+    u.nt = s.n;
+    u.slot = -1;
+    return u;
+  }
+  const int lane = threadIdx.x & 63;
+  const int per = (a.B + 63) / 64, b0 = min(lane * per, a.B), b1 = min(b0 + per, a.B);
+  auto tiles = [&](int b) { return decode_span(row_keys(a, b), row_queries(a, b), a.win_left).n; };
+  int sum = 0;
+  for (int b = b0; b < b1; ++b) sum += tiles(b);
+  const int total = __builtin_amdgcn_readlane(wave_scan(sum), 63) * each;
+  const int chunk = decode_chunk(total, a.pieces, a.least);
+  int units = 0, slots = 0;
+  for (int b = b0; b < b1; ++b) {
+    const int p = decode_pieces(tiles(b), chunk) * each;
+    units += p;
+    slots += p > each ? p : 0;
+  }
+  const int iu = wave_scan(units), is = wave_scan(slots);
+  int fu = iu - units, fs = is - slots;
+  if (wg == 0 && first_wave) {  // for the merge
+    int f = fu, g = fs;
+    for (int b = b0; b < b1; ++b) {
+      const int p = decode_pieces(tiles(b), chunk) * each;
+      a.head[2 * b] = f;
+      a.head[2 * b + 1] = g;
+      f += p;
+      g += p > each ? p : 0;
+    }
+    if (lane == 63) a.head[2 * a.B] = iu;
+  }
+  // the lane whose rows hold unit wg, then the row among them
+  int b = b0, n = 0, p = 1;
+  if (wg >= fu && wg < iu) {
+    for (;; ++b) {
+      n = tiles(b);
+      p = decode_pieces(n, chunk);
+      if (wg < fu + p * each) break;
+      fu += p * each;
+      fs += p > 1 ? p * each : 0;
+    }
+  }
+  const unsigned long long mine = __ballot(wg >= fu && wg < iu);
+  if (!mine) {
+    u.b = -1;
+    return u;
+  }
+  const int src = __builtin_ctzll(mine);
+  u.b = __builtin_amdgcn_readlane(b, src);
+  p = __builtin_amdgcn_readlane(p, src);
+  n = __builtin_amdgcn_readlane(n, src);
+  const int local = wg - __builtin_amdgcn_readlane(fu, src);
+  u.have = a.kv_lens ? clamp_len(scalar_load(a.kv_lens, u.b), a.cap) : a.cap;
+  u.ql = a.q_lens ? clamp_len(scalar_load(a.q_lens, u.b), a.Sq) : a.Sq;
+  u.item = local / p;
+  const int piece = local - u.item * p;
+  const int lo = decode_piece(n, p, piece);
+  u.t0 = decode_span(u.have, u.ql, a.win_left).lo + lo;
+  u.nt = decode_piece(n, p, piece + 1) - lo;
+  u.slot = p > 1 ? __builtin_amdgcn_readlane(fs, src) + local : -1;
+  return u;
+}
+
+template <int D, int NQ, int NW, bool kMods, bool kStream>
+__global__ __launch_bounds__(64 * NW, NQ == 4 ? 1 : 2) void decode_fp8_kernel(DecodeArgs a) {
+  using Tile = CodeTile<D, kStream>;
   constexpr int DV = Tile::DV, KC = Tile::KC, KW = Tile::KW;
   constexpr int KS = D / 32;           // k steps of S
   constexpr int OP = D + 4;            // floats per staged O row
   constexpr float kLazy = 8.0f;        // a maximum may be this stale (log2): P stays under 2^8
   __shared__ __attribute__((aligned(16))) float so[NW][16][OP];
   __shared__ float sml[NW][16][2];
-  __shared__ int sh[NW + 2];
 
   const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int r = lane & 15, g4 = lane >> 4;
-  const int wg = blockIdx.x;
-  const DecodeWalk W = decode_walk<256>(a, wg, sh);
-  int pos = wg * W.chunk;
-  const int end = min(pos + W.chunk, W.total);
-  if (pos >= end) return;
-  int b = __builtin_amdgcn_readfirstlane(W.b), bstart = __builtin_amdgcn_readfirstlane(W.start);
+  const DecodeUnit u = decode_unit(a, blockIdx.x, w == 0);
+  if (u.b < 0) return;
+  const int b = u.b, have = u.have, ql = u.ql, t0 = u.t0, nt = u.nt;
+  const int hk = u.item / a.rt, qb = u.item - hk * a.rt;
   const int R = a.g * a.Sq;  // query rows of a kv head
   const float cap_inv = a.softcap > 0.f ? 1.0f / a.softcap : 0.f;
+  const int row0 = qb * (16 * NQ);
 
-  while (pos < end) {
-    const int have = a.kv_lens ? clamp_len(scalar_load(a.kv_lens, b), a.cap) : a.cap;
-    const int ql = a.q_lens ? clamp_len(scalar_load(a.q_lens, b), a.Sq) : a.Sq;
-    const DecodeSpan span = decode_span(have, ql, a.win_left);
-    const int item = (pos - bstart) / span.n;  // of this row: kv head, query block
-    const int istart = bstart + item * span.n;
-    const int hk = item / a.rt, qb = item - hk * a.rt;
-    const int t0 = span.lo + (pos - istart);
-    const int nt = min(istart + span.n, end) - pos;
-    const int row0 = qb * (16 * NQ);
+  // Q rows as B operands; rows past the group's end repeat its last one
+  // (their results are not written)
+  u32x4 qf[NQ][KS];
+  int qlo[NQ], qhi[NQ];  // keys that this lane's rows see
+  float slope[NQ];
+  int qpos[NQ];
+  const uint16_t* qp = static_cast<const uint16_t*>(a.q) + b * a.qsb + (long long)hk * a.g * a.qsh;
+#pragma unroll
+  for (int n = 0; n < NQ; ++n) {
+    const int row = min(row0 + 16 * n + r, R - 1);
+    const int hq = row / a.Sq, i = row - hq * a.Sq;
+#pragma unroll
+    for (int s = 0; s < KS; ++s) {
+      const int d = D >= 64 ? (s >> 1) * 64 + 16 * g4 + 8 * (s & 1) : 8 * g4;
+      qf[n][s] = *reinterpret_cast<const u32x4*>(qp + hq * a.qsh + i * a.qst + d);
+    }
+    qpos[n] = have - ql + i;
+    qlo[n] = a.win_left < 0 ? 0 : max(qpos[n] - a.win_left, 0);
+    qhi[n] = a.win_right < 0 ? have - 1 : (int)min((long long)have - 1, (long long)qpos[n] + a.win_right);
+    if (i >= ql) qhi[n] = -1;  // a padded query sees nothing
+    slope[n] = kMods && a.alibi ? a.alibi[hk * a.g + hq] : 0.f;
+  }
+  const int vlo = a.win_left < 0 ? 0 : max(have - ql - a.win_left, 0);  // before it no row sees a key
 
-    // Q rows as B operands; rows past the group's end repeat its last one
-    // (their results are not written)
-    u32x4 qf[NQ][KS];
-    int qlo[NQ], qhi[NQ];  // keys that this lane's rows see
-    float slope[NQ];
-    int qpos[NQ];
-    const uint16_t* qp = static_cast<const uint16_t*>(a.q) + (size_t)(b * a.Hkv + hk) * R * D;
+  f32x4 acc[NQ][DV];
+  float m[NQ], l[NQ];
+#pragma unroll
+  for (int n = 0; n < NQ; ++n) {
+    m[n] = -INFINITY;
+    l[n] = 0.f;
+#pragma unroll
+    for (int t = 0; t < DV; ++t) acc[n][t] = f32x4{0.f, 0.f, 0.f, 0.f};
+  }
+
+  // This wave's tiles: t0 + w, t0 + w + NW, ...; lane i holds run index (in
+  // runs of the cache, -1 for a bad page) and scales of the i-th of them.
+  const int mine = nt > w ? (nt - w + NW - 1) / NW : 0;
+  int run_l = 0;
+  float ks_l = 1.f, vs_l = 1.f;
+  auto table = [&](int i0) {
+    const int i = i0 + lane;
+    run_l = -1;
+    ks_l = vs_l = 1.f;
+    if (i < mine) {
+      const int t = t0 + w + NW * i;
+      const int pg = t / a.page_runs;
+      // (a row without keys walks one tile that is not there: its scale may be anything)
+      const int page = t * kTileKeys >= have || pg >= a.max_pages ? -1 : a.page_table ? a.page_table[(size_t)b * a.max_pages + pg] : b;
+      if (page >= 0 && page < a.num_pages) {
+        run_l = (page * a.Hkv + hk) * a.page_runs + (t - pg * a.page_runs);
+        ks_l = a.ks[run_l];
+        vs_l = a.vs[run_l];
+      }
+    }
+  };
+  auto code_at = [&](int i) { return (size_t)max(__builtin_amdgcn_readlane(run_l, i & 63), 0) * (kTileKeys * D); };
+  Tile x;
+  // Tile i; the next one's codes are requested as soon as this one's registers are
+  // free: its K behind the S product, its V behind the PV product.
+  auto step = [&](int i, bool more) {
+    const int run = __builtin_amdgcn_readlane(run_l, i & 63);
+    const float ksc = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(ks_l), i & 63));
+    const float vsc = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(vs_l), i & 63));
+    const int k0 = (t0 + w + NW * i) * kTileKeys;
+    const size_t next = more ? code_at(i + 1) : 0;
+    if (run < 0) x.zero_k();  // a page id outside the cache reads as zero keys
+    f32x4 s[NQ][2];
+#pragma unroll
+    for (int n = 0; n < NQ; ++n)
+#pragma unroll
+      for (int j = 0; j < 2; ++j) s[n][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int j = 0; j < 2; ++j)
+#pragma unroll
+      for (int c = 0; c < KC; ++c)
+#pragma unroll
+        for (int y = 0; y < KW / 2; ++y) {
+          const uint32_t w0 = x.k[j][c][2 * y], w1 = x.k[j][c][2 * y + 1];
+          const u32x4 kf{cvt_e4m3_lo(w0, ksc), cvt_e4m3_hi(w0, ksc), cvt_e4m3_lo(w1, ksc), cvt_e4m3_hi(w1, ksc)};
+#pragma unroll
+          for (int n = 0; n < NQ; ++n) s[n][j] = mma16(kf, qf[n][KW / 2 * c + y], s[n][j]);
+        }
+    if (more) x.load_k(a.k + next, r, g4);
+    // scores in log2 units
+    bool whole = true;
 #pragma unroll
     for (int n = 0; n < NQ; ++n) {
-      const int row = min(row0 + 16 * n + r, R - 1);
-#pragma unroll
-      for (int s = 0; s < KS; ++s) {
-        const int d = D >= 64 ? (s >> 1) * 64 + 16 * g4 + 8 * (s & 1) : 8 * g4;
-        qf[n][s] = *reinterpret_cast<const u32x4*>(qp + (size_t)row * D + d);
-      }
-      const int hq = row / a.Sq, i = row - hq * a.Sq;
-      qpos[n] = have - ql + i;
-      qlo[n] = a.win_left < 0 ? 0 : max(qpos[n] - a.win_left, 0);
-      qhi[n] = a.win_right < 0 ? have - 1 : (int)min((long long)have - 1, (long long)qpos[n] + a.win_right);
-      if (i >= ql) qhi[n] = -1;  // a padded query sees nothing
-      slope[n] = kMods && a.alibi ? a.alibi[hk * a.g + hq] : 0.f;
-    }
-    const int vlo = a.win_left < 0 ? 0 : max(have - ql - a.win_left, 0);  // before it no row sees a key
-
-    f32x4 acc[NQ][DV];
-    float m[NQ], l[NQ];
-#pragma unroll
-    for (int n = 0; n < NQ; ++n) {
-      m[n] = -INFINITY;
-      l[n] = 0.f;
-#pragma unroll
-      for (int t = 0; t < DV; ++t) acc[n][t] = f32x4{0.f, 0.f, 0.f, 0.f};
-    }
-
-    // This wave's tiles: t0 + w, t0 + w + NW, ...; lane i holds run index (in
-    // runs of the cache, -1 for a bad page) and scales of the i-th of them.
-    const int mine = nt > w ? (nt - w + NW - 1) / NW : 0;
-    int run_l = 0;
-    float ks_l = 1.f, vs_l = 1.f;
-    auto table = [&](int i0) {
-      const int i = i0 + lane;
-      run_l = -1;
-      ks_l = vs_l = 1.f;
-      if (i < mine) {
-        const int t = t0 + w + NW * i;
-        const int pg = t / a.page_runs;
-        // (a row without keys walks one tile that is not there: its scale may be anything)
-        const int page = t * kTileKeys >= have || pg >= a.max_pages ? -1 : a.page_table ? a.page_table[(size_t)b * a.max_pages + pg] : b;
-        if (page >= 0 && page < a.num_pages) {
-          run_l = (page * a.Hkv + hk) * a.page_runs + (t - pg * a.page_runs);
-          ks_l = a.ks[run_l];
-          vs_l = a.vs[run_l];
-        }
-      }
-    };
-    auto load = [&](Tile& x, int i) {
-      const int run = max(__builtin_amdgcn_readlane(run_l, i & 63), 0);
-      const size_t at = (size_t)run * (kTileKeys * D);
-      x.load(a.k + at, a.v + at, r, g4);
-    };
-    auto compute = [&](Tile& x, int i) {
-      const int run = __builtin_amdgcn_readlane(run_l, i & 63);
-      const float ksc = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(ks_l), i & 63));
-      const float vsc = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(vs_l), i & 63));
-      const int k0 = (t0 + w + NW * i) * kTileKeys;
-      if (run < 0) x.zero();  // a page id outside the cache reads as zero keys
-      // keys that no row sees may hold anything (also NaN codes): P = 0 there must meet V = 0
-      if (k0 < vlo || k0 + kTileKeys > have) {
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          const int key = k0 + 16 * (e >> 2) + 4 * g4 + (e & 3);
-          const bool ok = key >= vlo && key < have;
-#pragma unroll
-          for (int y = 0; y < Tile::VW; ++y) x.v[e][y] = ok ? x.v[e][y] : 0u;
-        }
-      }
-      f32x4 s[NQ][2];
-#pragma unroll
-      for (int n = 0; n < NQ; ++n)
-#pragma unroll
-        for (int j = 0; j < 2; ++j) s[n][j] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
       for (int j = 0; j < 2; ++j)
 #pragma unroll
-        for (int c = 0; c < KC; ++c)
-#pragma unroll
-          for (int y = 0; y < KW / 2; ++y) {
-            const uint32_t w0 = x.k[j][c][2 * y], w1 = x.k[j][c][2 * y + 1];
-            const u32x4 kf{cvt_e4m3_lo(w0, ksc), cvt_e4m3_hi(w0, ksc), cvt_e4m3_lo(w1, ksc), cvt_e4m3_hi(w1, ksc)};
-#pragma unroll
-            for (int n = 0; n < NQ; ++n) s[n][j] = mma16(kf, qf[n][KW / 2 * c + y], s[n][j]);
+        for (int i2 = 0; i2 < 4; ++i2) {
+          const float raw = s[n][j][i2];
+          if constexpr (kMods) {
+            float dsdx;
+            s[n][j][i2] = score_mods_flat(raw, a.scale, slope[n], qpos[n], k0 + 16 * j + 4 * i2 + g4, a.softcap, cap_inv,
+                                          &dsdx);
+          } else {
+            s[n][j][i2] = raw * a.scale_log2;
           }
-      // scores in log2 units
-      bool whole = true;
+        }
+      whole = whole && qlo[n] <= k0 && qhi[n] >= k0 + kTileKeys - 1;
+    }
+    if (!__all(whole)) {
 #pragma unroll
-      for (int n = 0; n < NQ; ++n) {
+      for (int n = 0; n < NQ; ++n)
 #pragma unroll
         for (int j = 0; j < 2; ++j)
 #pragma unroll
           for (int i2 = 0; i2 < 4; ++i2) {
-            const float raw = s[n][j][i2];
-            if constexpr (kMods) {
-              float dsdx;
-              s[n][j][i2] = score_mods_flat(raw, a.scale, slope[n], qpos[n], k0 + 16 * j + 4 * g4 + i2, a.softcap, cap_inv,
-                                            &dsdx);
-            } else {
-              s[n][j][i2] = raw * a.scale_log2;
-            }
+            const int key = k0 + 16 * j + 4 * i2 + g4;
+            s[n][j][i2] = key >= qlo[n] && key <= qhi[n] ? s[n][j][i2] : -INFINITY;
           }
-        whole = whole && qlo[n] <= k0 && qhi[n] >= k0 + kTileKeys - 1;
-      }
-      if (!__all(whole)) {
-#pragma unroll
-        for (int n = 0; n < NQ; ++n)
-#pragma unroll
-          for (int j = 0; j < 2; ++j)
-#pragma unroll
-            for (int i2 = 0; i2 < 4; ++i2) {
-              const int key = k0 + 16 * j + 4 * g4 + i2;
-              s[n][j][i2] = key >= qlo[n] && key <= qhi[n] ? s[n][j][i2] : -INFINITY;
-            }
-      }
-      u32x4 ph[NQ], pl[NQ];
-#pragma unroll
-      for (int n = 0; n < NQ; ++n) {
-        float mx = fmaxf(fmaxf(fmaxf(s[n][0][0], s[n][0][1]), fmaxf(s[n][0][2], s[n][0][3])),
-                         fmaxf(fmaxf(s[n][1][0], s[n][1][1]), fmaxf(s[n][1][2], s[n][1][3])));
-        if (__any(mx > m[n] + kLazy)) {
-          const float mnew = fmaxf(m[n], quad_max(mx));
-          const float alpha = m[n] == -INFINITY ? 0.f : fast_exp2(m[n] - mnew);
-          m[n] = mnew;
-          l[n] *= alpha;
-#pragma unroll
-          for (int t = 0; t < DV; ++t)
-#pragma unroll
-            for (int i2 = 0; i2 < 4; ++i2) acc[n][t][i2] *= alpha;
-        }
-        const float ref = m[n] == -INFINITY ? 0.f : m[n];
-#pragma unroll
-        for (int y = 0; y < 4; ++y) {
-          const float p0 = fast_exp2(s[n][y >> 1][2 * (y & 1)] - ref), p1 = fast_exp2(s[n][y >> 1][2 * (y & 1) + 1] - ref);
-          l[n] += p0 + p1;
-          const uint32_t hi = pack_bf16x2(p0, p1);
-          ph[n][y] = hi;
-          pl[n][y] = pack_bf16x2(p0 - bf16_lo(hi), p1 - bf16_hi(hi));
-        }
-      }
-#pragma unroll
-      for (int t2 = 0; t2 < DV / 2; ++t2) {  // d = DV r + 2 t2 and + 1
-        const int q = t2 >> 1;               // word of the row piece
-        u32x4 v0, v1;
-#pragma unroll
-        for (int y = 0; y < 4; ++y) {
-          const uint32_t w0 = x.v[2 * y][q], w1 = x.v[2 * y + 1][q];
-          const uint32_t pr = __builtin_amdgcn_perm(w1, w0, (t2 & 1) ? 0x07030602u : 0x05010400u);
-          v0[y] = cvt_e4m3_lo(pr, vsc);
-          v1[y] = cvt_e4m3_hi(pr, vsc);
-        }
-#pragma unroll
-        for (int n = 0; n < NQ; ++n) {
-          acc[n][2 * t2] = mma16(v0, ph[n], acc[n][2 * t2]);
-          acc[n][2 * t2] = mma16(v0, pl[n], acc[n][2 * t2]);
-          acc[n][2 * t2 + 1] = mma16(v1, ph[n], acc[n][2 * t2 + 1]);
-          acc[n][2 * t2 + 1] = mma16(v1, pl[n], acc[n][2 * t2 + 1]);
-        }
-      }
-    };
-    for (int i0 = 0; i0 < mine; i0 += 64) {
-      table(i0);
-      const int i1 = min(i0 + 64, mine);
-      Tile x, y;
-      load(x, i0);
-      for (int i = i0; i < i1; i += 2) {
-        if (i + 1 < i1) load(y, i + 1);
-        compute(x, i);
-        if (i + 1 < i1) {
-          if (i + 2 < i1) load(x, i + 2);
-          compute(y, i + 1);
-        }
-      }
     }
-
-    // join the waves: M = max m, L = sum l 2^(m - M), O = sum O 2^(m - M)
-    const bool full = nt == span.n;
-    const int slot = decode_slot(wg, istart, W.chunk);
+    u32x4 ph[NQ], pl[NQ];
 #pragma unroll
     for (int n = 0; n < NQ; ++n) {
-      __syncthreads();  // (the buffer's readers of the block before)
-      const float lt = quad_sum(l[n]);
-      if (g4 == 0) {
-        sml[w][r][0] = m[n];
-        sml[w][r][1] = lt;
+      float mx = fmaxf(fmaxf(fmaxf(s[n][0][0], s[n][0][1]), fmaxf(s[n][0][2], s[n][0][3])),
+                       fmaxf(fmaxf(s[n][1][0], s[n][1][1]), fmaxf(s[n][1][2], s[n][1][3])));
+      if (__any(mx > m[n] + kLazy)) {
+        const float mnew = fmaxf(m[n], quad_max(mx));
+        const float alpha = m[n] == -INFINITY ? 0.f : fast_exp2(m[n] - mnew);
+        m[n] = mnew;
+        l[n] *= alpha;
+#pragma unroll
+        for (int t = 0; t < DV; ++t)
+#pragma unroll
+          for (int i2 = 0; i2 < 4; ++i2) acc[n][t][i2] *= alpha;
       }
-      // lane (r, g4): d = 4 DV g4 + DV i + t
+      const float ref = m[n] == -INFINITY ? 0.f : m[n];
 #pragma unroll
-      for (int i = 0; i < 4; ++i)
-#pragma unroll
-        for (int t = 0; t < DV; ++t) so[w][r][4 * DV * g4 + DV * i + t] = acc[n][t][i];
-      __syncthreads();
-      const int orow = tid >> 4, d0 = (tid & 15) * DV;
-      const int row = row0 + 16 * n + orow;
-      if (row < R) {
-        float M = sml[0][orow][0];
-#pragma unroll
-        for (int i = 1; i < NW; ++i) M = fmaxf(M, sml[i][orow][0]);
-        const float ref = M == -INFINITY ? 0.f : M;
-        float L = 0.f, x[DV];
-#pragma unroll
-        for (int t = 0; t < DV; ++t) x[t] = 0.f;
-#pragma unroll
-        for (int i = 0; i < NW; ++i) {
-          const float c = fast_exp2(sml[i][orow][0] - ref);
-          L = fmaf(sml[i][orow][1], c, L);
-#pragma unroll
-          for (int t = 0; t < DV; ++t) x[t] = fmaf(so[i][orow][d0 + t], c, x[t]);
-        }
-        if (full) {
-          const size_t at = (size_t)(b * a.Hkv + hk) * R + row;
-          const float inv = L > 0.f ? 1.0f / L : (L == 0.f ? 0.f : L);  // (NaN is passed on)
-          uint16_t* o = static_cast<uint16_t*>(a.o) + at * D + d0;
-#pragma unroll
-          for (int t = 0; t < DV; t += 2)
-            *reinterpret_cast<uint32_t*>(o + t) = pack_bf16x2(x[t] * inv, x[t + 1] * inv);
-          if ((tid & 15) == 0) a.lse[at] = L == 0.f ? -INFINITY : (M + log2f(L)) * kLn2;
-        } else {
-          const size_t at = (size_t)slot * (16 * NQ) + 16 * n + orow;
-#pragma unroll
-          for (int t = 0; t < DV; ++t) a.part[at * D + d0 + t] = x[t];
-          if ((tid & 15) == 0) *reinterpret_cast<float2*>(a.part_ml + at * 2) = make_float2(M, L);
-        }
+      for (int y = 0; y < 4; ++y) {
+        const float p0 = fast_exp2(s[n][y >> 1][2 * (y & 1)] - ref), p1 = fast_exp2(s[n][y >> 1][2 * (y & 1) + 1] - ref);
+        l[n] += p0 + p1;
+        const uint32_t hi = pack_bf16x2(p0, p1);
+        ph[n][y] = hi;
+        pl[n][y] = pack_bf16x2(p0 - bf16_lo(hi), p1 - bf16_hi(hi));
       }
     }
-    pos += nt;
-    if (pos < end && pos >= bstart + span.n * a.Hkv * a.rt) {
-      bstart += span.n * a.Hkv * a.rt;
-      ++b;
+    // keys that no row sees may hold anything (also NaN codes): P = 0 there must meet V = 0
+    if (run < 0 || k0 < vlo || k0 + kTileKeys > have) {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const int key = k0 + 16 * (e >> 2) + 4 * (e & 3) + g4;
+        const bool ok = run >= 0 && key >= vlo && key < have;
+#pragma unroll
+        for (int y = 0; y < Tile::VW; ++y) x.v[e][y] = ok ? x.v[e][y] : 0u;
+      }
+    }
+#pragma unroll
+    for (int t2 = 0; t2 < DV / 2; ++t2) {  // d = DV r + 2 t2 and + 1
+      const int q = t2 >> 1;               // word of the row piece
+      u32x4 v0, v1;
+#pragma unroll
+      for (int y = 0; y < 4; ++y) {
+        const uint32_t w0 = x.v[2 * y][q], w1 = x.v[2 * y + 1][q];
+        const uint32_t pr = __builtin_amdgcn_perm(w1, w0, (t2 & 1) ? 0x07030602u : 0x05010400u);
+        v0[y] = cvt_e4m3_lo(pr, vsc);
+        v1[y] = cvt_e4m3_hi(pr, vsc);
+      }
+#pragma unroll
+      for (int n = 0; n < NQ; ++n) {
+        acc[n][2 * t2] = mma16(v0, ph[n], acc[n][2 * t2]);
+        acc[n][2 * t2] = mma16(v0, pl[n], acc[n][2 * t2]);
+        acc[n][2 * t2 + 1] = mma16(v1, ph[n], acc[n][2 * t2 + 1]);
+        acc[n][2 * t2 + 1] = mma16(v1, pl[n], acc[n][2 * t2 + 1]);
+      }
+    }
+    if (more) x.load_v(a.v + next, r, g4);
+  };
+  for (int i0 = 0; i0 < mine; i0 += 64) {
+    table(i0);
+    const int i1 = min(i0 + 64, mine);
+    const size_t first = code_at(i0);
+    x.load_k(a.k + first, r, g4);
+    x.load_v(a.v + first, r, g4);
+    for (int i = i0; i < i1; ++i) step(i, i + 1 < i1);
+  }
+
+  // join the waves: M = max m, L = sum l 2^(m - M), O = sum O 2^(m - M); TPR
+  // threads per row, CW columns each
+  constexpr int TPR = 4 * NW < D / 2 ? 4 * NW : D / 2, CW = D / TPR;
+#pragma unroll
+  for (int n = 0; n < NQ; ++n) {
+    if (n) __syncthreads();  // (the buffer's readers of the block before)
+    const float lt = quad_sum(l[n]);
+    if (g4 == 0) {
+      sml[w][r][0] = m[n];
+      sml[w][r][1] = lt;
+    }
+    // lane (r, g4): d = 4 DV g4 + DV i + t
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+      for (int t = 0; t < DV; ++t) so[w][r][4 * DV * g4 + DV * i + t] = acc[n][t][i];
+    __syncthreads();
+    const int orow = tid / TPR, d0 = (tid % TPR) * CW;
+    const int row = row0 + 16 * n + orow;
+    if (orow < 16 && row < R) {
+      float M = sml[0][orow][0];
+#pragma unroll
+      for (int i = 1; i < NW; ++i) M = fmaxf(M, sml[i][orow][0]);
+      const float ref = M == -INFINITY ? 0.f : M;
+      float L = 0.f, x[CW];
+#pragma unroll
+      for (int t = 0; t < CW; ++t) x[t] = 0.f;
+#pragma unroll
+      for (int i = 0; i < NW; ++i) {
+        const float c = fast_exp2(sml[i][orow][0] - ref);
+        L = fmaf(sml[i][orow][1], c, L);
+#pragma unroll
+        for (int t = 0; t < CW; ++t) x[t] = fmaf(so[i][orow][d0 + t], c, x[t]);
+      }
+      if (u.slot < 0) {
+        const size_t at = (size_t)(b * a.Hkv + hk) * R + row;
+        const float inv = L > 0.f ? 1.0f / L : (L == 0.f ? 0.f : L);  // (NaN is passed on)
+        uint16_t* o = static_cast<uint16_t*>(a.o) + at * D + d0;
+#pragma unroll
+        for (int t = 0; t < CW; t += 2) *reinterpret_cast<uint32_t*>(o + t) = pack_bf16x2(x[t] * inv, x[t + 1] * inv);
+        if (d0 == 0) a.lse[at] = L == 0.f ? -INFINITY : (M + log2f(L)) * kLn2;
+      } else {
+        const size_t at = (size_t)u.slot * (16 * NQ) + 16 * n + orow;
+#pragma unroll
+        for (int t = 0; t < CW; ++t) a.part[at * D + d0 + t] = x[t];
+        if (d0 == 0) *reinterpret_cast<float2*>(a.part_ml + at * 2) = make_float2(M, L);
+      }
     }
   }
 }
@@ -474,28 +490,37 @@ __global__ __launch_bounds__(256, NQ == 4 ? 1 : 2) void decode_fp8_kernel(Decode
 // pieces.  Lane s of 64 holds piece s's factor, the columns go over the lanes.
 template <int D>
 __global__ __launch_bounds__(256) void decode_fp8_merge(DecodeArgs a, int rows_per) {
-  constexpr int CPL = D >= 64 ? D / 64 : 1;
+  constexpr int CPL = D >= 64 ? D / 64 : 1, DEEP = 8;
   const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
   const int R = a.g * a.Sq;
   const int rows = a.B * a.Hkv * R;
   const int orow = blockIdx.x * 4 + w;
   if (orow >= rows) return;
-  const int chunk = a.head[0];
   const int bh = orow / R, row = orow - bh * R;
   const int b = bh / a.Hkv, hk = bh - b * a.Hkv;
   const int qb = row / rows_per, in = row - qb * rows_per;
-  const int f = a.head[1 + b], n = (a.head[2 + b] - f) / (a.Hkv * a.rt);
-  const int s = f + (hk * a.rt + qb) * n, e = s + n;
-  const int w0 = s / chunk, w1 = (e - 1) / chunk;
-  if (w0 == w1) return;  // one workgroup had it all
+  const int pn = (a.head[2 * b + 2] - a.head[2 * b]) / (a.Hkv * a.rt);
+  if (pn == 1) return;  // one workgroup had it all
+  const int slot = a.head[2 * b + 1] + (hk * a.rt + qb) * pn;
   const int col = lane * CPL < D ? lane * CPL : 0;
-  auto at = [&](int p) { return (size_t)(p == w0 ? decode_slot(w0, s, chunk) : 2 * p) * rows_per + in; };
+  auto at = [&](int p) { return (size_t)(slot + p) * rows_per + in; };
   float M = -INFINITY, L = 0.f, acc[CPL];
 #pragma unroll
   for (int k = 0; k < CPL; ++k) acc[k] = 0.f;
-  for (int p0 = w0; p0 <= w1; p0 += 64) {
+  for (int p0 = 0; p0 < pn; p0 += 64) {
     float2 ml = make_float2(-INFINITY, 0.f);
-    if (p0 + lane <= w1) ml = *reinterpret_cast<const float2*>(a.part_ml + at(p0 + lane) * 2);
+    if (p0 + lane < pn) ml = *reinterpret_cast<const float2*>(a.part_ml + at(p0 + lane) * 2);
+    const int np = min(64, pn - p0);
+    float x[DEEP][CPL];
+    auto load = [&](int i0) {
+#pragma unroll
+      for (int i = 0; i < DEEP; ++i) {
+        const float* p = a.part + at(p0 + min(i0 + i, np - 1)) * D + col;
+#pragma unroll
+        for (int k = 0; k < CPL; ++k) x[i][k] = p[k];
+      }
+    };
+    load(0);  // ahead of the factors
     float mx = ml.x;
 #pragma unroll
     for (int d = 32; d >= 1; d >>= 1) mx = fmaxf(mx, __shfl_xor(mx, d));
@@ -508,16 +533,8 @@ __global__ __launch_bounds__(256) void decode_fp8_merge(DecodeArgs a, int rows_p
     M = mnew;
 #pragma unroll
     for (int k = 0; k < CPL; ++k) acc[k] *= old;
-    const int np = min(64, w1 - p0 + 1);
-    constexpr int DEEP = 8;
     for (int i0 = 0; i0 < np; i0 += DEEP) {
-      float x[DEEP][CPL];
-#pragma unroll
-      for (int i = 0; i < DEEP; ++i) {
-        const float* p = a.part + at(p0 + min(i0 + i, np - 1)) * D + col;
-#pragma unroll
-        for (int k = 0; k < CPL; ++k) x[i][k] = p[k];
-      }
+      if (i0) load(i0);
 #pragma unroll
       for (int i = 0; i < DEEP; ++i) {
         const float ci = __shfl(c, (i0 + i) & 63);

@@ -3,10 +3,10 @@
 // and where the pieces of an item that several workgroups share lie.
 //
 // An item is (batch row b, kv head, block of query rows); it walks n_b tiles of
-// kRunTokens keys, from the first one that a query sees.  All items' tiles,
-// one after another (b slowest, then kv head, then query block), are cut into
-// equal chunks, one per workgroup: rows of any lengths give every workgroup
-// the same number of tiles.
+// kTileKeys keys, from the first one that a query sees. A workgroup takes one
+// item, or where an item's walk is longer than the call's chunk one of its
+// ceil(n_b / chunk) equal pieces: rows of any lengths give pieces of about the
+// same size, and no workgroup more than a chunk.
 #pragma once
 #include "index.h"
 
@@ -28,14 +28,23 @@ FA_HD DecodeSpan decode_span(int have, int ql, int left) {
 }
 FA_HD int clamp_len(int n, int most) { return n < 0 ? 0 : (n > most ? most : n); }
 
-// Tiles per chunk: `total` tiles over `wgs` workgroups, at least `least`.
-FA_HD int decode_chunk(int total, int wgs, int least) {
-  const int c = (total + wgs - 1) / wgs;
+// Tiles per chunk: `total` tiles (of all items) over `pieces` workgroups, at least `least`.
+FA_HD int decode_chunk(int total, int pieces, int least) {
+  const int c = total / pieces + (total % pieces ? 1 : 0);
   return c > least ? c : least;
 }
+FA_HD int decode_pieces(int n, int chunk) { return n / chunk + (n % chunk ? 1 : 0); }
+// Tiles [first, first + count) of piece p of an n-tile walk in `pieces`.
+FA_HD int decode_piece(int n, int pieces, int p) { return (int)((long long)n * p / pieces); }
 
-// Partial results: workgroup w keeps two slots, 2 w for the item that its
-// chunk starts in, 2 w + 1 for another one that it ends in.
-FA_HD int decode_slot(int w, int item_start, int chunk) { return 2 * w + (item_start > w * chunk ? 1 : 0); }
+// Workgroups that a call needs at most: items, plus a piece more for every
+// chunk's worth of tiles (n / chunk each, and the chunks are `pieces` in all).
+FA_HD long long decode_grid(long long items, int most_tiles, int pieces, int least) {
+  const long long each = items * decode_pieces(most_tiles, least), sum = items + pieces;
+  return each < sum ? each : sum;
+}
+// Slots for partial results: the pieces of items that have several.  Each of them is
+// longer than half a chunk, so there are fewer than 2 total / chunk.
+FA_HD long long decode_slots(long long grid, int pieces) { return grid < 2ll * pieces ? grid : 2ll * pieces; }
 
 }  // namespace fa

@@ -448,7 +448,7 @@ PyObject* py_decode(PyObject*, PyObject* const* a, Py_ssize_t n) {
   if (k->device() != dev || v->device() != dev || ks->device() != dev || vs->device() != dev ||
       (slopes && slopes->device() != dev))
     REFUSE(PyExc_ValueError, "query and cache must be on one device");
-  const at::Tensor qq = dense16(*q);
+  const at::Tensor qq = rows_ok(*q) ? *q : dense16(*q);
   at::Tensor o = at::empty(qq.sizes(), qq.options());
   at::Tensor lse = at::empty(qq.sizes().slice(0, 3), qq.options().dtype(at::kFloat));
   int rc = FA_OK;
@@ -481,11 +481,11 @@ PyObject* py_decode(PyObject*, PyObject* const* a, Py_ssize_t n) {
     if (ql) c.q_lens = (qn = row_ints(*ql, dev)).const_data_ptr<int32_t>();
     const size_t bytes = g_decode_ws(&p, &c);
     at::Tensor ws = at::empty({static_cast<int64_t>(bytes < 256 ? 256 : bytes)}, qq.options().dtype(at::kByte));
-    const void* qp = qq.const_data_ptr();
+    const fa_strided qs = strided(qq);
     void *op = o.mutable_data_ptr(), *wp = ws.mutable_data_ptr();
     float* lp = lse.mutable_data_ptr<float>();
     Py_BEGIN_ALLOW_THREADS
-    rc = g_decode(&p, &c, qp, op, lp, wp, bytes, stream);
+    rc = g_decode(&p, &c, &qs, op, lp, wp, bytes, stream);
     Py_END_ALLOW_THREADS
   }
   return Py_BuildValue("iNN", rc, THPVariable_Wrap(o), THPVariable_Wrap(lse));

@@ -211,7 +211,7 @@ def load():
     lib.fa_kv_append.argtypes = [ctypes.POINTER(FaKvAppendCall), v]
     lib.fa_kv_append.restype = i
     FC = ctypes.POINTER(FaFp8Cache)
-    lib.fa_fwd_kvcache_fp8.argtypes = [P, FC, v, v, v, v, ctypes.c_size_t, v]
+    lib.fa_fwd_kvcache_fp8.argtypes = [P, FC, ctypes.POINTER(FaStrided), v, v, v, ctypes.c_size_t, v]
     lib.fa_fwd_kvcache_fp8.restype = i
     lib.fa_fwd_kvcache_fp8_workspace_bytes.argtypes = [P, FC]
     lib.fa_fwd_kvcache_fp8_workspace_bytes.restype = ctypes.c_size_t

@@ -1,14 +1,11 @@
 // The work partition of decode over a paged cache (csrc/decode_index.h) on the
-// CPU: for many batches of lengths, windows, query blocks and workgroup counts,
-// every tile of every item is taken by exactly one workgroup, no two pieces of
-// different items share a slot, and the pieces that the merge looks for
-// are the ones that the workgroups wrote.  Prints "ok <cases> <tiles>".
+// CPU: for many batches of lengths, windows, query blocks and chunk sizes, the
+// pieces of every item cover its tiles exactly once, none is longer than the
+// chunk, the units fit the grid and the pieces of divided items the slots that
+// the host reserves.  Prints "ok <cases> <tiles>".
 #include <cstdio>
 #include <cstdlib>
-#include <map>
 #include <random>
-#include <set>
-#include <utility>
 #include <vector>
 
 #include "decode_index.h"
@@ -27,9 +24,10 @@ int main() {
   for (int it = 0; it < 4000; ++it) {
     const int B = pick(1, it % 7 == 0 ? 300 : 9), Hkv = pick(1, 5), rt = pick(1, 3), Sq = pick(1, 6);
     const int cap = it % 5 == 0 ? pick(1, 40) : pick(1, 5000), left = pick(0, 2) ? -1 : pick(0, 700);
-    const int wgs = pick(1, 512), least = pick(1, 20);
+    const int pieces = pick(1, 512), least = pick(1, 20);
     std::vector<DecodeSpan> span;
-    std::vector<int> first{0};
+    long long total = 0;
+    int most = 1;
     for (int b = 0; b < B; ++b) {
       const int have = clamp_len(pick(-3, cap + 3), cap), ql = clamp_len(pick(-1, Sq + 1), Sq);
       const DecodeSpan s = decode_span(have, ql, left);
@@ -41,49 +39,32 @@ int main() {
       }
       if (ql > 0 && have > 0 && s.lo + s.n > (have + kTileKeys - 1) / kTileKeys) fail("span past the keys", s.lo, s.n);
       span.push_back(s);
-      first.push_back(first.back() + s.n * Hkv * rt);
+      total += (long long)s.n * Hkv * rt;
+      most = imax(most, s.n);
     }
-    const int total = first.back(), chunk = decode_chunk(total, wgs, least);
-    if ((long long)chunk * wgs < total || chunk < least) fail("chunk", chunk, total);
-    std::map<int, int> slot_item;                       // slot -> item start
-    std::map<int, std::set<std::pair<int, int>>> got;   // item start -> pieces (slot, tiles)
-    std::vector<char> seen(total, 0);
-    for (int w = 0; w < wgs; ++w) {
-      int pos = w * chunk;
-      const int end = imin(pos + chunk, total);
-      if (pos >= end) continue;
-      int b = 0;
-      while (first[b + 1] <= pos) ++b;
-      while (pos < end) {
-        const DecodeSpan s = span[b];
-        const int item = (pos - first[b]) / s.n, istart = first[b] + item * s.n;
-        const int nt = imin(istart + s.n, end) - pos;
-        if (item >= Hkv * rt || nt < 1) fail("item", item, nt);
-        for (int t = pos; t < pos + nt; ++t)
-          if (seen[t]++) fail("tile twice", t, w);
-        tiles += nt;
-        if (nt != s.n) {
-          const int slot = decode_slot(w, istart, chunk);
-          if (slot < 0 || slot >= 2 * wgs) fail("slot", slot, wgs);
-          if (!slot_item.emplace(slot, istart).second) fail("slot twice", slot, w);
-          got[istart].insert({slot, nt});
-        }
-        pos += nt;
-        if (pos < end && pos >= first[b + 1]) ++b;
+    // the longest walk that the host can know of
+    int bound = (cap + kTileKeys - 1) / kTileKeys;
+    if (left >= 0) bound = imin(bound, (left + Sq + kTileKeys - 2) / kTileKeys + 1);
+    if (most > bound) fail("walk longer than the host's bound", most, bound);
+    const int chunk = decode_chunk((int)total, pieces, least);
+    if ((long long)chunk * pieces < total || chunk < least) fail("chunk", chunk, total);
+    long long units = 0, slots = 0;
+    for (int b = 0; b < B; ++b) {
+      const int n = span[b].n, p = decode_pieces(n, chunk);
+      int at = 0;
+      for (int i = 0; i < p; ++i) {
+        const int lo = decode_piece(n, p, i), hi = decode_piece(n, p, i + 1);
+        if (lo != at || hi <= lo || hi - lo > chunk) fail("piece", lo, hi);
+        at = hi;
+        tiles += hi - lo;
       }
+      if (at != n) fail("tiles left out", at, n);
+      units += (long long)p * Hkv * rt;
+      if (p > 1) slots += (long long)p * Hkv * rt;
     }
-    for (int t = 0; t < total; ++t)
-      if (!seen[t]) fail("tile left out", t, total);
-    for (int b = 0; b < B; ++b)  // as the merge looks for them
-      for (int i = 0; i < Hkv * rt; ++i) {
-        const int s = first[b] + i * span[b].n, e = s + span[b].n, w0 = s / chunk, w1 = (e - 1) / chunk;
-        std::set<int> want;
-        if (w0 != w1)
-          for (int w = w0; w <= w1; ++w) want.insert(w == w0 ? decode_slot(w0, s, chunk) : 2 * w);
-        std::set<int> have;
-        for (const auto& p : got[s]) have.insert(p.first);
-        if (have != want) fail("merge", b, i);
-      }
+    const long long grid = decode_grid((long long)B * Hkv * rt, bound, pieces, least);
+    if (units > grid) fail("more units than workgroups", units, grid);
+    if (slots > decode_slots(grid, pieces)) fail("more pieces than slots", slots, pieces);
     ++cases;
   }
   std::printf("ok %lld %lld\n", cases, tiles);

@@ -168,6 +168,13 @@ def _decode_cache(**kw):
     return c
 
 
+def _decode_q(data=16, **kw):
+    q = _lib.FaStrided(data, 256, 64, 64, 4)
+    for k, v in kw.items():
+        setattr(q, k, v)
+    return ctypes.byref(q)
+
+
 @pytest.mark.parametrize("pkw,ckw,code", [
     (dict(abi_version=9), {}, -8), (dict(dtype=0), {}, -3), (dict(D=96), {}, -4), (dict(Hq=3), {}, -2), (dict(Sq=0), {}, -2),
     (dict(Skv=129), {}, -2), (dict(softcap=-1.0), {}, -2), (dict(q_doc_ids=16), {}, -4), (dict(kv_num_blocks=16), {}, -4),
@@ -176,7 +183,7 @@ def _decode_cache(**kw):
 def test_c_decode_refuses(pkw, ckw, code):
     lib = _lib.load()
     p, c = _decode_params(**pkw), _decode_cache(**ckw)
-    assert lib.fa_fwd_kvcache_fp8(ctypes.byref(p), ctypes.byref(c), 16, 16, 16, 16, 1 << 40, None) == code
+    assert lib.fa_fwd_kvcache_fp8(ctypes.byref(p), ctypes.byref(c), _decode_q(), 16, 16, 16, 1 << 40, None) == code
     assert lib.fa_fwd_kvcache_fp8_workspace_bytes(ctypes.byref(p), ctypes.byref(c)) == 0
 
 
@@ -186,10 +193,12 @@ def test_c_decode_workspace():
     need = lib.fa_fwd_kvcache_fp8_workspace_bytes(ctypes.byref(p), ctypes.byref(c))
     assert need > 0
     call = lambda q, ws, n: lib.fa_fwd_kvcache_fp8(ctypes.byref(p), ctypes.byref(c), q, 16, 16, ws, n, None)  # noqa: E731
-    assert call(16, 16, need - 1) == -6 and call(16, None, need) == -6 and call(16, 24, need) == -6
-    assert call(None, 16, need) == -1 and call(24, 16, need) == -2
-    assert lib.fa_fwd_kvcache_fp8(None, ctypes.byref(c), 16, 16, 16, 16, need, None) == -1
-    assert lib.fa_fwd_kvcache_fp8(ctypes.byref(p), None, 16, 16, 16, 16, need, None) == -1
+    ok = _decode_q()
+    assert call(ok, 16, need - 1) == -6 and call(ok, None, need) == -6 and call(ok, 24, need) == -6
+    assert call(None, 16, need) == -1 and call(_decode_q(None), 16, need) == -1 and call(_decode_q(24), 16, need) == -2
+    assert call(_decode_q(heads=2), 16, need) == -2 and call(_decode_q(stride_h=36), 16, need) == -2
+    assert lib.fa_fwd_kvcache_fp8(None, ctypes.byref(c), ok, 16, 16, 16, need, None) == -1
+    assert lib.fa_fwd_kvcache_fp8(ctypes.byref(p), None, ok, 16, 16, 16, need, None) == -1
 
 
 @pytest.mark.parametrize("cname,pyname", [("fa_rotary", "FaRotary"), ("fa_strided", "FaStrided"),

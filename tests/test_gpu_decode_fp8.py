@@ -175,6 +175,8 @@ def test_whole_table_strides_and_no_table():
     v = q.transpose(1, 2).contiguous().transpose(1, 2)
     got = pf.flex_decode_fp8(v, c.cache, c.lens.long(), c.table.long(), enable_gqa=True)
     assert (got == want).all()
+    odd = q.new_zeros(3, 6, 2, 129)[..., 1:]  # rows that are not 16-byte aligned
+    assert (pf.flex_decode_fp8(odd.copy_(q), c.cache, c.lens, c.table, enable_gqa=True) == want).all()
     rows = [t[c.table[:, 0].long()].contiguous() for t in c.cache]
     assert (pf.flex_decode_fp8(q, pf.Fp8KVCache(*rows), [96] * 3, enable_gqa=True) == want).all()
     # slots of nobody's pages and of unused rows do not matter: garbage elsewhere changes nothing
