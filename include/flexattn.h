@@ -415,8 +415,8 @@ int fa_kv_append(const fa_kv_append_call *c, void *stream);
  * as zero keys.  Document ids and block tables are refused.  Workgroups take
  * equal shares of all rows' tiles of 32 keys; the partial results of items
  * that several of them share are joined in a fixed order by a second launch.
- * The workspace is 16-byte aligned, of the size that the other function gives
- * (0 where a call would be refused); calls that overlap in time need one each. */
+ * The workspace is 16-byte aligned, of the size that the other function gives (0:
+ * the call needs none, or would be refused); calls that overlap in time need one each. */
 typedef struct fa_fp8_cache {
   const void *k, *v;
   const float *k_scale, *v_scale;

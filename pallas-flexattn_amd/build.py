@@ -122,8 +122,9 @@ def build_launch() -> str:
            sysconfig.get_paths()["include"]]
     tmp = LAUNCH_OUT + ".tmp"
     rc, errs = _run([CXX, "-O2", "-std=c++17", "-fPIC", "-shared", f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
-                     *[f"-isystem{d}" for d in inc], LAUNCH_SRC, "-o", tmp, "-L" + lib, "-ltorch_python", "-ltorch_cpu",
-                     "-lc10", "-Wl,-rpath," + lib])
+                     "-D__HIP_PLATFORM_AMD__=1", "-DUSE_ROCM=1", *[f"-isystem{d}" for d in inc], "-isystem/opt/rocm/include",
+                     LAUNCH_SRC, "-o", tmp, "-L" + lib, "-ltorch_python", "-ltorch_cpu", "-lc10", "-lc10_hip",
+                     "-Wl,-rpath," + lib])
     if rc != 0:
         raise RuntimeError(f"compile failed on {os.path.basename(LAUNCH_SRC)} ({rc}):\n{errs}")
     os.replace(tmp, LAUNCH_OUT)

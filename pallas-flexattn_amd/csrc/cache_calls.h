@@ -218,6 +218,6 @@ int decode_args(const fa_params* p, const fa_fp8_cache* kv, int cus, fa::DecodeA
   const size_t slots = a->by_item ? 0 : (size_t)fa::decode_slots(grid, a->pieces) * 16 * L->nq;
   L->part = ((2 * (size_t)p->B + 2) * sizeof(int) + 255) & ~(size_t)255;
   L->ml = L->part + slots * p->D * sizeof(float);
-  L->bytes = L->ml + slots * 2 * sizeof(float);
+  L->bytes = a->by_item ? 0 : L->ml + slots * 2 * sizeof(float);
   return FA_OK;
 }

@@ -677,17 +677,19 @@ int fa_fwd_kvcache_fp8(const fa_params* p, const fa_fp8_cache* kv, const fa_stri
   if (rc) return rc;
   if (!q || !q->data || !o || !lse) return FA_ERR_NULL;
   if (q->heads != p->Hq || !rows16(*q, 2) || !aligned16({o})) return FA_ERR_SHAPE;
-  if (!workspace || workspace_bytes < L.bytes || !aligned16({workspace})) return FA_ERR_WORKSPACE;
+  if (L.bytes && (!workspace || workspace_bytes < L.bytes || !aligned16({workspace}))) return FA_ERR_WORKSPACE;
   a.q = q->data;
   a.qsb = q->stride_b;
   a.qsh = q->stride_h;
   a.qst = q->stride_t;
   a.o = o;
   a.lse = lse;
-  char* ws = static_cast<char*>(workspace);
-  a.head = reinterpret_cast<int*>(ws);
-  a.part = reinterpret_cast<float*>(ws + L.part);
-  a.part_ml = reinterpret_cast<float*>(ws + L.ml);
+  if (L.bytes) {
+    char* ws = static_cast<char*>(workspace);
+    a.head = reinterpret_cast<int*>(ws);
+    a.part = reinterpret_cast<float*>(ws + L.part);
+    a.part_ml = reinterpret_cast<float*>(ws + L.ml);
+  }
   return fa::launch_decode_fp8(a, p->D, L.nq, p->alibi_slopes != nullptr || p->softcap > 0.f, L.stream,
                                static_cast<hipStream_t>(stream));
 }

@@ -29,7 +29,7 @@
 #pragma once
 #include "decode_index.h"
 #include "dma.h"
-#include "kargs.h"
+#include "common.h"
 
 namespace fa {
 
@@ -78,6 +78,19 @@ __device__ __forceinline__ float quad_max(float x) {
 __device__ __forceinline__ float quad_sum(float x) {
   const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
   return pair_sum(__uint_as_float(r[0]) + __uint_as_float(r[1]));
+}
+
+// tanh to within 2.4 2^-24 of its value (the soft-cap of a small score would
+// lose what 1 - 2 / (e^2x + 1) cancels): an odd polynomial, minimax in x^2, below 0.8.
+__device__ __forceinline__ float tanh_full(float x) {
+  const float t = fabsf(x), y = x * x;
+  const float big = fmaf(-2.0f, fast_rcp(fast_exp2(t * (2.0f * kLog2e)) + 1.0f), 1.0f);
+  float p = fmaf(0.0016673924401402473f, y, -0.007573986891657114f);
+  p = fmaf(p, y, 0.02142648957669735f);
+  p = fmaf(p, y, -0.053895365446805954f);
+  p = fmaf(p, y, 0.13332898914813995f);
+  p = fmaf(p, y, -0.3333333432674408f);
+  return t < 0.8f ? fmaf(x * y, p, x) : copysignf(big, x);
 }
 
 // Loads of the cache.  kStream: past the caches (non-temporal), where every
@@ -350,9 +363,9 @@ __global__ __launch_bounds__(64 * NW, NQ == 4 ? 1 : 2) void decode_fp8_kernel(De
         for (int i2 = 0; i2 < 4; ++i2) {
           const float raw = s[n][j][i2];
           if constexpr (kMods) {
-            float dsdx;
-            s[n][j][i2] = score_mods_flat(raw, a.scale, slope[n], qpos[n], k0 + 16 * j + 4 * i2 + g4, a.softcap, cap_inv,
-                                          &dsdx);
+            float y = fmaf(slope[n], (float)(k0 + 16 * j + 4 * i2 + g4 - qpos[n]), raw * a.scale);
+            if (a.softcap > 0.f) y = a.softcap * tanh_full(y * cap_inv);
+            s[n][j][i2] = y * kLog2e;
           } else {
             s[n][j][i2] = raw * a.scale_log2;
           }

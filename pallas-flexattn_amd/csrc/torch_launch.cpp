@@ -5,15 +5,19 @@
 // handed over by address (bind), so it links against torch alone.
 //
 // The calls around a KV cache (rotary, append, decode over e4m3 pages) are checked here
-// too: their struct arguments are filled from the tensors' own shapes and strides.
+// too: their struct arguments are filled from the tensors' own shapes and strides,
+// and they run on the current stream of their tensors' device.
 //
 // Why: a small training step is bound by the host.  At B2 H4 S300 D64 the
 // Python form of these two calls took 13 us (forward) and 18 us (backward; about
 // 34 on the autograd engine's thread) of a 136 us step whose kernels take 40.
 #include <torch/csrc/Exceptions.h>
+#include <torch/csrc/autograd/custom_function.h>
 #include <torch/csrc/autograd/python_variable.h>
 
 #include <ATen/ATen.h>
+#include <c10/core/DeviceGuard.h>
+#include <c10/hip/HIPStream.h>
 
 #include <cstdint>
 
@@ -132,17 +136,19 @@ decltype(&fa_apply_rotary) g_rotary = nullptr;
 decltype(&fa_kv_append) g_append = nullptr;
 decltype(&fa_fwd_kvcache_fp8) g_decode = nullptr;
 decltype(&fa_fwd_kvcache_fp8_workspace_bytes) g_decode_ws = nullptr;
+decltype(&fa_strerror) g_strerror = nullptr;
 
-// bind_cache(fa_apply_rotary, fa_kv_append, fa_fwd_kvcache_fp8, fa_fwd_kvcache_fp8_workspace_bytes)
+// bind_cache(fa_apply_rotary, fa_kv_append, fa_fwd_kvcache_fp8, fa_fwd_kvcache_fp8_workspace_bytes, fa_strerror)
 PyObject* py_bind_cache(PyObject*, PyObject* const* a, Py_ssize_t n) {
-  if (n != 4) {
-    PyErr_SetString(PyExc_TypeError, "bind_cache takes 4 addresses");
+  if (n != 5) {
+    PyErr_SetString(PyExc_TypeError, "bind_cache takes 5 addresses");
     return nullptr;
   }
   g_rotary = reinterpret_cast<decltype(g_rotary)>(address(a[0]));
   g_append = reinterpret_cast<decltype(g_append)>(address(a[1]));
   g_decode = reinterpret_cast<decltype(g_decode)>(address(a[2]));
   g_decode_ws = reinterpret_cast<decltype(g_decode_ws)>(address(a[3]));
+  g_strerror = reinterpret_cast<decltype(g_strerror)>(address(a[4]));
   if (PyErr_Occurred()) return nullptr;
   Py_RETURN_NONE;
 }
@@ -197,19 +203,105 @@ at::Tensor row_ints(const at::Tensor& t, const at::Device& dev) {
   return t.to(dev, at::kInt).contiguous();
 }
 
-// rotary(q, k | None, inv_freq, interleaved, scale, positions | None, offset, inverse, stream)
-// -> (status, q'[, k'])
+void* stream_of(const at::Device& dev) { return c10::hip::getCurrentHIPStream(dev.index()).stream(); }
+
+struct Turn {  // how a rotary call turns, besides its tensors
+  bool interleaved, inverse;
+  double scale;
+  int64_t offset;
+};
+
+// fa_apply_rotary on checked tensors; k and pos may be undefined.
+std::vector<at::Tensor> turn(const at::Tensor& q, const at::Tensor& k, const at::Tensor& f, const at::Tensor& pos,
+                             const Turn& t) {
+  const c10::DeviceGuard guard(q.device());
+  std::vector<at::Tensor> out;
+  at::Tensor src[2], p;
+  const int64_t B = q.size(0), T = q.size(2), D = q.size(3);
+  fa_rotary_call c{};
+  c.abi_version = FA_ABI_VERSION;
+  c.dtype = q.scalar_type() == at::kFloat ? FA_DTYPE_F32 : FA_DTYPE_BF16;
+  c.B = static_cast<int32_t>(B);
+  c.T = static_cast<int32_t>(T);
+  c.D = static_cast<int32_t>(D);
+  c.inverse = t.inverse;
+  c.rotary.inv_freq = f.const_data_ptr<double>();
+  c.rotary.pairs = static_cast<int32_t>(f.size(0));
+  c.rotary.interleaved = t.interleaved;
+  c.rotary.scale = static_cast<float>(t.scale);
+  for (const at::Tensor* x : {&q, &k}) {
+    if (!x->defined()) continue;
+    out.push_back(at::empty(x->sizes(), x->options()));
+    if (x->numel() == 0) continue;
+    at::Tensor& s = src[c.count];
+    s = x->stride(3) == 1 || D == 1 ? *x : x->contiguous();
+    c.in[c.count] = strided(s);
+    c.out[c.count++] = out.back().mutable_data_ptr();
+  }
+  if (pos.defined()) {
+    p = pos.size(-1) <= 1 || pos.stride(-1) == 1 ? pos : pos.contiguous();
+    c.positions = p.const_data_ptr();
+    c.positions_64 = p.scalar_type() == at::kLong;
+    c.positions_stride = p.dim() == 2 && p.size(0) > 1 ? p.stride(0) : 0;
+  }
+  c.offset = t.offset;
+  if (c.count) {
+    const int rc = g_rotary(&c, stream_of(q.device()));
+    TORCH_CHECK(rc == FA_OK, "flexattn C ABI error ", rc, ": ", g_strerror(rc));
+  }
+  return out;
+}
+
+// The rotation as an autograd node: in Python, its two crossings of the
+// interpreter (one from the engine's thread) took 50 of 105 us at B2 H4 S300 D64.
+struct RotaryFunction : torch::autograd::Function<RotaryFunction> {
+  static torch::autograd::variable_list forward(torch::autograd::AutogradContext* ctx, const at::Tensor& q,
+                                                const std::optional<at::Tensor>& k, const at::Tensor& f,
+                                                const std::optional<at::Tensor>& pos, bool interleaved, bool inverse,
+                                                double scale, int64_t offset) {
+    ctx->set_materialize_grads(false);
+    ctx->save_for_backward({f, pos ? *pos : at::Tensor()});
+    ctx->saved_data["interleaved"] = interleaved;
+    ctx->saved_data["inverse"] = inverse;
+    ctx->saved_data["scale"] = scale;
+    ctx->saved_data["offset"] = offset;
+    return turn(q, k ? *k : at::Tensor(), f, pos ? *pos : at::Tensor(), {interleaved, inverse, scale, offset});
+  }
+  static std::optional<at::Tensor> given(const at::Tensor& t) {
+    return t.defined() ? std::optional<at::Tensor>(t) : std::nullopt;
+  }
+  // The rotation's transpose; a node again where the gradient is differentiated.
+  static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx,
+                                                 torch::autograd::variable_list g) {
+    const auto saved = ctx->get_saved_variables();
+    const Turn t{ctx->saved_data["interleaved"].toBool(), !ctx->saved_data["inverse"].toBool(),
+                 ctx->saved_data["scale"].toDouble(), ctx->saved_data["offset"].toInt()};
+    at::Tensor gq = ctx->needs_input_grad(0) ? g[0] : at::Tensor();
+    at::Tensor gk = g.size() > 1 && ctx->needs_input_grad(1) ? g[1] : at::Tensor();
+    torch::autograd::variable_list out(8);
+    if (!gq.defined() && !gk.defined()) return out;
+    const bool first = gq.defined();
+    const at::Tensor a = first ? gq : gk, b = first ? gk : at::Tensor();
+    const auto r = at::GradMode::is_enabled()
+                       ? apply(a, given(b), saved[0], given(saved[1]), t.interleaved, t.inverse, t.scale, t.offset)
+                       : turn(a, b, saved[0], saved[1], t);
+    out[first ? 0 : 1] = r[0];
+    if (r.size() > 1) out[1] = r[1];
+    return out;
+  }
+};
+
+// rotary(q, k | None, inv_freq, interleaved, scale, positions | None, offset) -> q' or (q', k'); differentiable
 PyObject* py_rotary(PyObject*, PyObject* const* a, Py_ssize_t n) {
   HANDLE_TH_ERRORS
-  if (n != 9 || !g_rotary) REFUSE(PyExc_TypeError, "rotary takes 9 arguments, after bind_cache");
+  if (n != 7 || !g_rotary) REFUSE(PyExc_TypeError, "rotary takes 7 arguments, after bind_cache");
   const at::Tensor *q = tensor(a[0]), *k, *pos;
   if (!q || !optional(a[1], &k)) return nullptr;
   const at::Tensor* f = tensor(a[2]);
   if (!f || !optional(a[5], &pos)) return nullptr;
-  const int interleaved = PyObject_IsTrue(a[3]), inverse = PyObject_IsTrue(a[7]);
+  const int interleaved = PyObject_IsTrue(a[3]);
   const double scale = PyFloat_AsDouble(a[4]);
   const long long offset = PyLong_AsLongLong(a[6]);
-  void* stream = address(a[8]);
   if (PyErr_Occurred()) return nullptr;
   if (q->dim() != 4 || (k && k->dim() != 4)) REFUSE(PyExc_ValueError, "query and key must be (B, H, T, D)");
   if (q->scalar_type() != at::kBFloat16 && q->scalar_type() != at::kFloat)
@@ -231,41 +323,15 @@ PyObject* py_rotary(PyObject*, PyObject* const* a, Py_ssize_t n) {
   if (!dev.is_cuda()) REFUSE(PyExc_ValueError, "query and key must be GPU tensors");
   if ((k && k->device() != dev) || f->device() != dev || (pos && pos->device() != dev))
     REFUSE(PyExc_ValueError, "query, key, inv_freq and positions must be on one device");
-  const at::Tensor* in[2] = {q, k};
-  at::Tensor src[2], out[2], p;
-  fa_rotary_call c{};
-  c.abi_version = FA_ABI_VERSION;
-  c.dtype = q->scalar_type() == at::kFloat ? FA_DTYPE_F32 : FA_DTYPE_BF16;
-  c.B = static_cast<int32_t>(B);
-  c.T = static_cast<int32_t>(T);
-  c.D = static_cast<int32_t>(D);
-  c.inverse = inverse;
-  c.rotary.inv_freq = f->const_data_ptr<double>();
-  c.rotary.pairs = static_cast<int32_t>(f->size(0));
-  c.rotary.interleaved = interleaved;
-  c.rotary.scale = static_cast<float>(scale);
-  for (int i = 0; i < (k ? 2 : 1); ++i) {
-    out[i] = at::empty(in[i]->sizes(), in[i]->options());
-    if (in[i]->numel() == 0) continue;
-    src[i] = in[i]->stride(3) == 1 || D == 1 ? *in[i] : in[i]->contiguous();
-    c.in[c.count] = strided(src[i]);
-    c.out[c.count++] = out[i].mutable_data_ptr();
-  }
-  if (pos) {
-    p = pos->size(-1) <= 1 || pos->stride(-1) == 1 ? *pos : pos->contiguous();
-    c.positions = p.const_data_ptr();
-    c.positions_64 = p.scalar_type() == at::kLong;
-    c.positions_stride = p.dim() == 2 && p.size(0) > 1 ? p.stride(0) : 0;
-  }
-  c.offset = offset;
-  int rc = FA_OK;
-  if (c.count) {
-    Py_BEGIN_ALLOW_THREADS
-    rc = g_rotary(&c, stream);
-    Py_END_ALLOW_THREADS
-  }
-  if (!k) return Py_BuildValue("iN", rc, THPVariable_Wrap(out[0]));
-  return Py_BuildValue("iNN", rc, THPVariable_Wrap(out[0]), THPVariable_Wrap(out[1]));
+  const at::Tensor none;
+  const bool grad = at::GradMode::is_enabled() && (q->requires_grad() || (k && k->requires_grad()));
+  const Turn t{interleaved != 0, false, scale, offset};
+  const auto out = grad ? RotaryFunction::apply(*q, RotaryFunction::given(k ? *k : none), *f,
+                                                RotaryFunction::given(pos ? *pos : none), t.interleaved, t.inverse, t.scale,
+                                                t.offset)
+                        : turn(*q, k ? *k : none, *f, pos ? *pos : none, t);
+  if (!k) return THPVariable_Wrap(out[0]);
+  return Py_BuildValue("NN", THPVariable_Wrap(out[0]), THPVariable_Wrap(out[1]));
   END_HANDLE_TH_ERRORS
 }
 
@@ -326,10 +392,10 @@ bool lens_ok(const at::Tensor* t, int64_t B, const char* shape_text) {
 }
 
 // append(k cache, v cache, k scale | None, v scale | None, key, value, kv_lens, table | None, new_lens | None,
-//        inv_freq | None, interleaved, scale, query | None, stream) -> (status, query' | None)
+//        inv_freq | None, interleaved, scale, query | None) -> (status, query' | None)
 PyObject* py_append(PyObject*, PyObject* const* a, Py_ssize_t n) {
   HANDLE_TH_ERRORS
-  if (n != 14 || !g_append) REFUSE(PyExc_TypeError, "append takes 14 arguments, after bind_cache");
+  if (n != 13 || !g_append) REFUSE(PyExc_TypeError, "append takes 13 arguments, after bind_cache");
   const at::Tensor *kc = tensor(a[0]), *vc, *ks, *vs, *k, *v, *lens, *table, *fresh, *f, *q;
   if (!kc || !(vc = tensor(a[1])) || !optional(a[2], &ks) || !optional(a[3], &vs) || !(k = tensor(a[4])) ||
       !(v = tensor(a[5])) || !(lens = tensor(a[6])) || !optional(a[7], &table) || !optional(a[8], &fresh) ||
@@ -337,7 +403,6 @@ PyObject* py_append(PyObject*, PyObject* const* a, Py_ssize_t n) {
     return nullptr;
   const int interleaved = PyObject_IsTrue(a[10]);
   const double scale = PyFloat_AsDouble(a[11]);
-  void* stream = address(a[13]);
   if (PyErr_Occurred()) return nullptr;
   if (k->dim() != 4 || k->sizes() != v->sizes() || (q && q->dim() != 4))
     REFUSE(PyExc_ValueError, "key and value must both be (B, Hkv, T, D), query (B, Hq, T, D)");
@@ -360,6 +425,7 @@ PyObject* py_append(PyObject*, PyObject* const* a, Py_ssize_t n) {
   if (vc->device() != dev || (ks && (ks->device() != dev || vs->device() != dev)) || k->device() != dev ||
       v->device() != dev || (q && q->device() != dev) || (f && f->device() != dev))
     REFUSE(PyExc_ValueError, "cache, tokens and inv_freq must be on one device");
+  const c10::DeviceGuard guard(dev);
   at::Tensor out;
   if (q) out = at::empty(q->sizes(), q->options());
   int rc = FA_OK;
@@ -405,9 +471,7 @@ PyObject* py_append(PyObject*, PyObject* const* a, Py_ssize_t n) {
       c.rotary.interleaved = interleaved;
       c.rotary.scale = static_cast<float>(scale);
     }
-    Py_BEGIN_ALLOW_THREADS
-    rc = g_append(&c, stream);
-    Py_END_ALLOW_THREADS
+    rc = g_append(&c, stream_of(dev));
   }
   if (!q) return Py_BuildValue("iO", rc, Py_None);
   return Py_BuildValue("iN", rc, THPVariable_Wrap(out));
@@ -415,10 +479,10 @@ PyObject* py_append(PyObject*, PyObject* const* a, Py_ssize_t n) {
 }
 
 // decode(q, k, v, k scale, v scale, kv_lens | None, table | None, q_lens | None, left, right, slopes | None,
-//        softcap, scale, gqa, stream) -> (status, o, lse)
+//        softcap, scale, gqa) -> (status, o, lse)
 PyObject* py_decode(PyObject*, PyObject* const* a, Py_ssize_t n) {
   HANDLE_TH_ERRORS
-  if (n != 15 || !g_decode) REFUSE(PyExc_TypeError, "decode takes 15 arguments, after bind_cache");
+  if (n != 14 || !g_decode) REFUSE(PyExc_TypeError, "decode takes 14 arguments, after bind_cache");
   const at::Tensor *q = tensor(a[0]), *k, *v, *ks, *vs, *lens, *table, *ql, *slopes;
   if (!q || !(k = tensor(a[1])) || !(v = tensor(a[2])) || !(ks = tensor(a[3])) || !(vs = tensor(a[4])) ||
       !optional(a[5], &lens) || !optional(a[6], &table) || !optional(a[7], &ql) || !optional(a[10], &slopes))
@@ -426,7 +490,6 @@ PyObject* py_decode(PyObject*, PyObject* const* a, Py_ssize_t n) {
   const long left = PyLong_AsLong(a[8]), right = PyLong_AsLong(a[9]);
   const double softcap = PyFloat_AsDouble(a[11]), scale = PyFloat_AsDouble(a[12]);
   const int gqa = PyObject_IsTrue(a[13]);
-  void* stream = address(a[14]);
   if (PyErr_Occurred()) return nullptr;
   if (q->dim() != 4) REFUSE(PyExc_ValueError, "query must be (B, Hq, Sq, D)");
   if (q->scalar_type() != at::kBFloat16) REFUSE(PyExc_TypeError, "flex_decode_fp8 takes bfloat16 queries");
@@ -448,6 +511,7 @@ PyObject* py_decode(PyObject*, PyObject* const* a, Py_ssize_t n) {
   if (k->device() != dev || v->device() != dev || ks->device() != dev || vs->device() != dev ||
       (slopes && slopes->device() != dev))
     REFUSE(PyExc_ValueError, "query and cache must be on one device");
+  const c10::DeviceGuard guard(dev);
   const at::Tensor qq = rows_ok(*q) ? *q : dense16(*q);
   at::Tensor o = at::empty(qq.sizes(), qq.options());
   at::Tensor lse = at::empty(qq.sizes().slice(0, 3), qq.options().dtype(at::kFloat));
@@ -480,13 +544,12 @@ PyObject* py_decode(PyObject*, PyObject* const* a, Py_ssize_t n) {
     if (lens) c.kv_lens = (ll = row_ints(*lens, dev)).const_data_ptr<int32_t>();
     if (ql) c.q_lens = (qn = row_ints(*ql, dev)).const_data_ptr<int32_t>();
     const size_t bytes = g_decode_ws(&p, &c);
-    at::Tensor ws = at::empty({static_cast<int64_t>(bytes < 256 ? 256 : bytes)}, qq.options().dtype(at::kByte));
+    at::Tensor ws;
+    if (bytes) ws = at::empty({static_cast<int64_t>(bytes)}, qq.options().dtype(at::kByte));
     const fa_strided qs = strided(qq);
-    void *op = o.mutable_data_ptr(), *wp = ws.mutable_data_ptr();
+    void *op = o.mutable_data_ptr(), *wp = bytes ? ws.mutable_data_ptr() : nullptr;
     float* lp = lse.mutable_data_ptr<float>();
-    Py_BEGIN_ALLOW_THREADS
-    rc = g_decode(&p, &c, &qs, op, lp, wp, bytes, stream);
-    Py_END_ALLOW_THREADS
+    rc = g_decode(&p, &c, &qs, op, lp, wp, bytes, stream_of(dev));
   }
   return Py_BuildValue("iNN", rc, THPVariable_Wrap(o), THPVariable_Wrap(lse));
   END_HANDLE_TH_ERRORS

@@ -248,7 +248,8 @@ def launcher():
         ext.bind(*(ctypes.cast(f, ctypes.c_void_p).value for f in (lib.fa_fwd, lib.fa_bwd_split,
                                                                             lib.fa_bwd_split_workspace_bytes)))
         ext.bind_cache(*(ctypes.cast(f, ctypes.c_void_p).value for f in (
-            lib.fa_apply_rotary, lib.fa_kv_append, lib.fa_fwd_kvcache_fp8, lib.fa_fwd_kvcache_fp8_workspace_bytes)))
+            lib.fa_apply_rotary, lib.fa_kv_append, lib.fa_fwd_kvcache_fp8, lib.fa_fwd_kvcache_fp8_workspace_bytes,
+            lib.fa_strerror)))
         _launch = ext
     return _launch
 

@@ -11,7 +11,7 @@ from typing import NamedTuple, Optional
 
 from . import _lib
 from .flash_attn import _resolve, _torch
-from .rotary import Rotary, _check_rotary, _on_device
+from .rotary import Rotary, _check_rotary
 
 RUN_TOKENS = 32  # tokens of a head that share a scale
 
@@ -50,8 +50,7 @@ def create_fp8_kv_cache(num_pages: int, kv_heads: int, page_size: int, head_dim:
 
 def _rows(x, like):
     """Per-row integers as a tensor (a list or array is copied to ``like``'s device)."""
-    torch = _torch()
-    return x if x is None or isinstance(x, torch.Tensor) else torch.as_tensor(x, device=like.device)
+    return x if x is None or hasattr(x, "data_ptr") else _torch().as_tensor(x, device=like.device)
 
 
 def append_kv_cache(cache, key, value, kv_lens, page_table=None, new_lens=None, rotary: Optional[Rotary] = None,
@@ -84,9 +83,8 @@ def append_kv_cache(cache, key, value, kv_lens, page_table=None, new_lens=None, 
     if rotary is not None:
         _check_rotary(rotary)
         inv_freq, inter, scale = rotary
-    rc, out = _on_device(cache[0], _lib.launcher().append, cache[0], cache[1], cache[2] if fp8 else None,
-                         cache[3] if fp8 else None, key, value, _rows(kv_lens, key), page_table,
-                         _rows(new_lens, key), inv_freq, inter, scale, query)
+    rc, out = _lib.launcher().append(cache[0], cache[1], cache[2] if fp8 else None, cache[3] if fp8 else None, key, value,
+                                     _rows(kv_lens, key), page_table, _rows(new_lens, key), inv_freq, inter, scale, query)
     if rc:
         _lib.check(rc)
     return out
@@ -122,9 +120,8 @@ def flex_decode_fp8(query, cache: Fp8KVCache, kv_lens=None, page_table=None, mas
             slopes = score.device_slopes(query.device)
     if scale is not None and not scale > 0:
         raise ValueError("scale must be positive")
-    rc, o, lse = _on_device(query, _lib.launcher().decode, query, *cache, _rows(kv_lens, query), page_table,
-                            _rows(query_lens, query), left, right, slopes, cap, 0.0 if scale is None else scale,
-                            enable_gqa)
+    rc, o, lse = _lib.launcher().decode(query, *cache, _rows(kv_lens, query), page_table, _rows(query_lens, query), left,
+                                        right, slopes, cap, 0.0 if scale is None else scale, enable_gqa)
     if rc:
         _lib.check(rc)
     return (o, lse) if return_lse else o

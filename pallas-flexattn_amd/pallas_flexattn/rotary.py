@@ -10,7 +10,7 @@ import math
 from typing import NamedTuple, Optional
 
 from . import _lib
-from .flash_attn import _stream, _torch
+from .flash_attn import _torch
 
 
 class Rotary(NamedTuple):
@@ -65,68 +65,9 @@ def rotary_embedding(rotary_dim: int, base: float = 10000.0, interleaved: bool =
     return Rotary(freq.to(device), interleaved, scale)
 
 
-def _on_device(t, fn, *args):
-    """fn(*args, stream) with t's device current, on its current stream."""
-    if not t.is_cuda:
-        return fn(*args, 0)  # the launcher says what is wrong
-    torch = _torch()
-    if t.get_device() != torch.cuda.current_device():
-        with torch.cuda.device(t.device):
-            return fn(*args, _stream())
-    return fn(*args, _stream())
-
-
 def _check_rotary(rotary):
     if not isinstance(rotary, Rotary):
         raise TypeError("rotary must be a Rotary (see rotary_embedding)")
-
-
-def _turn(q, k, rotary, positions, offset, inverse):
-    out = _on_device(q, _lib.launcher().rotary, q, k, rotary.inv_freq, rotary.interleaved, rotary.scale, positions,
-                     offset, inverse)
-    if out[0]:
-        _lib.check(out[0])
-    return out[1:]
-
-
-class _RotaryFn:
-    """torch.autograd.Function wrapper (created lazily so that importing the
-    package does not require torch)."""
-    fn = None
-
-    @classmethod
-    def get(cls):
-        if cls.fn is None:
-            torch = _torch()
-
-            class RotaryFunction(torch.autograd.Function):
-                @staticmethod
-                def forward(ctx, q, k, inv_freq, positions, cfg):
-                    # cfg: interleaved, scale, offset, inverse
-                    ctx.set_materialize_grads(False)
-                    ctx.save_for_backward(inv_freq, positions)
-                    ctx.cfg = cfg
-                    out = _turn(q, k, Rotary(inv_freq, cfg[0], cfg[1]), positions, cfg[2], cfg[3])
-                    return out if k is not None else out[0]
-
-                @staticmethod
-                def backward(ctx, gq, gk=None):
-                    # the rotation's transpose; through this Function, so that it can be differentiated again
-                    inv_freq, positions = ctx.saved_tensors
-                    gq = gq if ctx.needs_input_grad[0] else None
-                    gk = gk if ctx.needs_input_grad[1] else None
-                    inter, scale, offset, inverse = ctx.cfg
-                    cfg = (inter, scale, offset, not inverse)
-                    if gq is None and gk is None:
-                        return None, None, None, None, None
-                    if gq is None or gk is None:
-                        one = cls.fn.apply(gq if gq is not None else gk, None, inv_freq, positions, cfg)
-                        return (one, None, None, None, None) if gq is not None else (None, one, None, None, None)
-                    dq, dk = cls.fn.apply(gq, gk, inv_freq, positions, cfg)
-                    return dq, dk, None, None, None
-
-            cls.fn = RotaryFunction
-        return cls.fn
 
 
 def apply_rotary(query, key, rotary: Rotary, positions=None, offset: int = 0):
@@ -139,12 +80,7 @@ def apply_rotary(query, key, rotary: Rotary, positions=None, offset: int = 0):
     strides of the first three dimensions (a projection's (B, T, H, D) output
     transposed to (B, H, T, D) is read in place); the results are dense.  Head
     dims up to 1024, any even ``rotary_dim`` up to it; multiples of 16 take 16-byte accesses."""
-    torch = _torch()
     _check_rotary(rotary)
     if positions is not None and offset:
         raise ValueError("pass positions or an offset, not both")
-    if torch.is_grad_enabled() and (query.requires_grad or (key is not None and key.requires_grad)):
-        return _RotaryFn.get().apply(query, key, rotary.inv_freq, positions,
-                                     (rotary.interleaved, rotary.scale, offset, False))
-    out = _turn(query, key, rotary, positions, offset, False)
-    return out if key is not None else out[0]
+    return _lib.launcher().rotary(query, key, *rotary, positions, offset)

@@ -189,7 +189,7 @@ def test_c_decode_refuses(pkw, ckw, code):
 
 def test_c_decode_workspace():
     lib = _lib.load()
-    p, c = _decode_params(), _decode_cache()
+    p, c = _decode_params(Skv=1 << 20), _decode_cache(max_pages=1 << 14)
     need = lib.fa_fwd_kvcache_fp8_workspace_bytes(ctypes.byref(p), ctypes.byref(c))
     assert need > 0
     call = lambda q, ws, n: lib.fa_fwd_kvcache_fp8(ctypes.byref(p), ctypes.byref(c), q, 16, 16, ws, n, None)  # noqa: E731
@@ -197,6 +197,9 @@ def test_c_decode_workspace():
     assert call(ok, 16, need - 1) == -6 and call(ok, None, need) == -6 and call(ok, 24, need) == -6
     assert call(None, 16, need) == -1 and call(_decode_q(None), 16, need) == -1 and call(_decode_q(24), 16, need) == -2
     assert call(_decode_q(heads=2), 16, need) == -2 and call(_decode_q(stride_h=36), 16, need) == -2
+    # a walk short enough for one workgroup per item needs none
+    p1, c1 = _decode_params(), _decode_cache()
+    assert lib.fa_fwd_kvcache_fp8_workspace_bytes(ctypes.byref(p1), ctypes.byref(c1)) == 0
     assert lib.fa_fwd_kvcache_fp8(None, ctypes.byref(c), ok, 16, 16, 16, need, None) == -1
     assert lib.fa_fwd_kvcache_fp8(ctypes.byref(p), None, ok, 16, 16, 16, need, None) == -1
 
