@@ -9,26 +9,29 @@ bool rows16(const fa_strided& t, int es) {
   return aligned(t.data, 16) && !(t.stride_b & m) && !(t.stride_h & m) && !(t.stride_t & m);
 }
 
-// Heads that one thread takes its angles through: as many as leave every
-// compute unit eight workgroups of 256 threads (the angles of 8 pairs cost as much as
-// about ten heads' arithmetic, but only few tokens leave too few threads).
-int heads_per_thread(long long threads, int heads) {
-  const long long full = 8ll * 256 * device_cus();
-  long long groups = full / (threads > 0 ? threads : 1);
-  if (groups < 1) groups = 1;
-  if (groups > heads) groups = heads;
-  return (int)((heads + groups - 1) / groups);
+// Heads that one thread takes its angles through (`work`: threads of the call with
+// one head each): the angles of eight pairs cost about as much as four heads'
+// arithmetic, and past four there is nothing to gain; fewer where that would
+// leave under three workgroups of 256 threads per unit.  GPU time in us with 1 / 2 / 4 /
+// 8 heads: B4 Hq32 Hkv32 T8192 314 / 227 / 197 / 203, B1 Hq32 Hkv8 T3000 18.8 / 15.3 / 14.1 /
+// 14.0, T300 5.0 / 5.2 / 6.1 / 8.0, B32 T1 4.4 / 4.8 / 5.7 / 7.6 (D = 128).
+int heads_per_thread(long long work) {
+  const long long per = work / (3ll * 256 * device_cus());
+  return per < 1 ? 1 : per < 4 ? (int)per : 4;
 }
 
-int rotary_geometry(fa::RotaryArgs* a, bool vec) {
+// Threads of a rotary call per head.
+long long rotary_units(fa::RotaryArgs* a, bool vec) {
   const int pairs = (a->n + 7) / 8;
   a->units = vec ? a->D / 16 : pairs + (a->D - 2 * a->n + 15) / 16;
+  return (long long)a->B * a->T * a->units;
+}
+int rotary_groups(fa::RotaryArgs* a, long long threads, int per) {
   const int heads = a->t[0].heads + a->t[1].heads;
-  const long long tokens = (long long)a->B * a->T * a->units;
-  a->per = heads_per_thread(tokens, heads);
+  a->per = std::min(per, heads);
   a->groups = cdiv(heads, a->per);
   // (one thread index; the last workgroup's included)
-  return tokens * a->groups > 0x7fffff00ll ? FA_ERR_SHAPE : FA_OK;
+  return threads * a->groups > 0x7fffff00ll ? FA_ERR_SHAPE : FA_OK;
 }
 
 int rotary_args(const fa_rotary_call* c, fa::RotaryArgs* a, bool* vec) {
@@ -61,7 +64,8 @@ int rotary_args(const fa_rotary_call* c, fa::RotaryArgs* a, bool* vec) {
   a->pos64 = c->positions_64 != 0;
   a->pos_stride = c->positions_stride;
   a->offset = c->offset;
-  return rotary_geometry(a, *vec);
+  const long long threads = rotary_units(a, *vec);
+  return rotary_groups(a, threads, heads_per_thread(threads * (a->t[0].heads + a->t[1].heads)));
 }
 
 int append_args(const fa_kv_append_call* c, fa::AppendArgs* a) {
@@ -109,12 +113,14 @@ int append_args(const fa_kv_append_call* c, fa::AppendArgs* a) {
   }
   const long long runs = ((long long)c->T + FA_KV_RUN - 2) / FA_KV_RUN + 1;
   const long long token_threads = runs * FA_KV_RUN * c->B * (c->D / 16);
-  a->per = heads_per_thread(token_threads, Hkv);
-  a->groups = cdiv(Hkv, a->per);
-  const long long blocks = runs * c->B * a->groups;
-  if (blocks > 0x7fffffll) return FA_ERR_SHAPE;
   a->runs = (int)runs;
-  a->kv_blocks = (int)blocks;
+  auto heads = [&](long long work) {  // `work`: as heads_per_thread, keys and queries together
+    a->per = std::min(heads_per_thread(work), Hkv);
+    a->groups = cdiv(Hkv, a->per);
+    const long long blocks = runs * c->B * a->groups;
+    a->kv_blocks = (int)std::min(blocks, 0x7fffffll);
+    return blocks > 0x7fffffll ? FA_ERR_SHAPE : FA_OK;
+  };
   if (c->query.heads > 0) {
     if (!turn) return FA_ERR_SHAPE;  // nothing to do for the queries
     if (!c->query.data || !c->query_out) return FA_ERR_NULL;
@@ -129,9 +135,11 @@ int append_args(const fa_kv_append_call* c, fa::AppendArgs* a) {
     q.interleaved = a->interleaved;
     q.scale = a->scale;
     q.kv_lens = c->kv_lens;
-    return rotary_geometry(&q, true);
+    const long long threads = rotary_units(&q, true), work = token_threads * Hkv + threads * c->query.heads;
+    const int rc = heads(work);
+    return rc ? rc : rotary_groups(&q, threads, heads_per_thread(work));
   }
-  return FA_OK;
+  return heads(token_threads * Hkv);
 }
 
 struct DecodeLayout {

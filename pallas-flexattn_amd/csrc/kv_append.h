@@ -108,9 +108,9 @@ __global__ __launch_bounds__(2 * D) void kv_append_kernel(AppendArgs a) {
   const bool mine = pos >= len && tok < fresh;
   const bool begun = p0 < len, old = pos < len;
 
-  const RotaryUnit r = rotary_unit(u, a.freq ? a.n : 0, a.interleaved);
+  const RotaryUnit r = rotary_unit(u, a.freq ? a.n : 0, D, a.interleaved);
   float cs[8], sn[8];
-  if (a.freq && mine) rotary_angles(a.freq, 8 * u, a.n, (double)pos, a.scale, false, cs, sn);
+  if (a.freq && mine) rotary_angles(a.freq, r.p0, r.p1, a.n, (double)pos, a.scale, false, cs, sn);
   const int h1 = min((grp + 1) * a.per, a.Hkv);
   for (int h = grp * a.per; h < h1; ++h) {
     const size_t first = ((size_t)page * a.Hkv + h) * a.page_size + off;  // the run's first cache row
@@ -134,6 +134,12 @@ __global__ __launch_bounds__(2 * D) void kv_append_kernel(AppendArgs a) {
         store8(vd + r.b, vb);
       }
     } else {
+      const size_t si = first / kRunTokens;
+      int ke0 = 0, ve0 = 0;
+      if (begun) {  // (workgroup-uniform; read before the barrier, written behind it)
+        ke0 = scale_exp(a.ks[si]);
+        ve0 = scale_exp(a.vs[si]);
+      }
       float km = 0.f, vm = 0.f;
 #pragma unroll
       for (int t = 0; t < 8; ++t) {
@@ -159,15 +165,10 @@ __global__ __launch_bounds__(2 * D) void kv_append_kernel(AppendArgs a) {
           vm = fmaxf(vm, m[1][w]);
         }
       }
-      const size_t si = first / kRunTokens;
-      int ke = run_exp(km), ve = run_exp(vm), ke0 = ke, ve0 = ve;
-      if (begun) {  // workgroup-uniform
-        ke0 = scale_exp(a.ks[si]);
-        ve0 = scale_exp(a.vs[si]);
+      int ke = run_exp(km), ve = run_exp(vm);
+      if (begun) {
         ke = max(ke, ke0);
         ve = max(ve, ve0);
-        // every thread has the old scales before one of them writes the new
-        if (NW > 1) __syncthreads();
       }
       if (tid == 0) {
         a.ks[si] = ldexpf(1.f, ke);

@@ -39,16 +39,16 @@ struct RotaryArgs {
   int units, groups, per;
 };
 
-// sin and cos of pos * f radians.  The angle is taken to turns in 64 bits (its
-// absolute error grows as pos f 2^-52: 2e-10 turns at a million radians, where a 32-bit product
-// would be off by a hundredth of a turn), reduced to an eighth of a turn around
-// the nearest quarter, and the Taylor series of sine (to x^9) and cosine (to
-// x^10) on |x| <= pi / 4 leave under 2e-9: fp32 rounding is what remains.
-__device__ __forceinline__ void sincos_turns(double pos, double f, float* sn, float* cs) {
-  double t = pos * (f * 0.15915494309189533577);
+// sin and cos of 2 pi turns f radians, turns = pos / (2 pi).  The angle is kept in
+// turns in 64 bits (off by pos f 2^-52: 2e-10 at a million radians, where a 32-bit
+// product would be off by a hundredth of a turn) until whole turns and the nearest
+// quarter are taken off; the Taylor series of sine (to x^9) and cosine (to x^10) on
+// |x| <= pi / 4 leave under 2e-9: fp32 rounding is what remains.
+__device__ __forceinline__ void sincos_turns(double turns, double f, float* sn, float* cs) {
+  double t = turns * f;
   t -= rint(t);
-  const double q = rint(4.0 * t);  // quarter turns, -2 .. 2
-  const float x = (float)(fma(-0.25, q, t) * 6.283185307179586477);
+  const float q = rintf(4.0f * (float)t);  // quarter turns, -2 .. 2
+  const float x = (float)fma(-0.25, (double)q, t) * 6.2831853f;
   const float z = x * x;
   float s = fmaf(z, 2.7557319e-6f, -1.9841270e-4f);
   s = fmaf(s, z, 8.3333333e-3f);
@@ -66,16 +66,18 @@ __device__ __forceinline__ void sincos_turns(double pos, double f, float* sn, fl
   *cs = ((k + 1) & 2) ? -b : b;
 }
 
-// (cos, sin) x scale of pairs first .. first + 7 (past the n-th: 1 and 0).
-__device__ __forceinline__ void rotary_angles(const double* freq, int first, int n, double pos, float scale, bool inverse,
+// (cos, sin) x scale of pairs p0 .. p0 + 3 and p1 .. p1 + 3 (past the n-th: 1 and 0).
+__device__ __forceinline__ void rotary_angles(const double* freq, int p0, int p1, int n, double pos, float scale, bool inverse,
                                               float* cs, float* sn) {
+  const double turns = pos * 0.15915494309189533577;
 #pragma unroll
   for (int j = 0; j < 8; ++j) {
+    const int p = j < 4 ? p0 + j : p1 + j - 4;
     cs[j] = 1.f;
     sn[j] = 0.f;
-    if (first + j < n) {
+    if (p < n) {
       float s, c;
-      sincos_turns(pos, freq[first + j], &s, &c);
+      sincos_turns(turns, freq[p], &s, &c);
       cs[j] = c * scale;
       sn[j] = (inverse ? -s : s) * scale;
     }
@@ -117,19 +119,24 @@ __device__ __forceinline__ void store1(uint16_t* p, float x) { *p = (uint16_t)(p
 __device__ __forceinline__ void store1(float* p, float x) { *p = x; }
 
 // Where unit u's two eight-element chunks start (vector form: 2n and D are
-// multiples of 16).  Half layout: chunk a holds the first elements of the
-// unit's pairs, chunk b the second ones; interleaved, and in the copied rest:
-// 16 consecutive elements.
+// multiples of 16), half of the rotated (or of the copied) elements apart, so that neighbouring
+// threads read neighbouring chunks: with 16 consecutive elements per thread float32
+// B4 H16 T1000 D64 took 11.5 us, so 9.4.  Half layout: chunk a holds the
+// first elements of pairs p0 .. p0 + 7, chunk b the second ones; interleaved:
+// chunk a pairs p0 .. p0 + 3, chunk b pairs p1 .. p1 + 3.
 struct RotaryUnit {
-  int a, b;
+  int a, b, p0, p1;
   bool turn, half;
 };
-__device__ __forceinline__ RotaryUnit rotary_unit(int u, int n, bool interleaved) {
+__device__ __forceinline__ RotaryUnit rotary_unit(int u, int n, int D, bool interleaved) {
   RotaryUnit r;
-  r.turn = 8 * u < n;
+  const int v = u - n / 8;  // unit of the copied elements
+  r.turn = v < 0;
   r.half = r.turn && !interleaved;
-  r.a = r.half ? 8 * u : 16 * u;
-  r.b = r.half ? 8 * u + n : 16 * u + 8;
+  r.a = r.turn ? 8 * u : 2 * n + 8 * v;
+  r.b = r.turn ? 8 * u + n : D / 2 + n + 8 * v;
+  r.p0 = r.half ? 8 * u : r.turn ? 4 * u : n;
+  r.p1 = r.half ? 8 * u + 4 : r.turn ? 4 * u + n / 2 : n;
   return r;
 }
 // Rotates the unit's 16 values in place.
@@ -170,7 +177,9 @@ __device__ __forceinline__ void rotary_thread(const RotaryArgs& a, unsigned id) 
   else if (a.pos64) pos = (double)static_cast<const long long*>(a.positions)[b * a.pos_stride + tok];
   else pos = (double)static_cast<const int*>(a.positions)[b * a.pos_stride + tok];
   float cs[8], sn[8];
-  rotary_angles(a.freq, 8 * u, a.n, pos, a.scale, a.inverse, cs, sn);
+  RotaryUnit r{0, 0, 8 * u, 8 * u + 4, true, true};
+  if constexpr (kVec) r = rotary_unit(u, a.n, a.D, a.interleaved);
+  rotary_angles(a.freq, r.p0, r.p1, a.n, pos, a.scale, a.inverse, cs, sn);
   const int all = a.t[0].heads + a.t[1].heads;
   const int h0 = grp * a.per, h1 = min(h0 + a.per, all);
   for (int hh = h0; hh < h1; ++hh) {
@@ -180,7 +189,6 @@ __device__ __forceinline__ void rotary_thread(const RotaryArgs& a, unsigned id) 
     const T* x = static_cast<const T*>(R.x) + b * R.sb + h * R.sh + tok * R.st;
     T* y = static_cast<T*>(R.y) + (((size_t)b * R.heads + h) * a.T + tok) * a.D;
     if constexpr (kVec) {
-      const RotaryUnit r = rotary_unit(u, a.n, a.interleaved);
       float xa[8], xb[8];
       load8(x + r.a, xa);
       load8(x + r.b, xb);
