@@ -8,8 +8,8 @@
 // D = 128), its codes go from HBM straight into the registers that feed the
 // matrix cores, the next tile's as soon as this one's are used; no LDS and no barrier inside
 // the walk.  The g query heads of a kv head and their Sq queries are one block
-// of g Sq rows (rows of a group are contiguous in memory), 16 NQ rows of it per
-// work item, so the cache is read once per group.
+// of g Sq rows (rows of a group are contiguous in memory), 16 NQ rows of it (16 or 32)
+// per work item: groups of up to that many rows read the cache once.
 //
 // Layouts (v_mfma_f32_16x16x32_bf16; lane l = 16 g + r):
 //   * S^T = K Q^T: A = 16 keys, lane (r, g) holds key r's bytes 64 c + 16 g + [0, 16)
@@ -251,7 +251,7 @@ __device__ __forceinline__ DecodeUnit decode_unit(const DecodeArgs& a, int wg, b
 }
 
 template <int D, int NQ, int NW, bool kMods, bool kStream>
-__global__ __launch_bounds__(64 * NW, NQ == 4 ? 1 : 2) void decode_fp8_kernel(DecodeArgs a) {
+__global__ __launch_bounds__(64 * NW, 2) void decode_fp8_kernel(DecodeArgs a) {
   using Tile = CodeTile<D, kStream>;
   constexpr int DV = Tile::DV, KC = Tile::KC, KW = Tile::KW;
   constexpr int KS = D / 32;           // k steps of S

@@ -46,8 +46,7 @@ template <int D, bool M>
 static void decode_nq(const DecodeArgs& a, int nq, bool stream, hipStream_t s) {
   if (nq == 1 && a.by_item) run_decode<D, 1, 8, M>(a, stream, s);
   else if (nq == 1) run_decode<D, 1, 4, M>(a, stream, s);
-  else if (nq == 2) run_decode<D, 2, 4, M>(a, stream, s);
-  else run_decode<D, 4, 4, M>(a, stream, s);
+  else run_decode<D, 2, 4, M>(a, stream, s);
   if (a.by_item) return;
   const int rows = a.B * a.Hkv * a.g * a.Sq;
   hipLaunchKernelGGL((decode_fp8_merge<D>), dim3(cdiv(rows, 4)), dim3(256), 0, s, a, 16 * nq);

@@ -37,7 +37,7 @@ int launch_quant_fp8(const QuantArgs& a, hipStream_t s);
 // Around a KV cache (kernels_cache.hip): rotary positions (f32 or bf16; vec:
 // 16-byte accesses), appends (D = 32, 64 or 128) and decode over e4m3 pages
 // (nq:
-// 16-row query blocks per work item, 1, 2 or 4; stream: cache reads past the caches)
+// 16-row query blocks per work item, 1 or 2; stream: cache reads past the caches)
 int launch_rotary(const RotaryArgs& a, bool f32, bool vec, hipStream_t s);
 int launch_append(const AppendArgs& a, int D, bool fp8, hipStream_t s);
 int launch_decode_fp8(const DecodeArgs& a, int D, int nq, bool mods, bool stream, hipStream_t s);

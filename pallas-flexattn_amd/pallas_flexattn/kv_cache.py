@@ -97,8 +97,8 @@ def flex_decode_fp8(query, cache: Fp8KVCache, kv_lens=None, page_table=None, mas
     gradient): ``query`` (B, Hq, Sq, D) bf16, ``cache`` an :class:`Fp8KVCache`, ``kv_lens`` (B,) the
     keys of each row, the queries' own included (None: the whole page table).  Made for
     short query blocks (decoding, speculative decoding, short chunks): the cache is read once for
-    every 64 rows of Sq * Hq / Hkv, and each row's keys are split over as many workgroups as the
-    batch needs.
+    every 16 to 32 rows of Sq * Hq / Hkv, and each row's keys are split over as many workgroups as
+    the batch needs.
 
     Query i sits at position ``kv_lens[b] - Sq + i`` (bottom-right aligned, as
     ``flex_attention_varlen``); with ``query_lens`` (B,) a row has only that many queries, at

@@ -99,6 +99,29 @@ def test_decode(case):
     assert (pf.flex_decode_fp8(q, c.cache, c.lens, c.table, mask_mod=mask, score_mod=score, enable_gqa=True) == o).all()
 
 
+LARGE = [
+    # lens, Hq, Hkv, Sq, D, pages per row of 512 tokens, mask, mods: page tables long enough that 32-row items (more than
+    # 16 rows) and reads past the caches are chosen
+    ([900, 40], 16, 2, 3, 128, 200, (-1, 0), 0), ([33, 2000], 8, 2, 5, 64, 200, None, 1), ([700, 0], 14, 2, 5, 32, 300, (300, 0), 0),
+    ([1500, 1], 4, 2, 1, 128, 400, None, 0), ([3000, 100], 4, 2, 2, 64, 600, (-1, 0), 1), ([600, 64], 32, 2, 1, 32, 800, None, 0),
+]
+
+
+@pytest.mark.parametrize("case", LARGE, ids=[str(i) for i in range(len(LARGE))])
+def test_large_tables(case):
+    import pallas_flexattn as pf
+    lens, Hq, Hkv, Sq, D, pages, win, mods = case
+    c = Cache(lens, Hkv, 512, D, 23, per_row=pages)
+    q = _q(len(lens), Hq, Sq, D, 24)
+    left, right = win or (-1, -1)
+    mask = None if win is None else pf.MaskSpec(left=left, right=right)
+    score = pf.compose_score_mods(pf.alibi_score_mod(Hq), pf.softcap_score_mod(15.0)) if mods else None
+    o, lse = pf.flex_decode_fp8(q, c.cache, c.lens, c.table, mask_mod=mask, score_mod=score, enable_gqa=True, return_lse=True)
+    keep = -(-max(lens) // 32) * 32
+    c.rows = [r[:, :, :keep] for r in c.rows]
+    _check(o, lse, q, c, lens, None, left, right, None, pf.alibi_slopes(Hq) if mods else None, 15.0 if mods else 0.0)
+
+
 def test_large_scores_and_scale():
     """Scores that change by hundreds from key to key (the running maximum moves all the time), a scale of one's own."""
     import pallas_flexattn as pf
@@ -182,6 +205,31 @@ def test_whole_table_strides_and_no_table():
     # slots of nobody's pages and of unused rows do not matter: garbage elsewhere changes nothing
     assert pf.flex_decode_fp8(q[:0], c.cache, c.lens[:0], c.table[:0], enable_gqa=True).shape == (0, 6, 2, 128)
     assert pf.flex_decode_fp8(q[:, :, :0], c.cache, c.lens, c.table, enable_gqa=True).numel() == 0
+
+
+def test_two_threads_at_once():
+    """The launcher from two threads, each on a stream of its own."""
+    import threading
+    import torch
+    import pallas_flexattn as pf
+    c = Cache([3000, 500], 2, 64, 64, 63)
+    q = _q(2, 8, 1, 64, 64)
+    want = pf.flex_decode_fp8(q, c.cache, c.lens, c.table, enable_gqa=True)
+    torch.cuda.synchronize()
+    got = [None, None]
+
+    def work(i):
+        s = torch.cuda.Stream()
+        with torch.cuda.stream(s):
+            got[i] = [pf.flex_decode_fp8(q, c.cache, c.lens, c.table, enable_gqa=True) for _ in range(20)]
+        s.synchronize()
+
+    ts = [threading.Thread(target=work, args=(i,)) for i in range(2)]
+    for t in ts:
+        t.start()
+    for t in ts:
+        t.join()
+    assert all(torch.equal(o, want) for g in got for o in g)
 
 
 def test_same_results_alone_and_in_a_batch_order():
