@@ -208,25 +208,25 @@ int decode_args(const fa_params* p, const fa_fp8_cache* kv, int cus, fa::DecodeA
   a->alibi = p->alibi_slopes;
   a->rt = (int)rt;
   // How the walk is cut (csrc/decode_index.h), from the longest walk that the
-  // sizes allow; measured as GPU time per call in replayed graphs, D = 128 unless named,
-  // by item in eight waves / in pieces of four.
-  // One workgroup per item, no second launch, where walks are short (8 items of 16
-  // tiles 7.2 / 10.7 us, 128 of 34 11.4 / 14.8, at 48 about even) or where the items
-  // fill half of the units and none is very long (128 of 96 23.8 / 25.0, of 127 29.5 /
-  // 29.9, 512 of 68 37.5 / 38.8, D = 64 512 of 65 19.9 / 22.3). Pieces beyond: 8 of 126 25.6 / 13.0,
-  // 64 of 127 26.7 / 19.9, 256 rows of mixed lengths to 257 61 / 56; they lose only
-  // on many equal long rows (D = 64 256 of 513 88 / 96).
-  a->by_item = tiles <= 48 || (2 * items >= cus && tiles <= 128);
-  // Pieces of one chunk each fill the GPU with two workgroups per unit; four at D <= 64,
-  // whose tiles are half the bytes (D = 64 256 mixed to 284 42.0 / 40.6, D = 128 64 of 1024 97 / 99).
-  a->pieces = (p->D <= 64 ? 4 : 2) * cus;
+  // sizes allow; GPU time per call in us in replayed graphs, D = 128 unless named, by item in
+  // eight waves / in pieces of four.  One workgroup per item, without a second launch, where
+  // walks are short (8 items of 16 tiles 7.2 / 10.7, 128 of 34 11.4 / 14.8, at 48 about even)
+  // or where the kv heads fill half of the units and no walk is very long (128 of 96 24.4 /
+  // 25.5, of 127 29.5 / 29.9, 256 of 121 45.2 / 49.8, 512 of 68 37.5 / 38.8, D = 64 512 of 65 19.9 / 22.3).
+  // Pieces beyond: 8 of 126 25.6 / 13.0, 64 of 127 26.7 / 19.9, 32 of 127 with two blocks of rows
+  // 27.4 / 21.2, 256 of mixed lengths to 257 61 / 55; they lose only on many equal
+  // long rows (D = 64 256 of 513 88 / 96).
+  a->by_item = tiles <= 48 || (2ll * p->B * p->Hkv >= cus && tiles <= 128);
+  // At most four pieces per unit (two where the rows are equally long: decode_unit).
+  a->pieces = 4 * cus;
   // At least 16 tiles a piece, four per wave, so that the merge stays short (8 of 500
   // 16.5 us, with 8 tiles 18.8); 8 where that makes at most 16 pieces (8 of 126 12.4, 11.8).
   a->least = tiles <= 128 ? 8 : 16;
   // A call that reads more than fits the 256 MB last-level cache beside other data
-  // reads past it (V of 64 items of 1024 tiles: 107 / 97 us, 256 mixed 61 / 56, at 100 MB
-  // even); smaller ones may find theirs there (D = 64 51 MB 14.3 / 15.2, D = 128 33 MB 14.8 / 15.7).
-  L->stream = 2ll * p->B * p->Hkv * tiles * fa::kTileKeys * p->D > 96ll << 20;
+  // reads past it (through / past the caches: 64 items of 1024 tiles 107 / 97 us, 256 mixed
+  // 61 / 56, 128 of 127, 133 MB, 36 / 29.5); smaller ones may find theirs there (100 MB 24.4 / 27.5,
+  // 33 MB 14.8 / 15.7, D = 64 51 MB 14.3 / 15.2).
+  L->stream = 2ll * p->B * p->Hkv * tiles * fa::kTileKeys * p->D > 112ll << 20;
   const long long grid = a->by_item ? items : fa::decode_grid(items, (int)tiles, a->pieces, a->least);
   if (grid > 0x7fffffll) return FA_ERR_SHAPE;
   a->grid = (int)grid;

@@ -46,8 +46,16 @@ int main() {
     int bound = (cap + kTileKeys - 1) / kTileKeys;
     if (left >= 0) bound = imin(bound, (left + Sq + kTileKeys - 2) / kTileKeys + 1);
     if (most > bound) fail("walk longer than the host's bound", most, bound);
-    const int chunk = decode_chunk((int)total, pieces, least);
+    int chunk = decode_chunk((int)total, pieces, least);
     if ((long long)chunk * pieces < total || chunk < least) fail("chunk", chunk, total);
+    for (int i = 0;; ++i) {  // as the device does
+      long long all = 0;
+      for (int b = 0; b < B; ++b) all += (long long)decode_pieces(span[b].n, chunk) * Hkv * rt;
+      if (all <= pieces || B * Hkv * rt >= pieces || i == kChunkTries) break;
+      const int next = decode_next_chunk(chunk, (int)all, pieces);
+      if (next <= chunk) fail("chunk does not grow", next, chunk);
+      chunk = next;
+    }
     long long units = 0, slots = 0;
     for (int b = 0; b < B; ++b) {
       const int n = span[b].n, p = decode_pieces(n, chunk);
