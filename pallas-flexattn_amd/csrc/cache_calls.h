@@ -170,7 +170,8 @@ int decode_args(const fa_params* p, const fa_fp8_cache* kv, int cus, fa::DecodeA
   const long long rows = (long long)g * p->Sq;
   if (rows * p->B * p->Hkv > 0x7ffffffll) return FA_ERR_SHAPE;
   // tiles that a row walks at most: all of its keys', or the window's
-  const int left = p->window_left < 0 ? -1 : p->window_left;
+  // (a window of at least all keys is none)
+  const int left = p->window_left < 0 || p->window_left >= p->Skv ? -1 : p->window_left;
   long long tiles = (p->Skv + fa::kTileKeys - 1) / fa::kTileKeys;
   if (left >= 0) tiles = std::min(tiles, ((long long)left + p->Sq + fa::kTileKeys - 2) / fa::kTileKeys + 1);
   // Query rows of an item: 16, or 32 where the group has more and the call is long
@@ -215,8 +216,8 @@ int decode_args(const fa_params* p, const fa_fp8_cache* kv, int cus, fa::DecodeA
   // 25.5, of 127 29.5 / 29.9, 256 of 121 45.2 / 49.8, 512 of 68 37.5 / 38.8, D = 64 512 of 65 19.9 / 22.3).
   // Pieces beyond: 8 of 126 25.6 / 13.0, 64 of 127 26.7 / 19.9, 32 of 127 with two blocks of rows
   // 27.4 / 21.2, 256 of mixed lengths to 257 61 / 55; they lose only on many equal
-  // long rows (D = 64 256 of 513 88 / 96).
-  a->by_item = tiles <= 48 || (2ll * p->B * p->Hkv >= cus && tiles <= 128);
+  // long rows (D = 64 256 of 513 88 / 96). Over 256 rows are enough items as they are.
+  a->by_item = tiles <= 48 || (2ll * p->B * p->Hkv >= cus && tiles <= 128) || p->B > 64 * fa::kLaneRows;
   // At most four pieces per unit (two where the rows are equally long: decode_unit).
   a->pieces = 4 * cus;
   // At least 16 tiles a piece, four per wave, so that the merge stays short (8 of 500

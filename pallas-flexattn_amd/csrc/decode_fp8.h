@@ -204,8 +204,8 @@ struct DecodeUnit {
   int item;              // kv head * rt + query block
   int t0, nt, slot;      // tiles, and the slot of a part of an item (-1: all of it)
 };
-// Every wave finds its workgroup's unit by itself: the rows' lengths are read
-// by the lanes (consecutive rows per lane), two scans give the chunk and the rows' first units.
+// Every wave finds its workgroup's unit by itself: the lanes hold the rows'
+// tiles (up to kLaneRows consecutive rows each), scans give the chunk and the rows' first units.
 __device__ __forceinline__ DecodeUnit decode_unit(const DecodeArgs& a, int wg, bool first_wave) {
   const int each = a.Hkv * a.rt;
   DecodeUnit u;
@@ -221,31 +221,33 @@ __device__ __forceinline__ DecodeUnit decode_unit(const DecodeArgs& a, int wg, b
     return u;
   }
   const int lane = threadIdx.x & 63;
-  const int per = (a.B + 63) / 64, b0 = min(lane * per, a.B), b1 = min(b0 + per, a.B);
-  auto tiles = [&](int b) { return decode_span(row_keys(a, b), row_queries(a, b), a.win_left).n; };
-  int sum = 0, n0 = 0;
-  bool same = true;  // this lane's rows have equally many tiles
-  for (int b = b0; b < b1; ++b) {
-    const int n = tiles(b);
-    same = same && (b == b0 || n == n0);
-    n0 = n;
-    sum += n;
+  const int per = (a.B + 63) / 64, b0 = lane * per;
+  int n[kLaneRows], sum = 0;  // tiles of this lane's rows, 0: no row
+  bool same = true;
+#pragma unroll
+  for (int j = 0; j < kLaneRows; ++j) {
+    const int b = b0 + j;
+    n[j] = j < per && b < a.B ? decode_span(row_keys(a, b), row_queries(a, b), a.win_left).n : 0;
+    sum += n[j];
   }
+  const int n0 = __builtin_amdgcn_readfirstlane(n[0]);
+#pragma unroll
+  for (int j = 0; j < kLaneRows; ++j) same = same && (n[j] == 0 || n[j] == n0);
   // Equal rows make equal pieces, two per compute unit; of unequal ones, whose
   // pieces differ by up to half, twice as many come out more even (GPU time with two / four:
   // 8 equal rows of 32768 keys 97 / 99 us, 32 of 3840 49.8 / 51.7, 32 mixed to 8192 59.8 / 54.9,
   // D = 64 32 mixed to 9000 48 / 42).
-  const bool equal = __all(same && (b0 == b1 || n0 == __builtin_amdgcn_readfirstlane(n0)));
-  const int pieces = equal ? a.pieces / 2 : a.pieces;
+  const int pieces = __all(same) ? a.pieces / 2 : a.pieces;
   const int total = __builtin_amdgcn_readlane(wave_scan(sum), 63) * each;
   int chunk = decode_chunk(total, pieces, a.least);
-  int units, slots, iu;
+  int p[kLaneRows], units, slots, iu;  // pieces per item, this lane's units and slots
   for (int i = 0;; ++i) {
     units = slots = 0;
-    for (int b = b0; b < b1; ++b) {
-      const int p = decode_pieces(tiles(b), chunk) * each;
-      units += p;
-      slots += p > each ? p : 0;
+#pragma unroll
+    for (int j = 0; j < kLaneRows; ++j) {
+      p[j] = decode_pieces(n[j], chunk);
+      units += p[j] * each;
+      slots += p[j] > 1 ? p[j] * each : 0;
     }
     iu = wave_scan(units);
     const int all = __builtin_amdgcn_readlane(iu, 63);
@@ -256,44 +258,46 @@ __device__ __forceinline__ DecodeUnit decode_unit(const DecodeArgs& a, int wg, b
   int fu = iu - units, fs = is - slots;
   if (wg == 0 && first_wave) {  // for the merge
     int f = fu, g = fs;
-    for (int b = b0; b < b1; ++b) {
-      const int p = decode_pieces(tiles(b), chunk) * each;
-      a.head[2 * b] = f;
-      a.head[2 * b + 1] = g;
-      f += p;
-      g += p > each ? p : 0;
+#pragma unroll
+    for (int j = 0; j < kLaneRows; ++j) {
+      if (n[j]) {
+        a.head[2 * (b0 + j)] = f;
+        a.head[2 * (b0 + j) + 1] = g;
+      }
+      f += p[j] * each;
+      g += p[j] > 1 ? p[j] * each : 0;
     }
     if (lane == 63) a.head[2 * a.B] = iu;
   }
-  // the lane whose rows hold unit wg, then the row among them
-  int b = b0, n = 0, p = 1;
-  if (wg >= fu && wg < iu) {
-    for (;; ++b) {
-      n = tiles(b);
-      p = decode_pieces(n, chunk);
-      if (wg < fu + p * each) break;
-      fu += p * each;
-      fs += p > 1 ? p * each : 0;
-    }
-  }
+  // the lane whose rows hold unit wg, and the row among them
   const unsigned long long mine = __ballot(wg >= fu && wg < iu);
   if (!mine) {
     u.b = -1;
     return u;
   }
+  int b = b0, nb = n[0], pb = p[0];
+#pragma unroll
+  for (int j = 1; j < kLaneRows; ++j) {
+    const bool later = b == b0 + j - 1 && wg >= fu + pb * each && n[j] != 0;
+    fu += later ? pb * each : 0;
+    fs += later && pb > 1 ? pb * each : 0;
+    b = later ? b0 + j : b;
+    nb = later ? n[j] : nb;
+    pb = later ? p[j] : pb;
+  }
   const int src = __builtin_ctzll(mine);
   u.b = __builtin_amdgcn_readlane(b, src);
-  p = __builtin_amdgcn_readlane(p, src);
-  n = __builtin_amdgcn_readlane(n, src);
+  pb = __builtin_amdgcn_readlane(pb, src);
+  nb = __builtin_amdgcn_readlane(nb, src);
   const int local = wg - __builtin_amdgcn_readlane(fu, src);
   u.have = a.kv_lens ? clamp_len(scalar_load(a.kv_lens, u.b), a.cap) : a.cap;
   u.ql = a.q_lens ? clamp_len(scalar_load(a.q_lens, u.b), a.Sq) : a.Sq;
-  u.item = local / p;
-  const int piece = local - u.item * p;
-  const int lo = decode_piece(n, p, piece);
+  u.item = local / pb;
+  const int piece = local - u.item * pb;
+  const int lo = decode_piece(nb, pb, piece);
   u.t0 = decode_span(u.have, u.ql, a.win_left).lo + lo;
-  u.nt = decode_piece(n, p, piece + 1) - lo;
-  u.slot = p > 1 ? __builtin_amdgcn_readlane(fs, src) + local : -1;
+  u.nt = decode_piece(nb, pb, piece + 1) - lo;
+  u.slot = pb > 1 ? __builtin_amdgcn_readlane(fs, src) + local : -1;
   return u;
 }
 

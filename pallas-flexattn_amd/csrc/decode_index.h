@@ -13,6 +13,7 @@
 namespace fa {
 
 constexpr int kTileKeys = 32;  // keys of a tile: one scale run
+constexpr int kLaneRows = 4;   // batch rows that a lane of a wave keeps (calls cut in pieces: 256 rows)
 
 struct DecodeSpan {
   int lo;  // first tile

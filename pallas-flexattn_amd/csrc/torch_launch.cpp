@@ -19,6 +19,7 @@
 #include <c10/core/DeviceGuard.h>
 #include <c10/hip/HIPStream.h>
 
+#include <algorithm>
 #include <cstdint>
 
 #include "../../include/flexattn.h"
@@ -487,7 +488,7 @@ PyObject* py_decode(PyObject*, PyObject* const* a, Py_ssize_t n) {
   if (!q || !(k = tensor(a[1])) || !(v = tensor(a[2])) || !(ks = tensor(a[3])) || !(vs = tensor(a[4])) ||
       !optional(a[5], &lens) || !optional(a[6], &table) || !optional(a[7], &ql) || !optional(a[10], &slopes))
     return nullptr;
-  const long left = PyLong_AsLong(a[8]), right = PyLong_AsLong(a[9]);
+  const int64_t left = std::min<int64_t>(PyLong_AsLong(a[8]), kMaxSize), right = std::min<int64_t>(PyLong_AsLong(a[9]), kMaxSize);
   const double softcap = PyFloat_AsDouble(a[11]), scale = PyFloat_AsDouble(a[12]);
   const int gqa = PyObject_IsTrue(a[13]);
   if (PyErr_Occurred()) return nullptr;

@@ -132,6 +132,33 @@ def test_large_scores_and_scale():
     _check(o, lse, q, c, lens, scale=0.7)
 
 
+def test_many_rows():
+    """Row counts around and past what a wave's lanes hold, with items cut in pieces: short rows beside long ones."""
+    import torch
+    import pallas_flexattn as pf
+    for B in (63, 64, 65, 129, 256, 257):
+        lens = [(37 * i) % 90 for i in range(B)]
+        lens[B // 2], lens[B - 1] = 2500, 1700
+        c = Cache(lens, 1, 512, 32, 33, per_row=9)  # (long enough tables to be cut in pieces)
+        q = _q(B, 2, 1, 32, 34)
+        o, lse = pf.flex_decode_fp8(q, c.cache, c.lens, c.table, enable_gqa=True, return_lse=True)
+        _check(o, lse, q, c, lens)
+
+
+def test_window_without_an_end():
+    """Window sides past every key, at the largest 32-bit number and above it."""
+    import pallas_flexattn as pf
+    c = Cache([70, 3], 1, 32, 64, 35)
+    q = _q(2, 2, 2, 64, 36)
+    want, wl = pf.flex_decode_fp8(q, c.cache, c.lens, c.table, mask_mod=pf.causal_mask, enable_gqa=True, return_lse=True)
+    _check(want, wl, q, c, [70, 3], None, -1, 0)
+    for left in (96, 2 ** 31 - 1, 2 ** 40):
+        got = pf.flex_decode_fp8(q, c.cache, c.lens, c.table, mask_mod=pf.sliding_window_mask(left, 0), enable_gqa=True)
+        assert (got == want).all()
+    both = pf.flex_decode_fp8(q, c.cache, c.lens, c.table, mask_mod=pf.sliding_window_mask(2 ** 40, 2 ** 40), enable_gqa=True)
+    assert (both == pf.flex_decode_fp8(q, c.cache, c.lens, c.table, enable_gqa=True)).all()
+
+
 def test_padded_queries():
     import torch
     import pallas_flexattn as pf
