@@ -39,6 +39,20 @@ struct AppendArgs {
   RotaryArgs q;
 };
 
+// Largest of a wave's non-negative values, in every lane (DPP row rotations,
+// then the swaps across rows: no LDS round trips).
+__device__ __forceinline__ float wave_max(float x) {
+  auto turn = [](float v, auto ctrl) {
+    return __uint_as_float(__builtin_amdgcn_update_dpp(0, __float_as_uint(v), decltype(ctrl)::value, 0xf, 0xf, false));
+  };
+  x = fmaxf(x, turn(x, Int<0x121>{}));  // row_ror 1, 2, 4, 8
+  x = fmaxf(x, turn(x, Int<0x122>{}));
+  x = fmaxf(x, turn(x, Int<0x124>{}));
+  x = fmaxf(x, turn(x, Int<0x128>{}));
+  const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  return pair_max(fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1])));
+}
+
 __device__ __forceinline__ float finite_max(float m, float x) {
   const float a = fabsf(x);
   return a < INFINITY ? fmaxf(m, a) : m;  // (NaN and infinities stay out: their codes are NaN)
@@ -101,7 +115,6 @@ __global__ __launch_bounds__(2 * D) void kv_append_kernel(AppendArgs a) {
   const long long pg = p0 / a.page_size;
   if (pg >= a.max_pages) return;  // past the table: dropped
   const int page = a.page_table ? a.page_table[(size_t)b * a.max_pages + pg] : b;
-  if (page < 0 || page >= a.num_pages) return;
   const int off = (int)(p0 - pg * a.page_size);
   const long long pos = p0 + row;
   const int tok = (int)(pos - len);
@@ -111,6 +124,7 @@ __global__ __launch_bounds__(2 * D) void kv_append_kernel(AppendArgs a) {
   const RotaryUnit r = rotary_unit(u, a.freq ? a.n : 0, D, a.interleaved);
   float cs[8], sn[8];
   if (a.freq && mine) rotary_angles(a.freq, r.p0, r.p1, a.n, (double)pos, a.scale, false, cs, sn);
+  if (page < 0 || page >= a.num_pages) return;  // (the page's id comes in beside the angles)
   const int h1 = min((grp + 1) * a.per, a.Hkv);
   for (int h = grp * a.per; h < h1; ++h) {
     const size_t first = ((size_t)page * a.Hkv + h) * a.page_size + off;  // the run's first cache row
@@ -146,11 +160,8 @@ __global__ __launch_bounds__(2 * D) void kv_append_kernel(AppendArgs a) {
         km = finite_max(finite_max(km, ka[t]), kb[t]);
         vm = finite_max(finite_max(vm, va[t]), vb[t]);
       }
-#pragma unroll
-      for (int o = 32; o > 0; o >>= 1) {
-        km = fmaxf(km, __shfl_xor(km, o));
-        vm = fmaxf(vm, __shfl_xor(vm, o));
-      }
+      km = wave_max(km);
+      vm = wave_max(vm);
       if constexpr (NW > 1) {
         // (two buffers: a wave is at most one head ahead of the barrier's slowest)
         float(*m)[NW] = red[h & 1];
