@@ -209,3 +209,33 @@ def test_other_stream_and_graph_replays():
         torch.cuda.synchronize()
         w = pf.apply_rotary(q, k, rot, offset=shift)
         assert torch.equal(yq, w[0]) and torch.equal(yk, w[1])
+
+
+def test_captured_gradient():
+    """Forward and gradient in a graph, replayed with other contents, eager work between the replays."""
+    import torch
+    import pallas_flexattn as pf
+    rot = pf.rotary_embedding(64)
+    q = torch.randn(1, 2, 33, 64, device="cuda").bfloat16().requires_grad_()
+    k = torch.randn(1, 1, 33, 64, device="cuda").bfloat16().requires_grad_()
+    gq, gk = torch.randn_like(q), torch.randn_like(k)
+
+    def step():
+        y = pf.apply_rotary(q, k, rot)
+        return [t.detach() for t in y] + list(torch.autograd.grad(y, (q, k), (gq, gk)))
+
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        step()
+    torch.cuda.current_stream().wait_stream(s)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = step()
+    for _ in range(3):
+        with torch.no_grad():
+            for t in (q, k, gq, gk):
+                t.copy_(torch.randn_like(t))
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(got, step()))
