@@ -407,8 +407,8 @@ typedef struct fa_kv_append_call {
 int fa_kv_append(const fa_kv_append_call *c, void *stream);
 
 /* Decode over a paged cache in e4m3 (p->dtype = FA_DTYPE_FP8_E4M3; q bf16 with
- * 16-byte aligned rows, o bf16 and lse float32 dense; D = 32, 64 or 128).  Row b has kv_lens[b] keys (null: p->Skv, the
- * tokens of its page table) and its queries are the newest of them: query i of
+ * 16-byte aligned rows, o bf16 and lse float32 dense; D = 32, 64 or 128).  Row b has kv_lens[b] keys (at most p->Skv;
+ * null: p->Skv, the tokens of its page table) and its queries are the newest of them: query i of
  * q_lens[b] (null: Sq) sits at position kv_lens[b] - q_lens[b] + i, which is
  * what p's window and ALiBi refer to; queries i >= q_lens[b] give o = 0 and
  * lse = -inf, as do queries that see no key.  Page ids outside the cache read

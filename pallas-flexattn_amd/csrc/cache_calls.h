@@ -144,6 +144,7 @@ int append_args(const fa_kv_append_call* c, fa::AppendArgs* a) {
 
 struct DecodeLayout {
   int nq;               // 16-row query blocks per work item
+  bool general;         // score modifiers, or a block's rows see different keys
   bool stream;          // cache reads past the caches
   size_t part, ml, bytes;
 };
@@ -153,7 +154,9 @@ int decode_args(const fa_params* p, const fa_fp8_cache* kv, int cus, fa::DecodeA
   if (p->abi_version != FA_ABI_VERSION) return FA_ERR_VERSION;
   if (p->dtype != FA_DTYPE_FP8_E4M3) return FA_ERR_DTYPE;
   if (p->D != 32 && p->D != 64 && p->D != 128) return FA_ERR_UNSUPPORTED;
-  if (p->B < 1 || p->Hq < 1 || p->Hkv < 1 || p->Hq % p->Hkv || p->Sq < 1 || p->Skv < 1) return FA_ERR_SHAPE;
+  if (p->B < 1 || p->Hq < 1 || p->Hkv < 1 || p->Hq % p->Hkv || p->Sq < 1 || p->Skv < 1 ||
+      p->Skv > 0x7fffffff - 2 * fa::kTileKeys)
+    return FA_ERR_SHAPE;
   if (!(p->softcap >= 0.f) || !(p->scale >= 0.f)) return FA_ERR_SHAPE;
   if (p->q_doc_ids || p->kv_doc_ids || p->doc_start || p->doc_end || p->kv_num_blocks || p->kv_indices ||
       p->full_kv_num_blocks || p->full_kv_indices)
@@ -193,7 +196,6 @@ int decode_args(const fa_params* p, const fa_fp8_cache* kv, int cus, fa::DecodeA
   a->kv_lens = kv->kv_lens;
   a->q_lens = kv->q_lens;
   a->B = p->B;
-  a->Hq = p->Hq;
   a->Hkv = p->Hkv;
   a->Sq = p->Sq;
   a->g = g;
@@ -202,7 +204,13 @@ int decode_args(const fa_params* p, const fa_fp8_cache* kv, int cus, fa::DecodeA
   a->num_pages = kv->num_pages;
   a->cap = p->Skv;
   a->win_left = left;
-  a->win_right = p->window_right < 0 ? -1 : p->window_right;
+  // (the first of Sq queries stands Sq - 1 before the last key at most)
+  a->win_right = p->window_right < 0 || p->window_right >= p->Sq - 1 ? -1 : p->window_right;
+  // A row of an item sees the item's keys or, padded, none, unless there are several queries
+  // and a window: then NaN values must be kept from the rows that do not see their key, which
+  // costs registers that the plain walk has no room for (D = 128: 138 for 126, three waves per
+  // SIMD for four; 256 mixed lengths to 257 tiles 58.3 us for 54.5).
+  L->general = p->alibi_slopes || p->softcap > 0.f || (p->Sq > 1 && (left >= 0 || a->win_right >= 0));
   a->scale = p->scale == 0.f ? 1.0f / sqrtf((float)p->D) : p->scale;
   a->scale_log2 = a->scale * fa::kLog2e;
   a->softcap = p->softcap;

@@ -690,8 +690,7 @@ int fa_fwd_kvcache_fp8(const fa_params* p, const fa_fp8_cache* kv, const fa_stri
     a.part = reinterpret_cast<float*>(ws + L.part);
     a.part_ml = reinterpret_cast<float*>(ws + L.ml);
   }
-  return fa::launch_decode_fp8(a, p->D, L.nq, p->alibi_slopes != nullptr || p->softcap > 0.f, L.stream,
-                               static_cast<hipStream_t>(stream));
+  return fa::launch_decode_fp8(a, p->D, L.nq, L.general, L.stream, static_cast<hipStream_t>(stream));
 }
 
 size_t fa_mask_build_workspace_bytes(const fa_mask_build* m) {

@@ -6,10 +6,11 @@
 // Bound by the reads of the cache (2 D + 1/4 bytes per key and kv head), so
 // everything is laid out for those: a wave takes 32-key tiles (4 + 4 KiB at
 // D = 128), its codes go from HBM straight into the registers that feed the
-// matrix cores, the next tile's as soon as this one's are used; no LDS and no barrier inside
-// the walk.  The g query heads of a kv head and their Sq queries are one block
-// of g Sq rows (rows of a group are contiguous in memory), 16 NQ rows of it (16 or 32)
-// per work item: groups of up to that many rows read the cache once.
+// matrix cores, the next tile's as soon as this one's are used; no LDS and no
+// barrier inside the walk.  The g query heads of a kv head and their Sq queries
+// are one block of g Sq rows, 16 NQ of them (16 or 32) per work item: groups of
+// up to that many rows read the cache once.  B8 Hq32 Hkv8 32768 keys D128: 86 us
+// for 538 MB (6.2 TB/s), 4.7 more for the join.
 //
 // Layouts (v_mfma_f32_16x16x32_bf16; lane l = 16 g + r):
 //   * S^T = K Q^T: A = 16 keys, lane (r, g) holds key r's bytes 64 c + 16 g + [0, 16)
@@ -20,16 +21,16 @@
 //     those lanes as the B operand of O^T += V^T P^T, whose k index may name the keys
 //     in that order; the A operand then wants the same eight keys of one d.
 //   * V rows: lane (r, g) loads bytes [DV r, DV r + DV) (DV = D / 16) of its eight
-//     keys: an instruction reads four consecutive rows, whole cache lines; v_perm_b32 pairs two keys' bytes, the conversion to bf16 makes the
+//     keys: an instruction reads four consecutive rows, whole cache lines;
+//     v_perm_b32 pairs two keys' bytes, the conversion to bf16 makes the
 //     operand's words.  MFMA t is then rows d = DV r + t, and a lane ends
-//     with 4 DV consecutive d of its query: 16-byte stores.
+//     with 4 DV consecutive d of its query.
 // P goes into the product as two bf16 pieces (its value and what that
 // rounding left): the matrix cores are idle most of the time anyway, and O
 // then carries only its own rounding.
 #pragma once
-#include "decode_index.h"
-#include "dma.h"
 #include "common.h"
+#include "decode_index.h"
 
 namespace fa {
 
@@ -42,7 +43,7 @@ struct DecodeArgs {
   const int *kv_lens, *q_lens;  // (B) or null: every key of the table, Sq
   void* o;           // bf16
   float* lse;
-  int B, Hq, Hkv, Sq, g;
+  int B, Hkv, Sq, g;  // g query heads per kv head
   int page_runs, max_pages, num_pages, cap;  // runs per page, keys of the table
   int win_left, win_right;
   float scale, scale_log2, softcap;
@@ -70,6 +71,8 @@ __device__ __forceinline__ f32x4 mma16(u32x4 a, u32x4 b, f32x4 c) {
   return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8_t, a), __builtin_bit_cast(bf16x8_t, b), c, 0, 0,
                                                  0);
 }
+// bit 7 of every byte of w that is a NaN code (S.1111.111)
+__device__ __forceinline__ uint32_t nan_codes(uint32_t w) { return ((w & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u; }
 // maximum over the four lanes that share a query (l, l ^ 16, l ^ 32, l ^ 48)
 __device__ __forceinline__ float quad_max(float x) {
   const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
@@ -97,7 +100,7 @@ __device__ __forceinline__ float tanh_large(float x) {
 }
 // tanh of a lane's eight values; a wave whose values are all small or all
 // large (ALiBi's far keys) takes one form (B16 H16 Sq4 D64, 1500-key window:
-// 14.8 us with both always, 13.6 with the second alone, which is not exact).
+// 13.9 us, with both always 14.8, with the second alone, which is not exact, 13.6).
 __device__ __forceinline__ void tanh8(f32x4* x) {
   float lo = INFINITY, hi = 0.f;
 #pragma unroll
@@ -301,7 +304,8 @@ __device__ __forceinline__ DecodeUnit decode_unit(const DecodeArgs& a, int wg, b
   return u;
 }
 
-template <int D, int NQ, int NW, bool kMods, bool kStream>
+// kGeneral: score modifiers, or windows that differ between an item's rows
+template <int D, int NQ, int NW, bool kGeneral, bool kStream>
 __global__ __launch_bounds__(64 * NW, 2) void decode_fp8_kernel(DecodeArgs a) {
   using Tile = CodeTile<D, kStream>;
   constexpr int DV = Tile::DV, KC = Tile::KC, KW = Tile::KW;
@@ -343,7 +347,7 @@ __global__ __launch_bounds__(64 * NW, 2) void decode_fp8_kernel(DecodeArgs a) {
     qlo[n] = a.win_left < 0 ? 0 : max(qpos[n] - a.win_left, 0);
     qhi[n] = a.win_right < 0 ? have - 1 : (int)min((long long)have - 1, (long long)qpos[n] + a.win_right);
     if (i >= ql) qhi[n] = -1;  // a padded query sees nothing
-    slope[n] = kMods && a.alibi ? a.alibi[hk * a.g + hq] : 0.f;
+    slope[n] = kGeneral && a.alibi ? a.alibi[hk * a.g + hq] : 0.f;
   }
   const int vlo = a.win_left < 0 ? 0 : max(have - ql - a.win_left, 0);  // before it no row sees a key
 
@@ -415,13 +419,13 @@ __global__ __launch_bounds__(64 * NW, 2) void decode_fp8_kernel(DecodeArgs a) {
 #pragma unroll
         for (int i2 = 0; i2 < 4; ++i2) {
           const float raw = s[n][j][i2];
-          if constexpr (kMods) {
+          if constexpr (kGeneral) {
             s[n][j][i2] = fmaf(slope[n], (float)(k0 + 16 * j + 4 * i2 + g4 - qpos[n]), raw * a.scale) * mod_in;
           } else {
             s[n][j][i2] = raw * a.scale_log2;
           }
         }
-      if constexpr (kMods) {
+      if constexpr (kGeneral) {
         if (a.softcap > 0.f) tanh8(s[n]);
 #pragma unroll
         for (int j = 0; j < 2; ++j)
@@ -430,7 +434,8 @@ __global__ __launch_bounds__(64 * NW, 2) void decode_fp8_kernel(DecodeArgs a) {
       }
       whole = whole && qlo[n] <= k0 && qhi[n] >= k0 + kTileKeys - 1;
     }
-    if (!__all(whole)) {
+    const bool all_whole = __all(whole);
+    if (!all_whole) {
 #pragma unroll
       for (int n = 0; n < NQ; ++n)
 #pragma unroll
@@ -466,14 +471,55 @@ __global__ __launch_bounds__(64 * NW, 2) void decode_fp8_kernel(DecodeArgs a) {
         pl[n][y] = pack_bf16x2(p0 - bf16_lo(hi), p1 - bf16_hi(hi));
       }
     }
-    // keys that no row sees may hold anything (also NaN codes): P = 0 there must meet V = 0
     if (run < 0 || k0 < vlo || k0 + kTileKeys > have) {
+      // keys that no row sees may hold anything (also NaN codes): P = 0 there must meet V = 0
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
         const int key = k0 + 16 * (e >> 2) + 4 * (e & 3) + g4;
         const bool ok = run >= 0 && key >= vlo && key < have;
 #pragma unroll
         for (int y = 0; y < Tile::VW; ++y) x.v[e][y] = ok ? x.v[e][y] : 0u;
+      }
+    }
+    if (kGeneral && !all_whole) {  // (otherwise a row sees the item's keys or none)
+      // A NaN value code of a key that only some rows see must reach those alone, and
+      // P = 0 would not keep it from the others: it is taken out, and the rows that see
+      // one (a product of its flags and the rows' visible keys counts them) get NaN.
+      uint32_t bad = 0u;
+#pragma unroll
+      for (int e = 0; e < 8; ++e)
+#pragma unroll
+        for (int y = 0; y < Tile::VW; ++y) bad |= nan_codes(x.v[e][y]);
+      if (__any(bad != 0u)) {
+        u32x4 seen[NQ];
+#pragma unroll
+        for (int n = 0; n < NQ; ++n)
+#pragma unroll
+          for (int y = 0; y < 4; ++y) {
+            const int key = k0 + 16 * (y >> 1) + 8 * (y & 1) + g4;  // and key + 4
+            seen[n][y] = (key >= qlo[n] && key <= qhi[n] ? 0x3f80u : 0u) |
+                         (key + 4 >= qlo[n] && key + 4 <= qhi[n] ? 0x3f800000u : 0u);
+          }
+#pragma unroll
+        for (int t = 0; t < DV; ++t) {
+          u32x4 flag;
+#pragma unroll
+          for (int y = 0; y < 4; ++y) {
+            const int sh = 8 * (t & 3) + 7;
+            flag[y] = ((nan_codes(x.v[2 * y][t >> 2]) >> sh) & 1u) * 0x3f80u |
+                      ((nan_codes(x.v[2 * y + 1][t >> 2]) >> sh) & 1u) * 0x3f800000u;
+          }
+#pragma unroll
+          for (int n = 0; n < NQ; ++n) {
+            const f32x4 hits = mma16(flag, seen[n], f32x4{0.f, 0.f, 0.f, 0.f});
+#pragma unroll
+            for (int i2 = 0; i2 < 4; ++i2) acc[n][t][i2] = hits[i2] > 0.f ? __builtin_nanf("") : acc[n][t][i2];
+          }
+        }
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+#pragma unroll
+          for (int y = 0; y < Tile::VW; ++y) x.v[e][y] &= ~((nan_codes(x.v[e][y]) >> 7) * 0xffu);
       }
     }
 #pragma unroll
@@ -542,10 +588,11 @@ __global__ __launch_bounds__(64 * NW, 2) void decode_fp8_kernel(DecodeArgs a) {
       }
       if (u.slot < 0) {
         const size_t at = (size_t)(b * a.Hkv + hk) * R + row;
-        const float inv = L > 0.f ? 1.0f / L : (L == 0.f ? 0.f : L);  // (NaN is passed on)
+        const float inv = L > 0.f ? 1.0f / L : L;  // (NaN is passed on)
         uint16_t* o = static_cast<uint16_t*>(a.o) + at * D + d0;
 #pragma unroll
-        for (int t = 0; t < CW; t += 2) *reinterpret_cast<uint32_t*>(o + t) = pack_bf16x2(x[t] * inv, x[t + 1] * inv);
+        for (int t = 0; t < CW; t += 2)  // a row that saw nothing may have met 0 * NaN
+          *reinterpret_cast<uint32_t*>(o + t) = L == 0.f ? 0u : pack_bf16x2(x[t] * inv, x[t + 1] * inv);
         if (d0 == 0) a.lse[at] = L == 0.f ? -INFINITY : (M + log2f(L)) * kLn2;
       } else {
         const size_t at = (size_t)u.slot * (16 * NQ) + 16 * n + orow;
@@ -615,11 +662,13 @@ __global__ __launch_bounds__(256) void decode_fp8_merge(DecodeArgs a, int rows_p
     }
   }
   const size_t out = (size_t)orow;
-  const float inv = L > 0.f ? 1.0f / L : (L == 0.f ? 0.f : L);
+  const float inv = L > 0.f ? 1.0f / L : L;
+#pragma unroll
+  for (int k = 0; k < CPL; ++k) acc[k] = L == 0.f ? 0.f : acc[k] * inv;  // (not 0 * NaN)
   if (lane * CPL < D) {
     uint16_t* o = static_cast<uint16_t*>(a.o) + out * D + col;
-    if constexpr (CPL == 2) *reinterpret_cast<uint32_t*>(o) = pack_bf16x2(acc[0] * inv, acc[CPL - 1] * inv);
-    else *o = (uint16_t)(pack_bf16x2(acc[0] * inv, 0.f) & 0xffffu);
+    if constexpr (CPL == 2) *reinterpret_cast<uint32_t*>(o) = pack_bf16x2(acc[0], acc[CPL - 1]);
+    else *o = (uint16_t)(pack_bf16x2(acc[0], 0.f) & 0xffffu);
   }
   if (lane == 0) a.lse[out] = L == 0.f ? -INFINITY : (M + log2f(L)) * kLn2;
 }

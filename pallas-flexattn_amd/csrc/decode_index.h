@@ -44,7 +44,12 @@ FA_HD int decode_next_chunk(int chunk, int units, int pieces) {
 }
 FA_HD int decode_pieces(int n, int chunk) { return n / chunk + (n % chunk ? 1 : 0); }
 // Tiles [first, first + count) of piece p of an n-tile walk in `pieces`.
-FA_HD int decode_piece(int n, int pieces, int p) { return (int)((long long)n * p / pieces); }
+// (n p / pieces in 32 bits: the remainder's product stays under pieces^2, and an
+// item has at most about as many pieces as the call asks for in all, a few thousand)
+FA_HD int decode_piece(int n, int pieces, int p) {
+  const int q = n / pieces, r = n - q * pieces;
+  return q * p + r * p / pieces;
+}
 
 // Workgroups that a call needs at most: items, plus a piece more for every
 // chunk's worth of tiles (n / chunk each, and the chunks are `pieces` in all).

@@ -36,27 +36,27 @@ int launch_append(const AppendArgs& a, int D, bool fp8, hipStream_t s) {
   return launch_status();
 }
 
-template <int D, int NQ, int NW, bool M>
+template <int D, int NQ, int NW, bool G>
 static void run_decode(const DecodeArgs& a, bool stream, hipStream_t s) {
-  if (stream) hipLaunchKernelGGL((decode_fp8_kernel<D, NQ, NW, M, true>), dim3(a.grid), dim3(64 * NW), 0, s, a);
-  else hipLaunchKernelGGL((decode_fp8_kernel<D, NQ, NW, M, false>), dim3(a.grid), dim3(64 * NW), 0, s, a);
+  if (stream) hipLaunchKernelGGL((decode_fp8_kernel<D, NQ, NW, G, true>), dim3(a.grid), dim3(64 * NW), 0, s, a);
+  else hipLaunchKernelGGL((decode_fp8_kernel<D, NQ, NW, G, false>), dim3(a.grid), dim3(64 * NW), 0, s, a);
 }
 
-template <int D, bool M>
+template <int D, bool G>
 static void decode_nq(const DecodeArgs& a, int nq, bool stream, hipStream_t s) {
-  if (nq == 1 && a.by_item) run_decode<D, 1, 8, M>(a, stream, s);
-  else if (nq == 1) run_decode<D, 1, 4, M>(a, stream, s);
-  else run_decode<D, 2, 4, M>(a, stream, s);
+  if (nq == 1 && a.by_item) run_decode<D, 1, 8, G>(a, stream, s);
+  else if (nq == 1) run_decode<D, 1, 4, G>(a, stream, s);
+  else run_decode<D, 2, 4, G>(a, stream, s);
   if (a.by_item) return;
   const int rows = a.B * a.Hkv * a.g * a.Sq;
   hipLaunchKernelGGL((decode_fp8_merge<D>), dim3(cdiv(rows, 4)), dim3(256), 0, s, a, 16 * nq);
 }
 
-int launch_decode_fp8(const DecodeArgs& a, int D, int nq, bool mods, bool stream, hipStream_t s) {
+int launch_decode_fp8(const DecodeArgs& a, int D, int nq, bool general, bool stream, hipStream_t s) {
   switch (D) {
-    case 32: mods ? decode_nq<32, true>(a, nq, stream, s) : decode_nq<32, false>(a, nq, stream, s); break;
-    case 64: mods ? decode_nq<64, true>(a, nq, stream, s) : decode_nq<64, false>(a, nq, stream, s); break;
-    case 128: mods ? decode_nq<128, true>(a, nq, stream, s) : decode_nq<128, false>(a, nq, stream, s); break;
+    case 32: general ? decode_nq<32, true>(a, nq, stream, s) : decode_nq<32, false>(a, nq, stream, s); break;
+    case 64: general ? decode_nq<64, true>(a, nq, stream, s) : decode_nq<64, false>(a, nq, stream, s); break;
+    case 128: general ? decode_nq<128, true>(a, nq, stream, s) : decode_nq<128, false>(a, nq, stream, s); break;
     default: return FA_ERR_UNSUPPORTED;
   }
   return launch_status();

@@ -40,6 +40,6 @@ int launch_quant_fp8(const QuantArgs& a, hipStream_t s);
 // 16-row query blocks per work item, 1 or 2; stream: cache reads past the caches)
 int launch_rotary(const RotaryArgs& a, bool f32, bool vec, hipStream_t s);
 int launch_append(const AppendArgs& a, int D, bool fp8, hipStream_t s);
-int launch_decode_fp8(const DecodeArgs& a, int D, int nq, bool mods, bool stream, hipStream_t s);
+int launch_decode_fp8(const DecodeArgs& a, int D, int nq, bool general, bool stream, hipStream_t s);
 
 }  // namespace fa

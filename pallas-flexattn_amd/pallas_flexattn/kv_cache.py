@@ -95,7 +95,7 @@ def flex_decode_fp8(query, cache: Fp8KVCache, kv_lens=None, page_table=None, mas
                     query_lens=None):
     """Attention of each row's newest queries over an 8-bit paged cache (no
     gradient): ``query`` (B, Hq, Sq, D) bf16, ``cache`` an :class:`Fp8KVCache`, ``kv_lens`` (B,) the
-    keys of each row, the queries' own included (None: the whole page table).  Made for
+    keys of each row, the queries' own included (None: the whole page table; cut to it).  Made for
     short query blocks (decoding, speculative decoding, short chunks): the cache is read once for
     every 16 to 32 rows of Sq * Hq / Hkv, and each row's keys are split over as many workgroups as
     the batch needs.
@@ -105,7 +105,8 @@ def flex_decode_fp8(query, cache: Fp8KVCache, kv_lens=None, page_table=None, mas
     ``kv_lens[b] - query_lens[b] + i``, and the padded ones return O = 0 and LSE = -inf, as do
     queries that see no key.  ``mask_mod``: ``causal_mask``, ``sliding_window_mask`` or another window
     :class:`MaskSpec` without documents, over these positions; ``score_mod``: the built-in ALiBi
-    and soft-cap descriptors.  Page ids outside the cache read as zero keys.  Scales must be powers of
+    and soft-cap descriptors.  What no query of a row sees may be anything, and a NaN stored for a
+    key reaches the queries that see it alone.  Page ids outside the cache read as zero keys.  Scales must be powers of
     two (:func:`append_kv_cache` writes no others): the kernel reads their exponents only."""
     if not isinstance(cache, Fp8KVCache):
         raise TypeError("cache must be an Fp8KVCache")

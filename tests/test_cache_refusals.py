@@ -177,7 +177,7 @@ def _decode_q(data=16, **kw):
 
 @pytest.mark.parametrize("pkw,ckw,code", [
     (dict(abi_version=9), {}, -8), (dict(dtype=0), {}, -3), (dict(D=96), {}, -4), (dict(Hq=3), {}, -2), (dict(Sq=0), {}, -2),
-    (dict(Skv=129), {}, -2), (dict(softcap=-1.0), {}, -2), (dict(q_doc_ids=16), {}, -4), (dict(kv_num_blocks=16), {}, -4),
+    (dict(Skv=129), {}, -2), (dict(Skv=2 ** 31 - 1), dict(max_pages=1 << 25), -2), (dict(softcap=-1.0), {}, -2), (dict(q_doc_ids=16), {}, -4), (dict(kv_num_blocks=16), {}, -4),
     ({}, dict(page_size=40), -2), ({}, dict(page_table=None), -2), ({}, dict(v_scale=None), -1), ({}, dict(k=24), -2),
     ({}, dict(num_pages=1 << 30, page_size=1 << 20), -2), (dict(B=1 << 14, Sq=1 << 14), {}, -2)])
 def test_c_decode_refuses(pkw, ckw, code):

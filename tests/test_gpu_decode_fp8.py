@@ -190,6 +190,55 @@ def test_pages_before_the_window_may_be_anything():
     _check(o, lse, q, c, lens, None, left, 0)
 
 
+@pytest.mark.parametrize("D,Hq,Sq,left", [(128, 4, 4, -1), (64, 2, 40, 37), (32, 12, 5, 70)])
+def test_nan_reaches_the_queries_that_see_it(D, Hq, Sq, left):
+    """NaN in single elements of keys and values that some queries see and others, masked, do not."""
+    import torch
+    import pallas_flexattn as pf
+    lens = [150, 97]
+    c = Cache(lens, 1, 32, D, 50)
+    q = _q(2, Hq, Sq, D, 55)
+    dims = {0: (0, D - 1), 1: (3, D // 2)}  # of the values, per row
+    codes = [t.view(torch.uint8) for t in c.cache[:2]]
+    hit = np.zeros((2, Hq, Sq, D), bool)
+    for b, n in enumerate(lens):
+        # a value of the newest key, of the one before the last query's, and of one that a window ends on; a key's element
+        for pos, what in ((n - 1, "v"), (n - 2, "k"), (max(n - Sq - max(left, 0), 0), "v")):
+            page = c.table[b, pos // 32].long()
+            for i in range(Sq):
+                at = n - Sq + i
+                if pos <= at and (left < 0 or at - pos <= left):
+                    hit[b, :, i, list(dims[b]) if what == "v" else slice(None)] = True
+            if what == "v":
+                for d in dims[b]:
+                    codes[1][page, :, pos % 32, d] = 0x7f if d else 0xff
+            else:
+                codes[0][page, :, pos % 32, 1] = 0x7f
+    o, lse = pf.flex_decode_fp8(q, c.cache, c.lens, c.table, mask_mod=pf.sliding_window_mask(left, 0), enable_gqa=True,
+                                return_lse=True)
+    assert np.array_equal(np.isnan(_np(o)), hit)
+    wo, wl, _ = kv_cache.decode(_np(q), _np(c.rows[0]), _np(c.rows[1]), lens, None, left, 0)
+    clean = ~hit.any(-1)
+    np.testing.assert_allclose(_np(o)[~hit & clean[..., None]], wo[~hit & clean[..., None]], rtol=2.0 ** -7, atol=1e-3)
+
+
+@pytest.mark.parametrize("masked", [False, True])
+@pytest.mark.parametrize("n", [70, 2000])  # in one workgroup per item, in pieces
+def test_padded_queries_are_zero_beside_nan(n, masked):
+    """Padded queries give 0 and -inf also where every value that the others see is NaN."""
+    import torch
+    import pallas_flexattn as pf
+    c = Cache([n, n, n], 1, 32, 64, 51)
+    q = _q(3, 4, 3, 64, 52)
+    c.cache[1].view(torch.uint8).fill_(0x7f)
+    ql = torch.tensor([0, 1, 3], device="cuda")
+    o, lse = pf.flex_decode_fp8(q, c.cache, c.lens, c.table, mask_mod=pf.causal_mask if masked else None, enable_gqa=True,
+                                return_lse=True, query_lens=ql)
+    for b, m in enumerate((0, 1, 3)):
+        assert torch.isnan(o[b, :, :m]).all() and torch.isfinite(lse[b, :, :m]).all()
+        assert (o[b, :, m:] == 0).all() and (lse[b, :, m:] == float("-inf")).all()
+
+
 def test_more_queries_than_keys():
     """Queries before the first position see nothing (a row of 2 keys, 4 causal queries)."""
     import pallas_flexattn as pf
