@@ -383,8 +383,8 @@ enum { FA_KV_RUN = 32 };
  * table null: page b is row b's).  Tokens whose position lies past max_pages
  * pages, or whose page id is outside [0, num_pages), are dropped; everything
  * else in the cache is left as it was.  Keys are rotated to their positions
- * first (rotary.pairs 0: not).  The pages that a call writes belong to one
- * batch row each.
+ * first (rotary.pairs 0: not).  The pages that a call writes are
+ * distinct, each at one place of one row's table.
  * cache_dtype FA_DTYPE_BF16: k_cache, v_cache bf16 (fa_fwd_kvcache's layout).
  * FA_DTYPE_FP8_E4M3: codes; a run's scale is 2^e with e the smallest integer in
  * [-126, 127] such that 448 2^e >= the largest finite |x| of its tokens, from the float32

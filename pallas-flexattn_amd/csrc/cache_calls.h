@@ -20,7 +20,7 @@ int heads_per_thread(long long work) {
   return per < 1 ? 1 : per < 4 ? (int)per : 4;
 }
 
-// Threads of a rotary call per head.
+// Threads of a rotary call per head (B T < 2^31).
 long long rotary_units(fa::RotaryArgs* a, bool vec) {
   const int pairs = (a->n + 7) / 8;
   a->units = vec ? a->D / 16 : pairs + (a->D - 2 * a->n + 15) / 16;
@@ -39,6 +39,7 @@ int rotary_args(const fa_rotary_call* c, fa::RotaryArgs* a, bool* vec) {
   if (c->abi_version != FA_ABI_VERSION) return FA_ERR_VERSION;
   if (c->dtype != FA_DTYPE_BF16 && c->dtype != FA_DTYPE_F32) return FA_ERR_DTYPE;
   if (c->B < 1 || c->T < 1 || c->D < 1 || c->D > 1024 || c->count < 1 || c->count > 2) return FA_ERR_SHAPE;
+  if ((long long)c->B * c->T > 0x7fffffffll) return FA_ERR_SHAPE;
   if (c->rotary.pairs < 1 || 2 * (long long)c->rotary.pairs > c->D) return FA_ERR_SHAPE;
   if (!c->rotary.inv_freq) return FA_ERR_NULL;
   if (!aligned(c->rotary.inv_freq, 8) || !aligned(c->positions, c->positions_64 ? 8 : 4)) return FA_ERR_SHAPE;
@@ -52,6 +53,7 @@ int rotary_args(const fa_rotary_call* c, fa::RotaryArgs* a, bool* vec) {
     *vec = *vec && rows16(t, es) && aligned(c->out[i], 16);
     a->t[i] = {t.data, c->out[i], t.stride_b, t.stride_h, t.stride_t, t.heads};
   }
+  if (c->count == 2 && (long long)c->in[0].heads + c->in[1].heads > 0x7fffffffll) return FA_ERR_SHAPE;
   a->B = c->B;
   a->T = c->T;
   a->D = c->D;
@@ -65,6 +67,7 @@ int rotary_args(const fa_rotary_call* c, fa::RotaryArgs* a, bool* vec) {
   a->pos_stride = c->positions_stride;
   a->offset = c->offset;
   const long long threads = rotary_units(a, *vec);
+  if (threads > 0x7fffff00ll) return FA_ERR_SHAPE;
   return rotary_groups(a, threads, heads_per_thread(threads * (a->t[0].heads + a->t[1].heads)));
 }
 
@@ -112,6 +115,7 @@ int append_args(const fa_kv_append_call* c, fa::AppendArgs* a) {
     a->scale = c->rotary.scale;
   }
   const long long runs = ((long long)c->T + FA_KV_RUN - 2) / FA_KV_RUN + 1;
+  if (runs * c->B > 0x7fffffll) return FA_ERR_SHAPE;
   const long long token_threads = runs * FA_KV_RUN * c->B * (c->D / 16);
   a->runs = (int)runs;
   auto heads = [&](long long work) {  // `work`: as heads_per_thread, keys and queries together
@@ -171,7 +175,7 @@ int decode_args(const fa_params* p, const fa_fp8_cache* kv, int cus, fa::DecodeA
   *a = fa::DecodeArgs{};
   const int g = p->Hq / p->Hkv;
   const long long rows = (long long)g * p->Sq;
-  if (rows * p->B * p->Hkv > 0x7ffffffll) return FA_ERR_SHAPE;
+  if (rows > 0x7ffffffll || (long long)p->B * p->Hkv > 0x7ffffffll / rows) return FA_ERR_SHAPE;
   // tiles that a row walks at most: all of its keys', or the window's
   // (a window of at least all keys is none)
   const int left = p->window_left < 0 || p->window_left >= p->Skv ? -1 : p->window_left;

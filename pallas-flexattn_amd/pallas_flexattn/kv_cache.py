@@ -73,8 +73,8 @@ def append_kv_cache(cache, key, value, kv_lens, page_table=None, new_lens=None, 
     float32 values; NaN and infinities are stored as NaN.
 
     Tokens past the page table's last page, or on a page id outside the cache, are
-    dropped.  The pages that one call writes must belong to one row each (shared prefix
-    pages are read, never appended to).  ``page_size`` must be a multiple of 32; tokens of
+    dropped.  The pages that one call writes must be distinct, each at one place of one row's
+    table (shared prefix pages are read, never appended to).  ``page_size`` must be a multiple of 32; tokens of
     any strides whose rows are 16-byte aligned are read in place.  No gradient."""
     fp8 = isinstance(cache, Fp8KVCache)
     if not fp8 and not (isinstance(cache, (tuple, list)) and len(cache) == 2):

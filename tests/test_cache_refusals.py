@@ -125,6 +125,20 @@ def test_c_rotary_refuses(kw, code):
     assert _lib.load().fa_apply_rotary(None, None) == -1
 
 
+def test_c_calls_refuse_sizes_past_64_bits():
+    """Products of sizes that would pass 2^63 are refused as well, and head counts that add up past 2^31."""
+    lib, big = _lib.load(), 2 ** 31 - 1
+    c = _rotary_call(B=big, T=big, D=1024)
+    assert lib.fa_apply_rotary(ctypes.byref(c), None) == -2
+    c = _rotary_call(count=2, T=1)
+    for i in range(2):
+        c.in_[i], c.out[i] = _lib.FaStrided(16, 0, 64, 64, 1 << 30), 16
+    assert lib.fa_apply_rotary(ctypes.byref(c), None) == -2
+    assert lib.fa_kv_append(ctypes.byref(_append_call(B=big, T=big)), None) == -2
+    p, kv = _decode_params(B=1 << 30, Hq=1 << 30, Hkv=1 << 30, Sq=16), _decode_cache(num_pages=1)
+    assert lib.fa_fwd_kvcache_fp8(ctypes.byref(p), ctypes.byref(kv), _decode_q(heads=1 << 30), 16, 16, 16, 1 << 40, None) == -2
+
+
 def _append_call(**kw):
     c = _lib.FaKvAppendCall()
     c.abi_version, c.cache_dtype, c.B, c.T, c.D = _lib.ABI_VERSION, _lib.DTYPE_FP8_E4M3, 2, 4, 64
