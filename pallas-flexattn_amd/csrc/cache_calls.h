@@ -228,8 +228,11 @@ int decode_args(const fa_params* p, const fa_fp8_cache* kv, int cus, fa::DecodeA
   // 25.5, of 127 29.5 / 29.9, 256 of 121 45.2 / 49.8, 512 of 68 37.5 / 38.8, D = 64 512 of 65 19.9 / 22.3).
   // Pieces beyond: 8 of 126 25.6 / 13.0, 64 of 127 26.7 / 19.9, 32 of 127 with two blocks of rows
   // 27.4 / 21.2, 256 of mixed lengths to 257 61 / 55; they lose only on many equal
-  // long rows (D = 64 256 of 513 88 / 96). Over 256 rows are enough items as they are.
-  a->by_item = tiles <= 48 || (2ll * p->B * p->Hkv >= cus && tiles <= 128) || p->B > 64 * fa::kLaneRows;
+  // long rows (D = 64 256 of 513 88 / 96) and many items (1024 rows to 156 with four heads 262 / 298),
+  // and keep one long row among many from being the call's time (300 rows with one head to 981
+  // 317 / 96, one of 3125 among 299 of 16 540 / 37; 1024 to 254 131 / 126). Past 1024 rows each
+  // workgroup's search for its piece costs more than that.
+  a->by_item = tiles <= 48 || (2ll * p->B * p->Hkv >= cus && tiles <= 128) || p->B > 64 * fa::kMostLaneRows;
   // At most four pieces per unit (two where the rows are equally long: decode_unit).
   a->pieces = 4 * cus;
   // At least 16 tiles a piece, four per wave, so that the merge stays short (8 of 500

@@ -207,35 +207,25 @@ struct DecodeUnit {
   int item;              // kv head * rt + query block
   int t0, nt, slot;      // tiles, and the slot of a part of an item (-1: all of it)
 };
-// Every wave finds its workgroup's unit by itself: the lanes hold the rows'
-// tiles (up to kLaneRows consecutive rows each), scans give the chunk and the rows' first units.
-__device__ __forceinline__ DecodeUnit decode_unit(const DecodeArgs& a, int wg, bool first_wave) {
+// Every wave finds its workgroup's unit by itself: scans over the lanes, each of
+// which holds the tiles of up to kRows consecutive rows, give the chunk and the rows' first units.
+template <int kRows>
+__device__ __forceinline__ DecodeUnit decode_piece_unit(const DecodeArgs& a, int wg, bool first_wave) {
   const int each = a.Hkv * a.rt;
   DecodeUnit u;
-  if (a.by_item) {
-    u.b = wg / each;
-    u.item = wg - u.b * each;
-    u.have = a.kv_lens ? clamp_len(scalar_load(a.kv_lens, u.b), a.cap) : a.cap;
-    u.ql = a.q_lens ? clamp_len(scalar_load(a.q_lens, u.b), a.Sq) : a.Sq;
-    const DecodeSpan s = decode_span(u.have, u.ql, a.win_left);
-    u.t0 = s.lo;
-    u.nt = s.n;
-    u.slot = -1;
-    return u;
-  }
   const int lane = threadIdx.x & 63;
   const int per = (a.B + 63) / 64, b0 = lane * per;
-  int n[kLaneRows], sum = 0;  // tiles of this lane's rows, 0: no row
+  int n[kRows], sum = 0;  // tiles of this lane's rows, 0: no row
   bool same = true;
 #pragma unroll
-  for (int j = 0; j < kLaneRows; ++j) {
+  for (int j = 0; j < kRows; ++j) {
     const int b = b0 + j;
     n[j] = j < per && b < a.B ? decode_span(row_keys(a, b), row_queries(a, b), a.win_left).n : 0;
     sum += n[j];
   }
   const int n0 = __builtin_amdgcn_readfirstlane(n[0]);
 #pragma unroll
-  for (int j = 0; j < kLaneRows; ++j) same = same && (n[j] == 0 || n[j] == n0);
+  for (int j = 0; j < kRows; ++j) same = same && (n[j] == 0 || n[j] == n0);
   // Equal rows make equal pieces, two per compute unit; of unequal ones, whose
   // pieces differ by up to half, twice as many come out more even (GPU time with two / four:
   // 8 equal rows of 32768 keys 97 / 99 us, 32 of 3840 49.8 / 51.7, 32 mixed to 8192 59.8 / 54.9,
@@ -243,18 +233,19 @@ __device__ __forceinline__ DecodeUnit decode_unit(const DecodeArgs& a, int wg, b
   const int pieces = __all(same) ? a.pieces / 2 : a.pieces;
   const int total = __builtin_amdgcn_readlane(wave_scan(sum), 63) * each;
   int chunk = decode_chunk(total, pieces, a.least);
-  int p[kLaneRows], units, slots, iu;  // pieces per item, this lane's units and slots
+  int p[kRows], units, slots, iu;  // pieces per item, this lane's units and slots
   for (int i = 0;; ++i) {
     units = slots = 0;
 #pragma unroll
-    for (int j = 0; j < kLaneRows; ++j) {
+    for (int j = 0; j < kRows; ++j) {
       p[j] = decode_pieces(n[j], chunk);
       units += p[j] * each;
       slots += p[j] > 1 ? p[j] * each : 0;
     }
     iu = wave_scan(units);
     const int all = __builtin_amdgcn_readlane(iu, 63);
-    if (all <= pieces || a.B * each >= pieces || i == kChunkTries) break;
+    // (over hundreds of rows the rounding evens out, and a try costs a division per row)
+    if (all <= pieces || a.B * each >= pieces || i == (kRows > kLaneRows ? 0 : kChunkTries)) break;
     chunk = decode_next_chunk(chunk, all, pieces);
   }
   const int is = wave_scan(slots);
@@ -262,7 +253,7 @@ __device__ __forceinline__ DecodeUnit decode_unit(const DecodeArgs& a, int wg, b
   if (wg == 0 && first_wave) {  // for the merge
     int f = fu, g = fs;
 #pragma unroll
-    for (int j = 0; j < kLaneRows; ++j) {
+    for (int j = 0; j < kRows; ++j) {
       if (n[j]) {
         a.head[2 * (b0 + j)] = f;
         a.head[2 * (b0 + j) + 1] = g;
@@ -280,7 +271,7 @@ __device__ __forceinline__ DecodeUnit decode_unit(const DecodeArgs& a, int wg, b
   }
   int b = b0, nb = n[0], pb = p[0];
 #pragma unroll
-  for (int j = 1; j < kLaneRows; ++j) {
+  for (int j = 1; j < kRows; ++j) {
     const bool later = b == b0 + j - 1 && wg >= fu + pb * each && n[j] != 0;
     fu += later ? pb * each : 0;
     fs += later && pb > 1 ? pb * each : 0;
@@ -302,6 +293,27 @@ __device__ __forceinline__ DecodeUnit decode_unit(const DecodeArgs& a, int wg, b
   u.nt = decode_piece(nb, pb, piece + 1) - lo;
   u.slot = pb > 1 ? __builtin_amdgcn_readlane(fs, src) + local : -1;
   return u;
+}
+__device__ __forceinline__ DecodeUnit decode_unit(const DecodeArgs& a, int wg, bool first_wave) {
+  DecodeUnit u;
+  if (a.by_item) {
+    const int each = a.Hkv * a.rt;
+    u.b = wg / each;
+    u.item = wg - u.b * each;
+    u.have = a.kv_lens ? clamp_len(scalar_load(a.kv_lens, u.b), a.cap) : a.cap;
+    u.ql = a.q_lens ? clamp_len(scalar_load(a.q_lens, u.b), a.Sq) : a.Sq;
+    const DecodeSpan s = decode_span(u.have, u.ql, a.win_left);
+    u.t0 = s.lo;
+    u.nt = s.n;
+    u.slot = -1;
+  } else if (a.B <= 64 * kLaneRows) {
+    u = decode_piece_unit<kLaneRows>(a, wg, first_wave);
+  } else {
+    u = decode_piece_unit<kMostLaneRows>(a, wg, first_wave);
+  }
+  // (the compiler does not see that the branches' values are one per wave: four registers more)
+  auto uniform = [](int x) { return __builtin_amdgcn_readfirstlane(x); };
+  return DecodeUnit{uniform(u.b), uniform(u.have), uniform(u.ql), uniform(u.item), uniform(u.t0), uniform(u.nt), uniform(u.slot)};
 }
 
 // kGeneral: score modifiers, or windows that differ between an item's rows

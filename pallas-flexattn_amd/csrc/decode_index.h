@@ -13,7 +13,9 @@
 namespace fa {
 
 constexpr int kTileKeys = 32;  // keys of a tile: one scale run
-constexpr int kLaneRows = 4;   // batch rows that a lane of a wave keeps (calls cut in pieces: 256 rows)
+// Batch rows whose tiles a lane of a wave keeps, in calls to 256 rows and in larger ones (those
+// to 1024 are cut in pieces).
+constexpr int kLaneRows = 4, kMostLaneRows = 16;
 
 struct DecodeSpan {
   int lo;  // first tile

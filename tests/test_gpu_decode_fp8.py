@@ -145,6 +145,18 @@ def test_many_rows():
         _check(o, lse, q, c, lens)
 
 
+@pytest.mark.parametrize("B", [258, 319, 1023, 1024, 1025])
+def test_hundreds_of_rows(B):
+    """More rows than a wave's lanes hold four each of, up to sixteen each and past that."""
+    import pallas_flexattn as pf
+    lens = [(37 * i) % 90 for i in range(B)]
+    lens[B // 3], lens[B - 1] = 2500, 1700
+    c = Cache(lens, 1, 512, 32, 37, per_row=9)
+    q = _q(B, 2, 1, 32, 38)
+    o, lse = pf.flex_decode_fp8(q, c.cache, c.lens, c.table, enable_gqa=True, return_lse=True)
+    _check(o, lse, q, c, lens)
+
+
 def test_window_without_an_end():
     """Window sides past every key, at the largest 32-bit number and above it."""
     import pallas_flexattn as pf
