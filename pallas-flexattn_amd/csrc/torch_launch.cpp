@@ -480,10 +480,10 @@ PyObject* py_append(PyObject*, PyObject* const* a, Py_ssize_t n) {
 }
 
 // decode(q, k, v, k scale, v scale, kv_lens | None, table | None, q_lens | None, left, right, slopes | None,
-//        softcap, scale, gqa) -> (status, o, lse)
+//        softcap, scale, gqa, kv_len | None) -> (status, o, lse)
 PyObject* py_decode(PyObject*, PyObject* const* a, Py_ssize_t n) {
   HANDLE_TH_ERRORS
-  if (n != 14 || !g_decode) REFUSE(PyExc_TypeError, "decode takes 14 arguments, after bind_cache");
+  if (n != 15 || !g_decode) REFUSE(PyExc_TypeError, "decode takes 15 arguments, after bind_cache");
   const at::Tensor *q = tensor(a[0]), *k, *v, *ks, *vs, *lens, *table, *ql, *slopes;
   if (!q || !(k = tensor(a[1])) || !(v = tensor(a[2])) || !(ks = tensor(a[3])) || !(vs = tensor(a[4])) ||
       !optional(a[5], &lens) || !optional(a[6], &table) || !optional(a[7], &ql) || !optional(a[10], &slopes))
@@ -491,6 +491,7 @@ PyObject* py_decode(PyObject*, PyObject* const* a, Py_ssize_t n) {
   const int64_t left = std::min<int64_t>(PyLong_AsLong(a[8]), kMaxSize), right = std::min<int64_t>(PyLong_AsLong(a[9]), kMaxSize);
   const double softcap = PyFloat_AsDouble(a[11]), scale = PyFloat_AsDouble(a[12]);
   const int gqa = PyObject_IsTrue(a[13]);
+  const int64_t kv_len = a[14] == Py_None ? 0 : PyLong_AsLong(a[14]);
   if (PyErr_Occurred()) return nullptr;
   if (q->dim() != 4) REFUSE(PyExc_ValueError, "query must be (B, Hq, Sq, D)");
   if (q->scalar_type() != at::kBFloat16) REFUSE(PyExc_TypeError, "flex_decode_fp8 takes bfloat16 queries");
@@ -505,8 +506,10 @@ PyObject* py_decode(PyObject*, PyObject* const* a, Py_ssize_t n) {
   if (slopes && (slopes->scalar_type() != at::kFloat || slopes->dim() != 1 || slopes->size(0) != Hq))
     REFUSE(PyExc_ValueError, "ALiBi needs one slope per q head");
   if (!(scale >= 0.0) || !(softcap >= 0.0)) REFUSE(PyExc_ValueError, "scale must be positive");
-  const int64_t pages = table ? table->size(1) : 1, cap = pages * k->size(2);
-  if (!sizes_fit(*q) || cap > kMaxSize) REFUSE(PyExc_ValueError, "sizes must be below 2^31");
+  const int64_t pages = table ? table->size(1) : 1, all = pages * k->size(2);
+  if (a[14] != Py_None && (kv_len < 1 || kv_len > all)) REFUSE(PyExc_ValueError, "kv_len must be in [1, max_pages * page_size]");
+  const int64_t cap = kv_len ? kv_len : all;
+  if (!sizes_fit(*q) || pages > kMaxSize || cap > kMaxSize) REFUSE(PyExc_ValueError, "sizes must be below 2^31");
   const at::Device dev = q->device();
   if (!dev.is_cuda()) REFUSE(PyExc_ValueError, "query and cache must be on the GPU");
   if (k->device() != dev || v->device() != dev || ks->device() != dev || vs->device() != dev ||

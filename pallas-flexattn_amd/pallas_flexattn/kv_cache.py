@@ -92,10 +92,12 @@ def append_kv_cache(cache, key, value, kv_lens, page_table=None, new_lens=None, 
 
 def flex_decode_fp8(query, cache: Fp8KVCache, kv_lens=None, page_table=None, mask_mod=None, score_mod=None,
                     scale: Optional[float] = None, enable_gqa: bool = False, return_lse: bool = False,
-                    query_lens=None):
+                    query_lens=None, kv_len: Optional[int] = None):
     """Attention of each row's newest queries over an 8-bit paged cache (no
     gradient): ``query`` (B, Hq, Sq, D) bf16, ``cache`` an :class:`Fp8KVCache`, ``kv_lens`` (B,) the
-    keys of each row, the queries' own included (None: the whole page table; cut to it).  Made for
+    keys of each row, the queries' own included (None: ``kv_len`` of them).  ``kv_len``: the most keys
+    that a row can have (None: the whole page table); longer rows are cut to it.  The work is
+    divided by it: a bound near the longest row is faster than a table made for far longer ones.  Made for
     short query blocks (decoding, speculative decoding, short chunks): the cache is read once for
     every 16 to 32 rows of Sq * Hq / Hkv, and each row's keys are split over as many workgroups as
     the batch needs.
@@ -122,7 +124,7 @@ def flex_decode_fp8(query, cache: Fp8KVCache, kv_lens=None, page_table=None, mas
     if scale is not None and not scale > 0:
         raise ValueError("scale must be positive")
     rc, o, lse = _lib.launcher().decode(query, *cache, _rows(kv_lens, query), page_table, _rows(query_lens, query), left,
-                                        right, slopes, cap, 0.0 if scale is None else scale, enable_gqa)
+                                        right, slopes, cap, 0.0 if scale is None else scale, enable_gqa, kv_len)
     if rc:
         _lib.check(rc)
     return (o, lse) if return_lse else o

@@ -125,6 +125,13 @@ def test_c_rotary_refuses(kw, code):
     assert _lib.load().fa_apply_rotary(None, None) == -1
 
 
+@pytest.mark.parametrize("kv_len,err", [(0, ValueError), (-1, ValueError), (129, ValueError), (2 ** 40, ValueError), (1.5, TypeError)])
+def test_decode_refuses_kv_len(kv_len, err):
+    with pytest.raises(err):
+        pf.flex_decode_fp8(_t(2, 4, 1, 64), _cache(pages=1), torch.zeros(2, dtype=torch.int32),
+                           torch.zeros(2, 2, dtype=torch.int32), enable_gqa=True, kv_len=kv_len)
+
+
 def test_c_calls_refuse_sizes_past_64_bits():
     """Products of sizes that would pass 2^63 are refused as well, and head counts that add up past 2^31."""
     lib, big = _lib.load(), 2 ** 31 - 1

@@ -157,6 +157,23 @@ def test_hundreds_of_rows(B):
     _check(o, lse, q, c, lens)
 
 
+def test_kv_len_bounds_the_keys():
+    """A bound on the keys under the table's width: same results, longer rows cut, rows without lengths that long."""
+    import pallas_flexattn as pf
+    lens = [70, 33, 0, 512]
+    c = Cache(lens, 2, 64, 64, 38, per_row=60)
+    q = _q(4, 4, 2, 64, 39)
+    kw = dict(mask_mod=pf.causal_mask, enable_gqa=True, return_lse=True)
+    for bound in (512, 513, 3839, 3840):
+        o, lse = pf.flex_decode_fp8(q, c.cache, c.lens, c.table, kv_len=bound, **kw)
+        _check(o, lse, q, c, lens, None, -1, 0)
+    o, lse = pf.flex_decode_fp8(q, c.cache, c.lens, c.table, kv_len=50, **kw)
+    _check(o, lse, q, c, [min(n, 50) for n in lens], None, -1, 0)
+    o, lse = pf.flex_decode_fp8(q, c.cache, None, c.table, kv_len=33, **kw)
+    want, wl = pf.flex_decode_fp8(q, c.cache, [33] * 4, c.table, kv_len=33, **kw)
+    assert (o[:2] == want[:2]).all() and (lse[:2] == wl[:2]).all()
+
+
 def test_window_without_an_end():
     """Window sides past every key, at the largest 32-bit number and above it."""
     import pallas_flexattn as pf
