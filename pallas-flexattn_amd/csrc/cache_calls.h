@@ -223,16 +223,17 @@ int decode_args(const fa_params* p, const fa_fp8_cache* kv, int cus, fa::DecodeA
   // How the walk is cut (csrc/decode_index.h), from the longest walk that the
   // sizes allow; GPU time per call in us in replayed graphs, D = 128 unless named, by item in
   // eight waves / in pieces of four.  One workgroup per item, without a second launch, where
-  // walks are short (8 items of 16 tiles 7.2 / 10.7, 128 of 34 11.4 / 14.8, at 48 about even)
-  // or where the kv heads fill half of the units and no walk is very long (128 of 96 24.4 /
-  // 25.5, of 127 29.5 / 29.9, 256 of 121 45.2 / 49.8, 512 of 68 37.5 / 38.8, D = 64 512 of 65 19.9 / 22.3).
-  // Pieces beyond: 8 of 126 25.6 / 13.0, 64 of 127 26.7 / 19.9, 32 of 127 with two blocks of rows
-  // 27.4 / 21.2, 256 of mixed lengths to 257 61 / 55; they lose only on many equal
-  // long rows (D = 64 256 of 513 88 / 96) and many items (1024 rows to 156 with four heads 262 / 298),
-  // and keep one long row among many from being the call's time (300 rows with one head to 981
-  // 317 / 96, one of 3125 among 299 of 16 540 / 37; 1024 to 254 131 / 126). Past 1024 rows each
-  // workgroup's search for its piece costs more than that.
-  a->by_item = tiles <= 48 || (2ll * p->B * p->Hkv >= cus && tiles <= 128) || p->B > 64 * fa::kMostLaneRows;
+  // walks are short (8 items of 16 tiles 7.2 / 10.7, 128 of 34 11.4 / 14.8, of up to 61 16.8 / 16.6)
+  // or where the kv heads fill the units and no walk is very long (256 of 121 45.2 / 49.8, of up to
+  // 118 30.3 / 30.8, most of them short 25.5 / 20.1; 512 of 68 37.5 / 38.8, of up to 127 59.4 / 56.1,
+  // D = 64 512 of 65 19.9 / 22.3).  Pieces beyond: 8 of 126 25.6 / 13.0, 128 of up to 122 27.8 / 23.2,
+  // of 125 29.8 / 28.7, 64 of 127 26.7 / 19.9, 32 of 127 with two blocks of rows 27.4 / 21.2, 256 of
+  // mixed lengths to 257 61 / 55; they lose on many equal long rows (D = 64 256 of 513 88 / 96) and
+  // many items (1024 rows to 156 with four heads 262 / 298), and keep one long row among many from
+  // being the call's time (300 rows with one head to 981 317 / 96, one of 3125 among 299 of 16
+  // 540 / 37; 1024 to 254 131 / 126). Past 1024 rows each workgroup's search for its piece costs
+  // more than that.
+  a->by_item = tiles <= 48 || ((long long)p->B * p->Hkv >= cus && tiles <= 128) || p->B > 64 * fa::kMostLaneRows;
   // At most four pieces per unit (two where the rows are equally long: decode_unit).
   a->pieces = 4 * cus;
   // At least 16 tiles a piece, four per wave, so that the merge stays short (8 of 500
