@@ -82,6 +82,8 @@ CASES = [
     ([2000, 40], 8, 2, 5, 128, 256, (100, 0), 1), ([333, 0, 90], 4, 4, 20, 64, 64, (50, 0), 0), ([640], 16, 2, 9, 128, 64, (-1, 0), 0),
     ([100, 7], 2, 1, 70, 32, 32, (-1, 0), 1), ([5000], 8, 8, 1, 128, 512, None, 0), ([90, 4000], 4, 1, 2, 64, 32, (1000, -1), 0),
     ([50, 60], 4, 2, 3, 128, 64, (-1, 2), 0), ([65] * 70, 2, 2, 1, 32, 32, None, 0), ([17, 450] * 140, 2, 1, 1, 32, 32, None, 0),
+    # chunks of a prompt: hundreds of rows per kv head, more queries than keys in a row, odd row counts
+    ([900, 350, 1700], 4, 2, 700, 64, 64, (-1, 0), 0), ([3001], 3, 1, 513, 128, 64, (200, 0), 1), ([400, 2], 2, 2, 301, 32, 32, (-1, 5), 0),
 ]
 
 
