@@ -212,6 +212,11 @@ struct Turn {  // how a rotary call turns, besides its tensors
   int64_t offset;
 };
 
+// Whether a forward-mode derivative (a dual tensor's tangent) comes with t: nothing here computes one, and a
+// dual tensor need not require grad.
+bool has_tangent(const at::Tensor& t) { return t.defined() && t._fw_grad(0).defined(); }
+const char* const kTangentText = "apply_rotary has no forward-mode derivative";
+
 // fa_apply_rotary on checked tensors; k and pos may be undefined.
 std::vector<at::Tensor> turn(const at::Tensor& q, const at::Tensor& k, const at::Tensor& f, const at::Tensor& pos,
                              const Turn& t) {
@@ -281,6 +286,7 @@ struct RotaryFunction : torch::autograd::Function<RotaryFunction> {
     at::Tensor gk = g.size() > 1 && ctx->needs_input_grad(1) ? g[1] : at::Tensor();
     torch::autograd::variable_list out(8);
     if (!gq.defined() && !gk.defined()) return out;
+    TORCH_CHECK_NOT_IMPLEMENTED(!has_tangent(gq) && !has_tangent(gk), kTangentText);
     const bool first = gq.defined();
     const at::Tensor a = first ? gq : gk, b = first ? gk : at::Tensor();
     const auto r = at::GradMode::is_enabled()
@@ -320,6 +326,7 @@ PyObject* py_rotary(PyObject*, PyObject* const* a, Py_ssize_t n) {
     if (!row && !(pos->dim() == 2 && pos->size(1) == T && (pos->size(0) == B || pos->size(0) == 1)))
       REFUSE(PyExc_ValueError, "positions must be (T,), (1, T) or (B, T)");
   }
+  if (has_tangent(*q) || (k && has_tangent(*k)) || has_tangent(*f)) REFUSE(PyExc_NotImplementedError, kTangentText);
   const at::Device dev = q->device();
   if (!dev.is_cuda()) REFUSE(PyExc_ValueError, "query and key must be GPU tensors");
   if ((k && k->device() != dev) || f->device() != dev || (pos && pos->device() != dev))
