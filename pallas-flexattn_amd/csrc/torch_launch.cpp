@@ -327,6 +327,8 @@ PyObject* py_rotary(PyObject*, PyObject* const* a, Py_ssize_t n) {
       REFUSE(PyExc_ValueError, "positions must be (T,), (1, T) or (B, T)");
   }
   if (has_tangent(*q) || (k && has_tangent(*k)) || has_tangent(*f)) REFUSE(PyExc_NotImplementedError, kTangentText);
+  if (f->requires_grad() && at::GradMode::is_enabled())
+    REFUSE(PyExc_NotImplementedError, "apply_rotary has no gradient of inv_freq: detach it");
   const at::Device dev = q->device();
   if (!dev.is_cuda()) REFUSE(PyExc_ValueError, "query and key must be GPU tensors");
   if ((k && k->device() != dev) || f->device() != dev || (pos && pos->device() != dev))

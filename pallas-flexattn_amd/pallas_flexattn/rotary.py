@@ -74,7 +74,8 @@ def apply_rotary(query, key, rotary: Rotary, positions=None, offset: int = 0):
     """Rotates ``query`` (B, Hq, T, D) and ``key`` (B, Hkv, T, D) (or None) to
     their positions in one launch -> (query', key'), or query' alone without a key.
     Differentiable in query and key (the gradient is the rotation back; to any
-    order); forward-mode derivatives are refused.
+    order); forward-mode derivatives are refused, and an ``inv_freq`` that
+    requires grad in grad mode.
 
     Token t of row b is at ``positions[b, t]`` (int32 or int64, (T,) or (B, T), on the
     GPU), or at ``offset + t`` without positions.  bfloat16 or float32 with any

@@ -40,3 +40,18 @@ def test_forward_mode_over_the_gradient_is_refused(create_graph):
             torch.autograd.grad(y, q, forward_ad.make_dual(g, torch.ones_like(g)), retain_graph=True, create_graph=create_graph)
         # (an ordinary gradient inside a dual level is one)
         assert torch.equal(torch.autograd.grad(y, q, g, retain_graph=True, create_graph=create_graph)[0], want)
+
+
+def test_frequencies_that_require_grad_are_refused():
+    """They would get no gradient.  (Without grad mode, or detached, they are numbers like any other: the next check, of the
+    device, is reached.)"""
+    rot = pf.rotary_embedding(32, device="cpu")
+    rot.inv_freq.requires_grad_()
+    q = torch.ones(1, 2, 3, 64)
+    for x in (q, q.clone().requires_grad_()):
+        with pytest.raises(NotImplementedError, match="inv_freq"):
+            pf.apply_rotary(x, None, rot)
+        with pytest.raises(ValueError, match="GPU"):
+            pf.apply_rotary(x, None, rot._replace(inv_freq=rot.inv_freq.detach()))
+    with torch.no_grad(), pytest.raises(ValueError, match="GPU"):
+        pf.apply_rotary(q, None, rot)
