@@ -482,6 +482,9 @@ PyObject* py_append(PyObject*, PyObject* const* a, Py_ssize_t n) {
       c.rotary.scale = static_cast<float>(scale);
     }
     rc = g_append(&c, stream_of(dev));
+    // written through raw pointers: autograd learns of it here (inference tensors have no version)
+    for (const at::Tensor* t : {kc, vc, ks, vs})
+      if (rc == FA_OK && t && !t->is_inference()) t->unsafeGetTensorImpl()->bump_version();
   }
   if (!q) return Py_BuildValue("iO", rc, Py_None);
   return Py_BuildValue("iN", rc, THPVariable_Wrap(out));
