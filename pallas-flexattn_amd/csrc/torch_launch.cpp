@@ -414,6 +414,7 @@ PyObject* py_append(PyObject*, PyObject* const* a, Py_ssize_t n) {
   const int interleaved = PyObject_IsTrue(a[10]);
   const double scale = PyFloat_AsDouble(a[11]);
   if (PyErr_Occurred()) return nullptr;
+  if (!ks != !vs) REFUSE(PyExc_TypeError, "an 8-bit cache has key and value scales");
   if (k->dim() != 4 || k->sizes() != v->sizes() || (q && q->dim() != 4))
     REFUSE(PyExc_ValueError, "key and value must both be (B, Hkv, T, D), query (B, Hq, T, D)");
   if (k->scalar_type() != at::kBFloat16 || v->scalar_type() != at::kBFloat16 || (q && q->scalar_type() != at::kBFloat16))
