@@ -412,7 +412,8 @@ int fa_kv_append(const fa_kv_append_call *c, void *stream);
  * q_lens[b] (null: Sq) sits at position kv_lens[b] - q_lens[b] + i, which is
  * what p's window and ALiBi refer to; queries i >= q_lens[b] give o = 0 and
  * lse = -inf, as do queries that see no key.  Page ids outside the cache read
- * as zero keys.  Document ids and block tables are refused.  Workgroups take
+ * as zero keys.  Document ids and block tables are refused, and a scale or soft-cap
+ * that is neither 0 (the default, none) nor a positive normal number.  Workgroups take
  * equal shares of all rows' tiles of 32 keys; the partial results of items
  * that several of them share are joined in a fixed order by a second launch.
  * The workspace is 16-byte aligned, of the size that the other function gives (0:

@@ -161,7 +161,8 @@ int decode_args(const fa_params* p, const fa_fp8_cache* kv, int cus, fa::DecodeA
   if (p->B < 1 || p->Hq < 1 || p->Hkv < 1 || p->Hq % p->Hkv || p->Sq < 1 || p->Skv < 1 ||
       p->Skv > 0x7fffffff - 2 * fa::kTileKeys)
     return FA_ERR_SHAPE;
-  if (!(p->softcap >= 0.f) || !(p->scale >= 0.f)) return FA_ERR_SHAPE;
+  auto number = [](float x) { return x == 0.f || (x >= FLT_MIN && x <= FLT_MAX); };
+  if (!number(p->softcap) || !number(p->scale)) return FA_ERR_SHAPE;
   if (p->q_doc_ids || p->kv_doc_ids || p->doc_start || p->doc_end || p->kv_num_blocks || p->kv_indices ||
       p->full_kv_num_blocks || p->full_kv_indices)
     return FA_ERR_UNSUPPORTED;

@@ -20,6 +20,7 @@
 #include <c10/hip/HIPStream.h>
 
 #include <algorithm>
+#include <cfloat>
 #include <cstdint>
 
 #include "../../include/flexattn.h"
@@ -519,6 +520,9 @@ PyObject* py_decode(PyObject*, PyObject* const* a, Py_ssize_t n) {
   if (slopes && (slopes->scalar_type() != at::kFloat || slopes->dim() != 1 || slopes->size(0) != Hq))
     REFUSE(PyExc_ValueError, "ALiBi needs one slope per q head");
   if (!(scale >= 0.0) || !(softcap >= 0.0)) REFUSE(PyExc_ValueError, "scale must be positive");
+  // (0: the default scale, no soft-cap: nothing else may become it)
+  auto fits = [](double x) { return x == 0.0 || (x >= FLT_MIN && x <= FLT_MAX); };
+  if (!fits(scale) || !fits(softcap)) REFUSE(PyExc_ValueError, "scale and soft-cap must be normal float32 numbers");
   const int64_t pages = table ? table->size(1) : 1, all = pages * k->size(2);
   if (a[14] != Py_None && (kv_len < 1 || kv_len > all)) REFUSE(PyExc_ValueError, "kv_len must be in [1, max_pages * page_size]");
   const int64_t cap = kv_len ? kv_len : all;
