@@ -429,6 +429,10 @@ size_t fa_fwd_kvcache_fp8_workspace_bytes(const fa_params *p, const fa_fp8_cache
 int fa_fwd_kvcache_fp8(const fa_params *p, const fa_fp8_cache *kv, const fa_strided *q, void *o, float *lse,
                        void *workspace, size_t workspace_bytes, void *stream);
 
+/* y[i] = x[i], n of them (device): lengths and page ids of callers that hold them
+ * in 64 bits.  What 32 bits do not hold becomes INT32_MIN or INT32_MAX. */
+int fa_int64_to_int32(const int64_t *x, int32_t *y, int64_t n, void *stream);
+
 /*
  * Block-mask construction on the device (create_block_mask, block_mask.py:54-129)
  * for the mask semantics of fa_params: the window (window_left, window_right)

@@ -664,6 +664,12 @@ int fa_kv_append(const fa_kv_append_call* c, void* stream) {
   return fa::launch_append(a, c->D, c->cache_dtype == FA_DTYPE_FP8_E4M3, static_cast<hipStream_t>(stream));
 }
 
+int fa_int64_to_int32(const int64_t* x, int32_t* y, int64_t n, void* stream) {
+  if (!x || !y) return FA_ERR_NULL;
+  if (n < 1 || n > 0x7fffff00ll || !aligned(x, 8) || !aligned(y, 4)) return FA_ERR_SHAPE;
+  return fa::launch_saturate(x, y, n, static_cast<hipStream_t>(stream));
+}
+
 size_t fa_fwd_kvcache_fp8_workspace_bytes(const fa_params* p, const fa_fp8_cache* kv) {
   fa::DecodeArgs a;
   DecodeLayout L;

@@ -62,4 +62,14 @@ int launch_decode_fp8(const DecodeArgs& a, int D, int nq, bool general, bool str
   return launch_status();
 }
 
+__global__ __launch_bounds__(256) void saturate_kernel(const int64_t* x, int32_t* y, unsigned n) {
+  const unsigned i = blockIdx.x * 256u + threadIdx.x;
+  if (i < n) y[i] = (int32_t)min(max(x[i], (int64_t)INT32_MIN), (int64_t)INT32_MAX);
+}
+
+int launch_saturate(const int64_t* x, int32_t* y, long long n, hipStream_t s) {
+  hipLaunchKernelGGL(saturate_kernel, dim3((unsigned)((n + 255) / 256)), dim3(256), 0, s, x, y, (unsigned)n);
+  return launch_status();
+}
+
 }  // namespace fa

@@ -35,11 +35,12 @@ int launch_fwd_fp8(const Fp8FwdArgs& a, int D, bool mods, bool q16, hipStream_t 
 int launch_quant_fp8(const QuantArgs& a, hipStream_t s);
 
 // Around a KV cache (kernels_cache.hip): rotary positions (f32 or bf16; vec:
-// 16-byte accesses), appends (D = 32, 64 or 128) and decode over e4m3 pages
-// (nq:
-// 16-row query blocks per work item, 1 or 2; stream: cache reads past the caches)
+// 16-byte accesses), appends (D = 32, 64 or 128), decode over e4m3 pages
+// (nq: 16-row query blocks per work item, 1 or 2; stream: cache reads past the
+// caches), and n < 2^31 64-bit lengths or page ids as 32-bit ones
 int launch_rotary(const RotaryArgs& a, bool f32, bool vec, hipStream_t s);
 int launch_append(const AppendArgs& a, int D, bool fp8, hipStream_t s);
 int launch_decode_fp8(const DecodeArgs& a, int D, int nq, bool general, bool stream, hipStream_t s);
+int launch_saturate(const int64_t* x, int32_t* y, long long n, hipStream_t s);
 
 }  // namespace fa

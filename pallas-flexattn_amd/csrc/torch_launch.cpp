@@ -138,19 +138,22 @@ decltype(&fa_apply_rotary) g_rotary = nullptr;
 decltype(&fa_kv_append) g_append = nullptr;
 decltype(&fa_fwd_kvcache_fp8) g_decode = nullptr;
 decltype(&fa_fwd_kvcache_fp8_workspace_bytes) g_decode_ws = nullptr;
+decltype(&fa_int64_to_int32) g_saturate = nullptr;
 decltype(&fa_strerror) g_strerror = nullptr;
 
-// bind_cache(fa_apply_rotary, fa_kv_append, fa_fwd_kvcache_fp8, fa_fwd_kvcache_fp8_workspace_bytes, fa_strerror)
+// bind_cache(fa_apply_rotary, fa_kv_append, fa_fwd_kvcache_fp8, fa_fwd_kvcache_fp8_workspace_bytes,
+//            fa_int64_to_int32, fa_strerror)
 PyObject* py_bind_cache(PyObject*, PyObject* const* a, Py_ssize_t n) {
-  if (n != 5) {
-    PyErr_SetString(PyExc_TypeError, "bind_cache takes 5 addresses");
+  if (n != 6) {
+    PyErr_SetString(PyExc_TypeError, "bind_cache takes 6 addresses");
     return nullptr;
   }
   g_rotary = reinterpret_cast<decltype(g_rotary)>(address(a[0]));
   g_append = reinterpret_cast<decltype(g_append)>(address(a[1]));
   g_decode = reinterpret_cast<decltype(g_decode)>(address(a[2]));
   g_decode_ws = reinterpret_cast<decltype(g_decode_ws)>(address(a[3]));
-  g_strerror = reinterpret_cast<decltype(g_strerror)>(address(a[4]));
+  g_saturate = reinterpret_cast<decltype(g_saturate)>(address(a[4]));
+  g_strerror = reinterpret_cast<decltype(g_strerror)>(address(a[5]));
   if (PyErr_Occurred()) return nullptr;
   Py_RETURN_NONE;
 }
@@ -199,13 +202,18 @@ bool freq_ok(const at::Tensor& f, int64_t D) {
   return f.dim() == 1 && f.scalar_type() == at::kDouble && f.is_contiguous() && f.size(0) >= 1 && 2 * f.size(0) <= D;
 }
 
-// A vector of one int per batch row as int32 on dev.
-at::Tensor row_ints(const at::Tensor& t, const at::Device& dev) {
-  if (t.scalar_type() == at::kInt && t.device() == dev && t.is_contiguous()) return t;
-  return t.to(dev, at::kInt).contiguous();
-}
-
 void* stream_of(const at::Device& dev) { return c10::hip::getCurrentHIPStream(dev.index()).stream(); }
+
+// Lengths or page ids, int32 or int64, as dense int32 on dev (the current device).  What 32 bits do not hold becomes
+// their first or last number: a page or a length as impossible as it.
+at::Tensor row_ints(const at::Tensor& t, const at::Device& dev) {
+  if (t.scalar_type() == at::kInt) return t.device() == dev && t.is_contiguous() ? t : t.to(dev).contiguous();
+  const at::Tensor x = t.to(dev).contiguous();
+  at::Tensor y = at::empty(x.sizes(), x.options().dtype(at::kInt));
+  const int rc = x.numel() ? g_saturate(x.const_data_ptr<int64_t>(), y.mutable_data_ptr<int32_t>(), x.numel(), stream_of(dev)) : FA_OK;
+  TORCH_CHECK(rc == FA_OK, "flexattn C ABI error ", rc, ": ", g_strerror(rc));
+  return y;
+}
 
 struct Turn {  // how a rotary call turns, besides its tensors
   bool interleaved, inverse;

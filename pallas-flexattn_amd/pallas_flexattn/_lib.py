@@ -115,7 +115,8 @@ EXPORTED = ("fa_fwd", "fa_fwd_fp8", "fa_fwd_fp8_q16", "fa_quantize_fp8", "fa_qua
             "fa_mask_build_workspace_bytes", "fa_build_block_mask", "fa_strerror", "fa_abi_version",
             "fa_mods_compile", "fa_mods_free_blob", "fa_mods_load", "fa_mods_unload", "fa_mods_fwd", "fa_mods_bwd",
             "fa_mods_bwd_dkdv", "fa_mods_bwd_dq", "fa_mods_source_hash",
-            "fa_apply_rotary", "fa_kv_append", "fa_fwd_kvcache_fp8", "fa_fwd_kvcache_fp8_workspace_bytes")
+            "fa_apply_rotary", "fa_kv_append", "fa_fwd_kvcache_fp8", "fa_fwd_kvcache_fp8_workspace_bytes",
+            "fa_int64_to_int32")
 
 MODS_MASK, MODS_SCORE, MODS_BUILTIN_SCORE, MODS_GENERAL = 1, 2, 4, 8
 
@@ -215,6 +216,8 @@ def load():
     lib.fa_fwd_kvcache_fp8.restype = i
     lib.fa_fwd_kvcache_fp8_workspace_bytes.argtypes = [P, FC]
     lib.fa_fwd_kvcache_fp8_workspace_bytes.restype = ctypes.c_size_t
+    lib.fa_int64_to_int32.argtypes = [v, v, ctypes.c_int64, v]
+    lib.fa_int64_to_int32.restype = i
     lib.fa_strerror.argtypes = [ctypes.c_int]
     lib.fa_strerror.restype = ctypes.c_char_p
     lib.fa_mods_source_hash.argtypes = []
@@ -249,7 +252,7 @@ def launcher():
                                                                             lib.fa_bwd_split_workspace_bytes)))
         ext.bind_cache(*(ctypes.cast(f, ctypes.c_void_p).value for f in (
             lib.fa_apply_rotary, lib.fa_kv_append, lib.fa_fwd_kvcache_fp8, lib.fa_fwd_kvcache_fp8_workspace_bytes,
-            lib.fa_strerror)))
+            lib.fa_int64_to_int32, lib.fa_strerror)))
         _launch = ext
     return _launch
 

@@ -6,6 +6,9 @@ batch row b sits in row t % page_size of page ``page_table[b, t // page_size]``.
 a (key, value) pair of tensors, read by ``flex_decode``; in 8 bits an :class:`Fp8KVCache`
 (OCP e4m3 with one power-of-two scale for each 32 tokens of a head), half the
 bytes, read by :func:`flex_decode_fp8`.  :func:`append_kv_cache` fills either.
+
+Lengths and page tables are int32 (read as they are) or int64, on the GPU; int64 ones cost a
+small launch each, in which numbers past 32 bits become the nearest that 32 bits hold.
 """
 from typing import NamedTuple, Optional
 

@@ -53,3 +53,9 @@ def test_c_decode_numbers(field, x):
     p, c = _decode_params(Skv=1 << 20, **{field: x}), _decode_cache(max_pages=1 << 14)
     assert lib.fa_fwd_kvcache_fp8(ctypes.byref(p), ctypes.byref(c), None, 16, 16, 16, 1 << 40, None) == -2
     assert lib.fa_fwd_kvcache_fp8_workspace_bytes(ctypes.byref(p), ctypes.byref(c)) == 0
+
+
+@pytest.mark.parametrize("a,code", [((None, 16, 1), -1), ((16, None, 1), -1), ((16, 16, 0), -2), ((16, 16, -1), -2),
+                                    ((16, 16, 2 ** 31), -2), ((12, 16, 1), -2), ((16, 18, 1), -2)])
+def test_c_int64_to_int32_refuses(a, code):
+    assert _lib.load().fa_int64_to_int32(*a, None) == code
