@@ -233,8 +233,10 @@ int decode_args(const fa_params* p, const fa_fp8_cache* kv, int cus, fa::DecodeA
   // many items (1024 rows to 156 with four heads 262 / 298), and keep one long row among many from
   // being the call's time (300 rows with one head to 981 317 / 96, one of 3125 among 299 of 16
   // 540 / 37; 1024 to 254 131 / 126). Past 1024 rows each workgroup's search for its piece costs
-  // more than that.
-  a->by_item = tiles <= 48 || ((long long)p->B * p->Hkv >= cus && tiles <= 128) || p->B > 64 * fa::kMostLaneRows;
+  // more than that, and the join's launch of a wave per query row has no room for more than 2^26 - 4
+  // of those (2^32 threads).
+  a->by_item = tiles <= 48 || ((long long)p->B * p->Hkv >= cus && tiles <= 128) || p->B > 64 * fa::kMostLaneRows ||
+               p->B * (long long)p->Hkv * rows > (1 << 26) - 4;
   // At most four pieces per unit (two where the rows are equally long: decode_unit).
   a->pieces = 4 * cus;
   // At least 16 tiles a piece, four per wave, so that the merge stays short (8 of 500
