@@ -356,12 +356,12 @@ __global__ __launch_bounds__(64 * NW, 2) void decode_fp8_kernel(DecodeArgs a) {
       qf[n][s] = *reinterpret_cast<const u32x4*>(qp + hq * a.qsh + i * a.qst + d);
     }
     qpos[n] = have - ql + i;
-    qlo[n] = a.win_left < 0 ? 0 : max(qpos[n] - a.win_left, 0);
+    qlo[n] = a.win_left < 0 ? 0 : window_first(qpos[n], a.win_left);
     qhi[n] = a.win_right < 0 ? have - 1 : (int)min((long long)have - 1, (long long)qpos[n] + a.win_right);
     if (i >= ql) qhi[n] = -1;  // a padded query sees nothing
     slope[n] = kGeneral && a.alibi ? a.alibi[hk * a.g + hq] : 0.f;
   }
-  const int vlo = a.win_left < 0 ? 0 : max(have - ql - a.win_left, 0);  // before it no row sees a key
+  const int vlo = a.win_left < 0 ? 0 : window_first(have - ql, a.win_left);  // before it no row sees a key
 
   f32x4 acc[NQ][DV];
   float m[NQ], l[NQ];

@@ -21,11 +21,13 @@ struct DecodeSpan {
   int lo;  // first tile
   int n;   // tiles (at least one: a row without keys still writes its outputs)
 };
+// First key that a query at pos (before the first key: negative) with a window of
+// left >= 0 sees, if any; no sum here passes 32 bits.
+FA_HD int window_first(int pos, int left) { return pos > left ? pos - left : 0; }
 // `have` keys, the newest `ql` of them the queries, the window's left reach
 // (< 0: none).
 FA_HD DecodeSpan decode_span(int have, int ql, int left) {
-  const long long first = left < 0 ? 0 : (long long)have - ql - left;  // (have - ql: the first query's position)
-  const int lo = first > 0 && ql > 0 ? (int)(first / kTileKeys) : 0;
+  const int lo = left >= 0 && ql > 0 ? window_first(have - ql, left) / kTileKeys : 0;  // (have - ql: the first query's position)
   const int end = ql > 0 ? have / kTileKeys + (have % kTileKeys ? 1 : 0) : 0;
   return DecodeSpan{lo < end ? lo : 0, lo < end ? end - lo : 1};
 }

@@ -26,3 +26,24 @@ def test_as_many_rows_as_a_launch_has_threads(kw):
 def test_fewer_rows_are_cut():
     rc, need = _plan(B=1, Hq=1, Hkv=1, Sq=(1 << 26) - 4, D=32)
     assert rc == -1 and need > 0
+
+
+def _native(name, tmp_path):
+    import os
+    import shutil
+    import subprocess
+    cxx = shutil.which("g++")
+    if cxx is None:
+        pytest.skip("no C++ compiler")
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    exe = tmp_path / "check"
+    subprocess.run([cxx, "-std=c++17", "-O1", "-g", "-fsanitize=address,undefined", "-fno-sanitize-recover=all",
+                    "-I" + os.path.join(root, "pallas-flexattn_amd", "csrc"),
+                    os.path.join(root, "tests", "native", name), "-o", str(exe)], check=True)
+    out = subprocess.run([str(exe)], capture_output=True, text=True)
+    assert out.returncode == 0, out.stderr
+    return out.stdout
+
+
+def test_windows_at_the_ends_of_32_bits(tmp_path):
+    assert _native("decode_window_check.cpp", tmp_path).startswith("ok 80")
