@@ -182,14 +182,7 @@ int decode_args(const fa_params* p, const fa_fp8_cache* kv, int cus, fa::DecodeA
   const int left = p->window_left < 0 || p->window_left >= p->Skv ? -1 : p->window_left;
   long long tiles = (p->Skv + fa::kTileKeys - 1) / fa::kTileKeys;
   if (left >= 0) tiles = std::min(tiles, ((long long)left + p->Sq + fa::kTileKeys - 2) / fa::kTileKeys + 1);
-  // Query rows of an item: 16, or 32 where the group has more and the call is long
-  // (from 24000 tiles of such items on). 32 read the cache half as often but
-  // leave half as many waves: in us with 16 / 32, D = 128, B1 8 heads of 32 rows 4000 keys 13.1 / 14.9,
-  // B32 to 1500 keys 29.6 / 31.9, to 6000 105 / 75; 4 heads of 56 102 / 67, of 136 B8 to
-  // 4000 28.7 / 33.2, B32 to 6000 190 / 128. 64 rows need twice the registers and were
-  // slower than 32 everywhere (78, 51.6 and 164 in the last three).
-  const long long items32 = p->B * (long long)p->Hkv * ((rows + 31) / 32);
-  L->nq = rows > 16 && items32 * tiles >= 24000 ? 2 : 1;
+  L->nq = fa::decode_blocks(rows, p->B * (long long)p->Hkv, tiles);
   const long long rt = (rows + 16 * L->nq - 1) / (16 * L->nq);
   const long long items = p->B * (long long)p->Hkv * rt;
   if (items * tiles > 0x7fffffffll - (1 << 20)) return FA_ERR_SHAPE;  // tile numbers of a call are 32 bits

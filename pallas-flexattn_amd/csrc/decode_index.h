@@ -33,6 +33,17 @@ FA_HD DecodeSpan decode_span(int have, int ql, int left) {
 }
 FA_HD int clamp_len(int n, int most) { return n < 0 ? 0 : (n > most ? most : n); }
 
+// 16-row blocks of an item (`rows` query rows per kv head, `heads` kv heads in all, walks of
+// up to `tiles`): one, or two where the group has more than 16 rows and the call is long (from
+// 24000 tiles of such items on). 32 rows read the cache half as often but leave half as many
+// waves: in us with 16 / 32, D = 128, B1 8 heads of 32 rows 4000 keys 13.1 / 14.9, B32 to 1500 keys
+// 29.6 / 31.9, to 6000 105 / 75; 4 heads of 56 102 / 67, of 136 B8 to 4000 28.7 / 33.2, B32 to
+// 6000 190 / 128. 64 rows need twice the registers and were slower than 32 everywhere (78, 51.6
+// and 164 in the last three).
+FA_HD int decode_blocks(long long rows, long long heads, long long tiles) {
+  return rows > 16 && heads * ((rows + 31) / 32) * tiles >= 24000 ? 2 : 1;
+}
+
 // Tiles per chunk, at first: `total` tiles (of all items) over `pieces` workgroups, at least `least`.
 FA_HD int decode_chunk(int total, int pieces, int least) {
   const int c = total / pieces + (total % pieces ? 1 : 0);

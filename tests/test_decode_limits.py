@@ -28,7 +28,7 @@ def test_fewer_rows_are_cut():
     assert rc == -1 and need > 0
 
 
-def _native(name, tmp_path):
+def _native(name, tmp_path, *args):
     import os
     import shutil
     import subprocess
@@ -40,10 +40,27 @@ def _native(name, tmp_path):
     subprocess.run([cxx, "-std=c++17", "-O1", "-g", "-fsanitize=address,undefined", "-fno-sanitize-recover=all",
                     "-I" + os.path.join(root, "pallas-flexattn_amd", "csrc"),
                     os.path.join(root, "tests", "native", name), "-o", str(exe)], check=True)
-    out = subprocess.run([str(exe)], capture_output=True, text=True)
+    out = subprocess.run([str(exe), *map(str, args)], capture_output=True, text=True)
     assert out.returncode == 0, out.stderr
     return out.stdout
 
 
 def test_windows_at_the_ends_of_32_bits(tmp_path):
     assert _native("decode_window_check.cpp", tmp_path).startswith("ok 80")
+
+
+def test_blocks_of_the_gpu_tests_cases(tmp_path):
+    """The cases of test_gpu_decode_blocks take the blocks of rows per item that they are there for (where items are cut in
+    pieces, the workspace shows it there as well)."""
+    from tests.test_gpu_decode_blocks import CASES
+    args, want = [], []
+    for lens, Hq, Hkv, Sq, D, tiles, win, mods, nq, pieces, stream in CASES:
+        left = -1 if win is None else win[0]
+        walk = tiles if left < 0 else min(tiles, (left + Sq + 30) // 32 + 1)
+        args += [Hq // Hkv * Sq, len(lens) * Hkv, walk]
+        want.append(nq)
+        assert stream == (2 * len(lens) * Hkv * walk * 32 * D > 112 << 20)
+        assert pieces == (walk > 48 and (len(lens) * Hkv < 256 or walk > 128))
+    assert [int(x) for x in _native("decode_plan.cpp", tmp_path, *args).split()] == want
+    assert {(c[4], bool(c[7] or c[6]), c[9]) for c in CASES if c[8] == 2} == {(D, g, p) for D in (32, 64, 128) for g in (False, True)
+                                                                            for p in (False, True)}
