@@ -239,17 +239,15 @@ __device__ __forceinline__ DecodeUnit decode_piece_unit(const DecodeArgs& a, int
 #pragma unroll
     for (int j = 0; j < kRows; ++j) {
       p[j] = decode_pieces(n[j], chunk);
-      units += p[j] * each;
-      slots += p[j] > 1 ? p[j] * each : 0;
+      decode_next_row(p[j], each, &units, &slots);
     }
     iu = wave_scan(units);
     const int all = __builtin_amdgcn_readlane(iu, 63);
-    // (over hundreds of rows the rounding evens out, and a try costs a division per row)
-    if (all <= pieces || a.B * each >= pieces || i == (kRows > kLaneRows ? 0 : kChunkTries)) break;
+    if (all <= pieces || a.B * each >= pieces || i == decode_tries(kRows)) break;
     chunk = decode_next_chunk(chunk, all, pieces);
   }
   const int is = wave_scan(slots);
-  int fu = iu - units, fs = is - slots;
+  const int fu = iu - units, fs = is - slots;
   if (wg == 0 && first_wave) {  // for the merge
     int f = fu, g = fs;
 #pragma unroll
@@ -258,8 +256,7 @@ __device__ __forceinline__ DecodeUnit decode_piece_unit(const DecodeArgs& a, int
         a.head[2 * (b0 + j)] = f;
         a.head[2 * (b0 + j) + 1] = g;
       }
-      f += p[j] * each;
-      g += p[j] > 1 ? p[j] * each : 0;
+      decode_next_row(p[j], each, &f, &g);
     }
     if (lane == 63) a.head[2 * a.B] = iu;
   }
@@ -269,21 +266,12 @@ __device__ __forceinline__ DecodeUnit decode_piece_unit(const DecodeArgs& a, int
     u.b = -1;
     return u;
   }
-  int b = b0, nb = n[0], pb = p[0];
-#pragma unroll
-  for (int j = 1; j < kRows; ++j) {
-    const bool later = b == b0 + j - 1 && wg >= fu + pb * each && n[j] != 0;
-    fu += later ? pb * each : 0;
-    fs += later && pb > 1 ? pb * each : 0;
-    b = later ? b0 + j : b;
-    nb = later ? n[j] : nb;
-    pb = later ? p[j] : pb;
-  }
+  const DecodeRow row = decode_find_row<kRows>(b0, n, p, each, wg, fu, fs);
   const int src = __builtin_ctzll(mine);
-  u.b = __builtin_amdgcn_readlane(b, src);
-  pb = __builtin_amdgcn_readlane(pb, src);
-  nb = __builtin_amdgcn_readlane(nb, src);
-  const int local = wg - __builtin_amdgcn_readlane(fu, src);
+  u.b = __builtin_amdgcn_readlane(row.b, src);
+  const int pb = __builtin_amdgcn_readlane(row.p, src);
+  const int nb = __builtin_amdgcn_readlane(row.n, src);
+  const int local = wg - __builtin_amdgcn_readlane(row.unit, src);
   u.have = a.kv_lens ? clamp_len(scalar_load(a.kv_lens, u.b), a.cap) : a.cap;
   u.ql = a.q_lens ? clamp_len(scalar_load(a.q_lens, u.b), a.Sq) : a.Sq;
   u.item = local / pb;
@@ -291,7 +279,7 @@ __device__ __forceinline__ DecodeUnit decode_piece_unit(const DecodeArgs& a, int
   const int lo = decode_piece(nb, pb, piece);
   u.t0 = decode_span(u.have, u.ql, a.win_left).lo + lo;
   u.nt = decode_piece(nb, pb, piece + 1) - lo;
-  u.slot = pb > 1 ? __builtin_amdgcn_readlane(fs, src) + local : -1;
+  u.slot = pb > 1 ? __builtin_amdgcn_readlane(row.slot, src) + local : -1;
   return u;
 }
 __device__ __forceinline__ DecodeUnit decode_unit(const DecodeArgs& a, int wg, bool first_wave) {

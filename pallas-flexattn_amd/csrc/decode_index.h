@@ -53,6 +53,8 @@ FA_HD int decode_chunk(int total, int pieces, int least) {
 // than `pieces`: a few workgroups over a round number leave some compute units with one
 // more than the others (8 rows of 3277 to 32768 keys: 84.5 us without, 72.4 with it).
 constexpr int kChunkTries = 6;
+// (over hundreds of rows the rounding evens out, and a try costs a division per row)
+constexpr int decode_tries(int lane_rows) { return lane_rows > kLaneRows ? 0 : kChunkTries; }
 FA_HD int decode_next_chunk(int chunk, int units, int pieces) {
   const int more = (int)((long long)chunk * (units - pieces) / (2ll * pieces));
   return chunk + (more > 1 ? more : 1);
@@ -64,6 +66,31 @@ FA_HD int decode_pieces(int n, int chunk) { return n / chunk + (n % chunk ? 1 : 
 FA_HD int decode_piece(int n, int pieces, int p) {
   const int q = n / pieces, r = n - q * pieces;
   return q * p + r * p / pieces;
+}
+
+// Which row a unit lies in.  A lane of a wave holds kRows consecutive rows, the first of them
+// number b0: their tiles n (0: no row) and pieces p per item, `each` items per row; its first
+// row's units begin at `unit`, its partial results at `slot`.
+struct DecodeRow {
+  int b, n, p;     // the row, its tiles, its pieces
+  int unit, slot;  // where the row's units and slots begin
+};
+FA_HD void decode_next_row(int p, int each, int* unit, int* slot) {
+  *unit += p * each;
+  *slot += p > 1 ? p * each : 0;
+}
+// (the lane whose units `wg` is one of; the others' results mean nothing)
+template <int kRows>
+FA_HD DecodeRow decode_find_row(int b0, const int (&n)[kRows], const int (&p)[kRows], int each, int wg, int unit, int slot) {
+  DecodeRow r{b0, n[0], p[0], unit, slot};
+#pragma unroll
+  for (int j = 1; j < kRows; ++j) {
+    const bool later = r.b == b0 + j - 1 && wg >= r.unit + r.p * each && n[j] != 0;
+    int u = r.unit, s = r.slot;
+    decode_next_row(r.p, each, &u, &s);
+    r = later ? DecodeRow{b0 + j, n[j], p[j], u, s} : r;
+  }
+  return r;
 }
 
 // Workgroups that a call needs at most: items, plus a piece more for every

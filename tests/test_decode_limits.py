@@ -64,3 +64,7 @@ def test_blocks_of_the_gpu_tests_cases(tmp_path):
     assert [int(x) for x in _native("decode_plan.cpp", tmp_path, *args).split()] == want
     assert {(c[4], bool(c[7] or c[6]), c[9]) for c in CASES if c[8] == 2} == {(D, g, p) for D in (32, 64, 128) for g in (False, True)
                                                                             for p in (False, True)}
+
+
+def test_every_workgroup_finds_its_work(tmp_path):
+    assert _native("decode_unit_check.cpp", tmp_path).startswith("ok 1500 ")
