@@ -206,8 +206,9 @@ int decode_args(const fa_params* p, const fa_fp8_cache* kv, int cus, fa::DecodeA
   a->win_right = p->window_right < 0 || p->window_right >= p->Sq - 1 ? -1 : p->window_right;
   // A row of an item sees the item's keys or, padded, none, unless there are several queries
   // and a window: then NaN values must be kept from the rows that do not see their key, which
-  // costs registers that the plain walk has no room for (D = 128: 138 for 126, three waves per
-  // SIMD for four; 256 mixed lengths to 257 tiles 58.3 us for 54.5).
+  // costs registers that the plain walk has no room for (D = 128: with it alone 138 for 126, three waves per
+  // SIMD for four; 256 mixed lengths to 257 tiles 58.3 us for 54.5. These kernels, with the
+  // modifiers too, take 146).
   L->general = p->alibi_slopes || p->softcap > 0.f || (p->Sq > 1 && (left >= 0 || a->win_right >= 0));
   a->scale = p->scale == 0.f ? 1.0f / sqrtf((float)p->D) : p->scale;
   a->scale_log2 = a->scale * fa::kLog2e;

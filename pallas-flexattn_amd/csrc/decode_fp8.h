@@ -8,9 +8,12 @@
 // D = 128), its codes go from HBM straight into the registers that feed the
 // matrix cores, the next tile's as soon as this one's are used; no LDS and no
 // barrier inside the walk.  The g query heads of a kv head and their Sq queries
-// are one block of g Sq rows, 16 NQ of them (16 or 32) per work item: groups of
-// up to that many rows read the cache once.  B8 Hq32 Hkv8 32768 keys D128: 86 us
-// for 538 MB (6.2 TB/s), 4.7 more for the join.
+// are g Sq rows, a head's queries one after another, 16 NQ of them (16 or 32) per work
+// item: groups of up to that many rows read the cache once.  Longer chunks of
+// queries read it once per item, from the batch row's first visible key to its last
+// whatever the item's own rows see: this is a kernel for few queries (B8 Hq32 Hkv8
+// 32768 keys D128: 86 us for 538 MB, 6.2 TB/s, 4.7 more for the join; a causal prompt of
+// 2000 tokens 170 us, where the bf16 prompt kernel takes 56).
 //
 // Layouts (v_mfma_f32_16x16x32_bf16; lane l = 16 g + r):
 //   * S^T = K Q^T: A = 16 keys, lane (r, g) holds key r's bytes 64 c + 16 g + [0, 16)
@@ -26,8 +29,10 @@
 //     operand's words.  MFMA t is then rows d = DV r + t, and a lane ends
 //     with 4 DV consecutive d of its query.
 // P goes into the product as two bf16 pieces (its value and what that
-// rounding left): the matrix cores are idle most of the time anyway, and O
-// then carries only its own rounding.
+// rounding left): the matrix cores are idle most of the time anyway, and a
+// weight is then off by at most 2^-16, where O's own rounding is 2^-8 (a bf16
+// weight would be off by as much).  Maxima may be stale by kLazy, which costs no bits:
+// P and its sum scale alike.
 #pragma once
 #include "common.h"
 #include "decode_index.h"

@@ -196,8 +196,9 @@ __device__ __forceinline__ void rotary_thread(const RotaryArgs& a, unsigned id) 
       store8(y + r.a, xa);
       store8(y + r.b, xb);
     } else {
-      // any 2n, D and alignment: units [0, ceil(n / 8)) take eight pairs each,
-      // the following ones sixteen copied elements each
+      // any 2n, D and alignment: units [0, ceil(n / 8)) take eight pairs each, the following ones
+      // sixteen copied elements each, one element per access (bf16 B4 H32 + 32 T8192 D96, forward
+      // and gradient: 24 rotated elements 1566 us, 32 of them in the other form 319)
       const int pair_units = (a.n + 7) / 8;
       if (u < pair_units) {
 #pragma unroll

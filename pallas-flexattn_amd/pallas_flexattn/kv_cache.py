@@ -78,7 +78,8 @@ def append_kv_cache(cache, key, value, kv_lens, page_table=None, new_lens=None, 
     Tokens past the page table's last page, or on a page id outside the cache, are
     dropped.  The pages that one call writes must be distinct, each at one place of one row's
     table (shared prefix pages are read, never appended to).  ``page_size`` must be a multiple of 32; tokens of
-    any strides whose rows are 16-byte aligned are read in place.  No gradient."""
+    any strides whose rows are 16-byte aligned are read in place.  No gradient; the versions of the
+    cache's tensors rise, so that autograd notices a cache that it had saved."""
     fp8 = isinstance(cache, Fp8KVCache)
     if not fp8 and not (isinstance(cache, (tuple, list)) and len(cache) == 2):
         raise TypeError("cache must be an Fp8KVCache or a (key, value) pair of tensors")
@@ -103,7 +104,9 @@ def flex_decode_fp8(query, cache: Fp8KVCache, kv_lens=None, page_table=None, mas
     divided by it: a bound near the longest row is faster than a table made for far longer ones.  Made for
     short query blocks (decoding, speculative decoding, short chunks): the cache is read once for
     every 16 to 32 rows of Sq * Hq / Hkv, and each row's keys are split over as many workgroups as
-    the batch needs.
+    the batch needs.  Chunks of hundreds of queries are right but not fast: every block of rows
+    walks all keys that any query of the batch row sees (a causal prompt of 2000 tokens with 32
+    heads 170 us, where ``flex_attention`` on bf16 keys takes 56).
 
     Query i sits at position ``kv_lens[b] - Sq + i`` (bottom-right aligned, as
     ``flex_attention_varlen``); with ``query_lens`` (B,) a row has only that many queries, at
