@@ -433,6 +433,106 @@ int fa_fwd_kvcache_fp8(const fa_params *p, const fa_fp8_cache *kv, const fa_stri
  * in 64 bits.  What 32 bits do not hold becomes INT32_MIN or INT32_MAX. */
 int fa_int64_to_int32(const int64_t *x, int32_t *y, int64_t n, void *stream);
 
+/* Attention of chunks of new tokens over a paged cache (prompts, parts of prompts, the mixed
+ * batches of a scheduler).  Row b has kv_lens[b] keys (at most kv_len; null: kv_len) and its
+ * queries are the newest of them: query i of q_lens[b] (null: T) sits at position
+ * kv_lens[b] - q_lens[b] + i, which is what the window and ALiBi refer to.  query is
+ * (B, Hq, T, D) bf16; queries i >= q_lens[b] give o = 0 and lse = -inf, as do queries that see no key.
+ * Packed (q_starts set, q_lens null): query is (1, Hq, T, D), row b's queries are its tokens
+ * q_starts[b] .. q_starts[b + 1] - 1; q_starts (B + 1) begins with 0 and does not fall; tokens
+ * behind its last entry give o = 0 and lse = -inf.  out: like query, strides of its own; lse float32, dense.
+ * cache_dtype FA_DTYPE_BF16: fa_fwd_kvcache's layout; FA_DTYPE_FP8_E4M3: struct fa_fp8_cache's (powers of two as
+ * scales).  page_size is a multiple of 32, D = 32, 64 or 128, rows are 16-byte aligned.  Page ids
+ * outside the cache read as zero keys.  What no query sees may hold anything; a value that is not finite
+ * reaches the queries that see its key alone.  alibi_slopes (Hq) or null, softcap 0: none, scale 0: D^-1/2.
+ * The workspace (16-byte aligned; 0 bytes: none) holds partial results where keys are split over workgroups. */
+typedef struct fa_prefill_call {
+  int32_t abi_version, cache_dtype;
+  int32_t B, Hkv, T, D, page_size, max_pages, num_pages, kv_len;
+  int32_t window_left, window_right; /* < 0: unlimited */
+  float scale, softcap;
+  const float *alibi_slopes;
+  fa_strided query, out;
+  float *lse;
+  const void *k_cache, *v_cache;
+  const float *k_scale, *v_scale;
+  const int32_t *page_table, *kv_lens, *q_lens, *q_starts;
+} fa_prefill_call;
+size_t fa_prefill_workspace_bytes(const fa_prefill_call *c);
+int fa_prefill(const fa_prefill_call *c, void *workspace, size_t workspace_bytes, void *stream);
+
+/* A cache of latent vectors, (num_pages, page_size, latent_dim + rope_dim) bf16: of each token latent_dim elements
+ * that are key and value of every head, and rope_dim elements that are key only.  latent_dim
+ * 128, 256 or 512, rope_dim 32 or 64, page_size a multiple of 32.
+ *
+ * fa_latent_append: token t < new_lens[b] (null: T) of latent (B, 1, T, latent_dim) and rope (B, 1, T, rope_dim) goes
+ * to position kv_lens[b] + t, as fa_kv_append's tokens do; the rotary part is rotated to that position
+ * (rotary.pairs 0: not), and so is query (B, heads, T, rope_dim) into query_out (heads 0: none). */
+typedef struct fa_latent_append_call {
+  int32_t abi_version, B, T, latent_dim, rope_dim, page_size, max_pages, num_pages;
+  fa_strided latent, rope, query;
+  void *query_out, *cache;
+  const int32_t *page_table, *kv_lens, *new_lens;
+  fa_rotary rotary;
+} fa_latent_append_call;
+int fa_latent_append(const fa_latent_append_call *c, void *stream);
+
+/* Attention of each row's newest queries over that cache (absorbed form): query (B, heads, T, latent_dim) and
+ * query_rope (B, heads, T, rope_dim) score a token by scale (q . latent + q_rope . rope); o (B, heads, T, latent_dim)
+ * bf16 and lse float32, dense, are the weighted latent vectors.  Lengths, positions, windows, padded queries, page ids
+ * and workspace as in fa_fwd_kvcache_fp8; scale is positive. */
+typedef struct fa_latent_call {
+  int32_t abi_version, B, T, latent_dim, rope_dim, page_size, max_pages, num_pages, kv_len;
+  int32_t window_left, window_right;
+  float scale;
+  fa_strided query, query_rope;
+  void *o;
+  float *lse;
+  const void *cache;
+  const int32_t *page_table, *kv_lens, *q_lens;
+} fa_latent_call;
+size_t fa_latent_decode_workspace_bytes(const fa_latent_call *c);
+int fa_latent_decode(const fa_latent_call *c, void *workspace, size_t workspace_bytes, void *stream);
+
+/* One tensor of a paged cache: num_pages pages of page_bytes each (a multiple of 4), one behind another, 4-byte
+ * aligned (16-byte accesses where both allow). */
+typedef struct fa_paged_tensor {
+  void *data;
+  int64_t page_bytes;
+} fa_paged_tensor;
+
+/* Page src[i] is copied to page dst[i], i < pairs, in each of count tensors.  Pairs with an id outside
+ * [0, num_pages), or twice the same, are left out.  The pages dst are distinct, and none of them is among src. */
+int fa_copy_pages(const fa_paged_tensor *t, int32_t count, int32_t num_pages, const int32_t *src, const int32_t *dst,
+                  int32_t pairs, void *stream);
+
+/* Rows that go on from other rows.  Row b of N takes the tokens of row parents[b] of B (null: N = B, its own;
+ * outside [0, B): none), kv_lens of them (at most the table's).  Pages that they fill are shared.  A page that they fill in part becomes
+ * the row's own: the first row that ends in it keeps it unless another row has the whole of it or keep[page] is set;
+ * the others get a copy.  Then come pages for room[b] (null: room_all) further tokens, at most to the
+ * table's end, and -1.  Copies and room take pages that no entry of the result names and keep does not
+ * hold, in ascending order, row by row (the copy first).  out_free: how many of those are left; below
+ * zero, so many were lacking, and the entries that lack one are -1.  Ids outside the cache are taken over as they are.
+ * The outputs must not overlap the inputs. */
+typedef struct fa_page_plan_call {
+  int32_t abi_version, B, N, max_pages, page_size, num_pages, room_all;
+  const int32_t *page_table, *kv_lens; /* (B, max_pages), (B) */
+  const int32_t *parents, *room;       /* (N) or NULL */
+  const uint8_t *keep;                 /* (num_pages), 0 or not, or NULL */
+  int32_t *out_table, *out_lens;       /* (N, max_pages), (N; not written by fa_compact_pages) */
+  int32_t *out_count;                  /* one number */
+  const fa_paged_tensor *tensors;      /* host memory */
+  int32_t tensor_count;
+} fa_page_plan_call;
+size_t fa_fork_rows_workspace_bytes(const fa_page_plan_call *c);
+int fa_fork_rows(const fa_page_plan_call *c, void *workspace, size_t workspace_bytes, void *stream);
+
+/* The pages in use move to the front: with n of them (named by a row within its tokens and room_all, or kept), those
+ * past the n-th id that are not kept move, in ascending order, to the free ids before it.  N = B, parents and room null.
+ * out_table: the rows' new ids, -1 past their tokens and room; out_count: n. */
+size_t fa_compact_pages_workspace_bytes(const fa_page_plan_call *c);
+int fa_compact_pages(const fa_page_plan_call *c, void *workspace, size_t workspace_bytes, void *stream);
+
 /*
  * Block-mask construction on the device (create_block_mask, block_mask.py:54-129)
  * for the mask semantics of fa_params: the window (window_left, window_right)

@@ -16,10 +16,13 @@ CSRC = os.path.join(HERE, "csrc")
 # direction, so the objects build in parallel.
 UNITS = [(os.path.join(CSRC, "capi.hip"), [], "capi"), (os.path.join(CSRC, "kernels_fp8.hip"), [], "kernels_fp8"),
          (os.path.join(CSRC, "kernels_cache.hip"), [], "kernels_cache"),
+         (os.path.join(CSRC, "kernels_pages.hip"), [], "kernels_pages"),
          (os.path.join(CSRC, "host.cpp"), [], "host")] + [
     (os.path.join(CSRC, "kernels.hip"), [f"-DFA_KERNELS_D={d}", f"-DFA_KERNELS_BWD={bwd}"],
      f"kernels_d{d}_{'bwd' if bwd else 'fwd'}")
-    for d in (128, 64, 32) for bwd in (1, 0)]
+    for d in (128, 64, 32) for bwd in (1, 0)] + [
+    (os.path.join(CSRC, "kernels_prefill.hip"), [f"-DFA_KERNELS_D={d}"], f"kernels_prefill_d{d}") for d in (128, 64, 32)] + [
+    (os.path.join(CSRC, "kernels_latent.hip"), [f"-DFA_KERNELS_L={n}"], f"kernels_latent_l{n}") for n in (512, 256, 128)]
 SOURCES = sorted({u[0] for u in UNITS})
 # CPython extension over torch tensors (host code, links against torch)
 LAUNCH_SRC = os.path.join(CSRC, "torch_launch.cpp")

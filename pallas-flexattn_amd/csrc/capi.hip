@@ -13,7 +13,9 @@
 #include <vector>
 
 #include "../../include/flexattn.h"
+#include "latent_args.h"
 #include "launch.h"
+#include "prefill_plan.h"
 #include "problem.h"
 #include "mask_build.h"
 
@@ -283,6 +285,7 @@ int fwd_fp8_launch(const fa_params* p, const fa_fp8_inputs* in, bool q16, void* 
 
 #include "user_mods.h"
 #include "cache_calls.h"
+#include "serve_calls.h"
 
 }  // namespace
 
@@ -698,6 +701,87 @@ int fa_fwd_kvcache_fp8(const fa_params* p, const fa_fp8_cache* kv, const fa_stri
     a.part_ml = reinterpret_cast<float*>(ws + L.ml);
   }
   return fa::launch_decode_fp8(a, p->D, L.nq, L.general, L.stream, static_cast<hipStream_t>(stream));
+}
+
+size_t fa_prefill_workspace_bytes(const fa_prefill_call* c) {
+  fa::PrefillArgs a;
+  PrefillLayout L;
+  return prefill_args(c, device_cus(), &a, &L) == FA_OK ? L.bytes : 0;
+}
+
+int fa_prefill(const fa_prefill_call* c, void* workspace, size_t workspace_bytes, void* stream) {
+  fa::PrefillArgs a;
+  PrefillLayout L;
+  const int rc = prefill_args(c, device_cus(), &a, &L);
+  if (rc) return rc;
+  if (L.bytes && (!workspace || workspace_bytes < L.bytes || !aligned16({workspace}))) return FA_ERR_WORKSPACE;
+  a.part = static_cast<float*>(workspace);
+  const bool fp8 = c->cache_dtype == FA_DTYPE_FP8_E4M3, mods = c->alibi_slopes || c->softcap > 0.f;
+  const hipStream_t s = static_cast<hipStream_t>(stream);
+  switch (c->D) {
+    case 32: return fa::launch_prefill<32>(a, fp8, mods, s);
+    case 64: return fa::launch_prefill<64>(a, fp8, mods, s);
+    default: return fa::launch_prefill<128>(a, fp8, mods, s);
+  }
+}
+
+int fa_latent_append(const fa_latent_append_call* c, void* stream) {
+  fa::LatentAppendArgs a;
+  const int rc = latent_append_args(c, &a);
+  return rc ? rc : fa::launch_latent_append(a, static_cast<hipStream_t>(stream));
+}
+
+size_t fa_latent_decode_workspace_bytes(const fa_latent_call* c) {
+  fa::LatentArgs a;
+  LatentLayout L;
+  return latent_args(c, device_cus(), &a, &L) == FA_OK ? L.bytes : 0;
+}
+
+int fa_latent_decode(const fa_latent_call* c, void* workspace, size_t workspace_bytes, void* stream) {
+  fa::LatentArgs a;
+  LatentLayout L;
+  const int rc = latent_args(c, device_cus(), &a, &L);
+  if (rc) return rc;
+  if (L.bytes && (!workspace || workspace_bytes < L.bytes || !aligned16({workspace}))) return FA_ERR_WORKSPACE;
+  if (L.bytes) {
+    char* ws = static_cast<char*>(workspace);
+    a.d.head = reinterpret_cast<int*>(ws);
+    a.d.part = reinterpret_cast<float*>(ws + L.part);
+    a.d.part_ml = reinterpret_cast<float*>(ws + L.ml);
+  }
+  const hipStream_t s = static_cast<hipStream_t>(stream);
+  switch (c->latent_dim) {
+    case 128: return fa::launch_latent<128>(a, c->rope_dim, L.nb, s);
+    case 256: return fa::launch_latent<256>(a, c->rope_dim, L.nb, s);
+    default: return fa::launch_latent<512>(a, c->rope_dim, L.nb, s);
+  }
+}
+
+int fa_copy_pages(const fa_paged_tensor* t, int32_t count, int32_t num_pages, const int32_t* src, const int32_t* dst,
+                  int32_t pairs, void* stream) {
+  if (num_pages < 1 || pairs < 0) return FA_ERR_SHAPE;
+  if (const int rc = tensors_ok(t, count)) return rc;
+  if (pairs == 0) return FA_OK;
+  if (!src || !dst) return FA_ERR_NULL;
+  return copy_tensors(t, count, num_pages, src, dst, nullptr, pairs, static_cast<hipStream_t>(stream));
+}
+
+size_t fa_fork_rows_workspace_bytes(const fa_page_plan_call* c) {
+  fa::PagePlan a;
+  PlanLayout L;
+  return plan_args(c, true, &a, &L) == FA_OK ? L.bytes : 0;
+}
+int fa_fork_rows(const fa_page_plan_call* c, void* workspace, size_t workspace_bytes, void* stream) {
+  return run_plan(c, true, workspace, workspace_bytes, stream);
+}
+
+size_t fa_compact_pages_workspace_bytes(const fa_page_plan_call* c) {
+  fa::PagePlan a;
+  PlanLayout L;
+  return plan_args(c, false, &a, &L) == FA_OK ? L.bytes : 0;
+}
+int fa_compact_pages(const fa_page_plan_call* c, void* workspace, size_t workspace_bytes, void* stream) {
+  return run_plan(c, false, workspace, workspace_bytes, stream);
 }
 
 size_t fa_mask_build_workspace_bytes(const fa_mask_build* m) {

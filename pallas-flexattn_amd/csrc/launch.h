@@ -11,6 +11,7 @@
 #include "fwd.h"
 #include "fwd_fp8.h"
 #include "kv_append.h"
+#include "page_plan.h"
 #include "problem.h"
 
 namespace fa {
@@ -41,6 +42,22 @@ int launch_quant_fp8(const QuantArgs& a, hipStream_t s);
 int launch_rotary(const RotaryArgs& a, bool f32, bool vec, hipStream_t s);
 int launch_append(const AppendArgs& a, int D, bool fp8, hipStream_t s);
 int launch_decode_fp8(const DecodeArgs& a, int D, int nq, bool general, bool stream, hipStream_t s);
+struct CopyArgs;
+struct LatentAppendArgs;
+struct LatentArgs;
+struct PrefillArgs;
+
+// Chunks of new tokens over a paged cache (kernels_prefill.hip: D = 32, 64 or 128; mods: ALiBi or a soft-cap), rows
+// over a cache of latent vectors (kernels_latent.hip: L = 128, 256 or 512, R = 32 or 64; nb: 16-row blocks per
+// work item, 1, 2 or 4), appends to it, and pages (kernels_pages.hip; marks null: in LDS, at most kPlanLds of them)
+template <int D>
+int launch_prefill(const PrefillArgs& a, bool fp8, bool mods, hipStream_t s);
+template <int L>
+int launch_latent(const LatentArgs& a, int R, int nb, hipStream_t s);
+int launch_latent_append(const LatentAppendArgs& a, hipStream_t s);
+constexpr int kCopyGrid = 2048, kPlanLds = 15 * 1024;
+int launch_copy_pages(const CopyArgs& a, hipStream_t s);
+int launch_page_plan(const PagePlan& a, bool fork, hipStream_t s);
 int launch_saturate(const int64_t* x, int32_t* y, long long n, hipStream_t s);
 
 }  // namespace fa

@@ -1,0 +1,91 @@
+// Work partition of attention of chunks of new tokens over a paged cache (prefill.h), plain C++ for the
+// device and for the host.
+//
+// The g query heads of a kv head share its keys: a batch row's q queries are g q rows (row r: query r / g, head
+// r % g of the group), kPrefillRows of them a work item, so an item's rows are neighbours in
+// time and see nearly the same keys, and a short chunk still fills an item.
+#pragma once
+#include "decode_index.h"
+
+namespace fa {
+
+struct PrefillArgs {
+  const void* q;            // bf16; element strides of (row, head, token)
+  long long qsb, qsh, qst;
+  void* o;
+  long long osb, osh, ost;
+  float* lse;               // (B, Hq, Sq), packed (Hq, Sq)
+  const char *k, *v;        // (num_pages, Hkv, page_size, D)
+  const float *ks, *vs;     // e4m3: (num_pages, Hkv, page_size / 32)
+  const int *page_table, *kv_lens, *q_lens;
+  const int* starts;        // packed: (B + 1), Sq tokens in all
+  int B, Hq, Hkv, Sq, g;
+  int page_runs, max_pages, num_pages, cap;
+  int win_left, win_right;
+  float scale, scale_log2, softcap;
+  const float* alibi;
+  int tiles;                // row tiles (of each kv head)
+  int n_splits;
+  float* part;              // n_splits > 1: (n_splits, rows, D), then (m, l) (n_splits, rows, 2); rows as lse's
+};
+
+constexpr int kPrefillRows = 128;  // rows of a work item
+constexpr int kPrefillKeys = 64;   // keys of a tile
+
+// Tokens [s, e) of packed rows: b in [0, B) a batch row; B and B + 1 the tokens behind the last and before the first, which
+// belong to none.
+struct TokenSpan {
+  int s, e;
+};
+FA_HD TokenSpan packed_span(const int* starts, int b, int B, int total) {
+  TokenSpan t;
+  t.s = b <= B ? clamp_len(starts[b], total) : 0;
+  t.e = b < B ? clamp_len(starts[b + 1], total) : b == B ? total : clamp_len(starts[0], total);
+  if (t.e < t.s) t.e = t.s;
+  return t;
+}
+FA_HD int row_tiles(int queries, int g) {  // (queries * g < 2^31: the host's check)
+  const int rows = queries * g;
+  return rows / kPrefillRows + (rows % kPrefillRows != 0);
+}
+// Row tiles of a call at most: packed rows end in a partly filled tile each.
+FA_HD long long prefill_tiles(bool packed, int B, int tokens, int g) {
+  const long long rows = (long long)tokens * g;
+  if (packed) return rows / kPrefillRows + B + 2;
+  return B * ((rows + kPrefillRows - 1) / kPrefillRows);
+}
+
+// Keys that the query at position pos sees of a row with `have` keys: [lo, hi] (hi < lo: none).
+struct KeySpan {
+  int lo, hi;
+};
+FA_HD KeySpan key_span(int pos, int have, int left, int right) {
+  KeySpan k;
+  k.lo = left < 0 ? 0 : window_first(pos, left);
+  const long long end = right < 0 ? have - 1 : (long long)pos + right;
+  k.hi = end < have - 1 ? (int)(end < -1 ? -1 : end) : have - 1;
+  return k;
+}
+// Tiles [t0, t1) of kPrefillKeys that queries i0 .. i1 (of ql, standing at have - ql + i) see.
+struct TileSpan {
+  int t0, t1;
+};
+FA_HD TileSpan tile_span(int have, int ql, int i0, int i1, int left, int right) {
+  const KeySpan a = key_span(have - ql + i0, have, left, right), b = key_span(have - ql + i1, have, left, right);
+  if (b.hi < a.lo || i1 < i0) return TileSpan{0, 0};
+  return TileSpan{a.lo / kPrefillKeys, b.hi / kPrefillKeys + 1};
+}
+
+// Ranges of keys that an item is cut into: workgroups for about `want` where there are fewer items, each at least
+// kPrefillLeast tiles of the longest row, at most kPrefillSplits.
+constexpr int kPrefillSplits = 32, kPrefillLeast = 4;
+FA_HD int prefill_splits(long long items, int most_tiles, int want) {
+  if (items >= want) return 1;
+  long long n = want / items;
+  const int most = most_tiles / kPrefillLeast;
+  if (n > most) n = most;
+  if (n > kPrefillSplits) n = kPrefillSplits;
+  return n < 1 ? 1 : (int)n;
+}
+
+}  // namespace fa

@@ -4,7 +4,7 @@
 // conversions for every pointer.  Host code only; the C ABI's entry points are
 // handed over by address (bind), so it links against torch alone.
 //
-// The calls around a KV cache (rotary, append, decode over e4m3 pages) are checked here
+// The calls around a KV cache (rotary, append, decode over e4m3 pages, prompts, latent vectors, pages) are checked here
 // too: their struct arguments are filled from the tensors' own shapes and strides,
 // and they run on the current stream of their tensors' device.
 //
@@ -22,6 +22,7 @@
 #include <algorithm>
 #include <cfloat>
 #include <cstdint>
+#include <vector>
 
 #include "../../include/flexattn.h"
 
@@ -584,6 +585,438 @@ PyObject* py_decode(PyObject*, PyObject* const* a, Py_ssize_t n) {
   END_HANDLE_TH_ERRORS
 }
 
+// ---------------------------------------- prompts, latent vectors and pages ----
+decltype(&fa_prefill) g_prefill = nullptr;
+decltype(&fa_prefill_workspace_bytes) g_prefill_ws = nullptr;
+decltype(&fa_latent_append) g_latent_append = nullptr;
+decltype(&fa_latent_decode) g_latent = nullptr;
+decltype(&fa_latent_decode_workspace_bytes) g_latent_ws = nullptr;
+decltype(&fa_copy_pages) g_copy_pages = nullptr;
+decltype(&fa_fork_rows) g_fork = nullptr;
+decltype(&fa_fork_rows_workspace_bytes) g_fork_ws = nullptr;
+decltype(&fa_compact_pages) g_compact = nullptr;
+decltype(&fa_compact_pages_workspace_bytes) g_compact_ws = nullptr;
+
+// bind_serve(fa_prefill, fa_prefill_workspace_bytes, fa_latent_append, fa_latent_decode,
+//            fa_latent_decode_workspace_bytes, fa_copy_pages, fa_fork_rows, fa_fork_rows_workspace_bytes,
+//            fa_compact_pages, fa_compact_pages_workspace_bytes)
+PyObject* py_bind_serve(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  if (n != 10) {
+    PyErr_SetString(PyExc_TypeError, "bind_serve takes 10 addresses");
+    return nullptr;
+  }
+  g_prefill = reinterpret_cast<decltype(g_prefill)>(address(a[0]));
+  g_prefill_ws = reinterpret_cast<decltype(g_prefill_ws)>(address(a[1]));
+  g_latent_append = reinterpret_cast<decltype(g_latent_append)>(address(a[2]));
+  g_latent = reinterpret_cast<decltype(g_latent)>(address(a[3]));
+  g_latent_ws = reinterpret_cast<decltype(g_latent_ws)>(address(a[4]));
+  g_copy_pages = reinterpret_cast<decltype(g_copy_pages)>(address(a[5]));
+  g_fork = reinterpret_cast<decltype(g_fork)>(address(a[6]));
+  g_fork_ws = reinterpret_cast<decltype(g_fork_ws)>(address(a[7]));
+  g_compact = reinterpret_cast<decltype(g_compact)>(address(a[8]));
+  g_compact_ws = reinterpret_cast<decltype(g_compact_ws)>(address(a[9]));
+  if (PyErr_Occurred()) return nullptr;
+  Py_RETURN_NONE;
+}
+
+// written through raw pointers: autograd learns of it here (inference tensors have no version)
+void written(const at::Tensor& t) {
+  if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
+}
+int64_t window(PyObject* x) { return std::max<int64_t>(std::min<int64_t>(PyLong_AsLong(x), kMaxSize), -1); }
+
+// prefill(q, k, v, k scale | None, v scale | None, kv_lens | None, table | None, q_lens | None, q_starts | None, left, right,
+//         slopes | None, softcap, scale, gqa, kv_len | None) -> (status, o, lse)
+PyObject* py_prefill(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  if (n != 16 || !g_prefill) REFUSE(PyExc_TypeError, "prefill takes 16 arguments, after bind_serve");
+  const at::Tensor *q = tensor(a[0]), *k, *v, *ks, *vs, *lens, *table, *ql, *starts, *slopes;
+  if (!q || !(k = tensor(a[1])) || !(v = tensor(a[2])) || !optional(a[3], &ks) || !optional(a[4], &vs) ||
+      !optional(a[5], &lens) || !optional(a[6], &table) || !optional(a[7], &ql) || !optional(a[8], &starts) ||
+      !optional(a[11], &slopes))
+    return nullptr;
+  const int64_t left = window(a[9]), right = window(a[10]);
+  const double softcap = PyFloat_AsDouble(a[12]), scale = PyFloat_AsDouble(a[13]);
+  const int gqa = PyObject_IsTrue(a[14]);
+  const int64_t kv_len = a[15] == Py_None ? 0 : PyLong_AsLong(a[15]);
+  if (PyErr_Occurred()) return nullptr;
+  if (!ks != !vs) REFUSE(PyExc_TypeError, "an 8-bit cache has key and value scales");
+  if (q->dim() != 4) REFUSE(PyExc_ValueError, "query must be (B, Hq, T, D), packed (1, Hq, tokens, D)");
+  if (q->scalar_type() != at::kBFloat16) REFUSE(PyExc_TypeError, "flex_prefill takes bfloat16 queries");
+  if (starts) {
+    if (ql) REFUSE(PyExc_ValueError, "pass query_lens or query_starts, not both");
+    if (starts->scalar_type() != at::kInt && starts->scalar_type() != at::kLong)
+      REFUSE(PyExc_TypeError, "query_starts must be int32 or int64");
+    if (q->size(0) != 1 || starts->dim() != 1 || starts->size(0) < 2 || starts->size(0) > kMaxSize)
+      REFUSE(PyExc_ValueError, "packed queries are (1, Hq, tokens, D), with query_starts (B + 1,) of at least one row");
+  }
+  const int64_t B = starts ? starts->size(0) - 1 : q->size(0), Hq = q->size(1), T = q->size(2), D = q->size(3);
+  if (!cache_ok(*k, *v, ks, vs, table, B, D)) return nullptr;
+  const int64_t Hkv = k->size(1);
+  if (Hq != Hkv && !gqa) REFUSE(PyExc_ValueError, "query and cache head counts differ: pass enable_gqa=True for grouped-query attention");
+  if (Hq % Hkv) REFUSE(PyExc_ValueError, "number of q heads must be a multiple of the number of kv heads");
+  if (!lens_ok(lens, B, "kv_lens must have one entry per batch row") ||
+      !lens_ok(ql, B, "query_lens must have one entry per batch row"))
+    return nullptr;
+  if (slopes && (slopes->scalar_type() != at::kFloat || slopes->dim() != 1 || slopes->size(0) != Hq || !slopes->is_contiguous()))
+    REFUSE(PyExc_ValueError, "ALiBi needs one slope per q head");
+  if (!(scale >= 0.0) || !(softcap >= 0.0)) REFUSE(PyExc_ValueError, "scale must be positive");
+  auto fits = [](double x) { return x == 0.0 || (x >= FLT_MIN && x <= FLT_MAX); };  // (0: the default, none)
+  if (!fits(scale) || !fits(softcap)) REFUSE(PyExc_ValueError, "scale and soft-cap must be normal float32 numbers");
+  const int64_t pages = table ? table->size(1) : 1, all = pages * k->size(2);
+  if (a[15] != Py_None && (kv_len < 1 || kv_len > all)) REFUSE(PyExc_ValueError, "kv_len must be in [1, max_pages * page_size]");
+  const int64_t cap = kv_len ? kv_len : all;
+  if (!sizes_fit(*q) || pages > kMaxSize || cap > kMaxSize) REFUSE(PyExc_ValueError, "sizes must be below 2^31");
+  const at::Device dev = q->device();
+  if (!dev.is_cuda()) REFUSE(PyExc_ValueError, "query and cache must be on the GPU");
+  if (k->device() != dev || v->device() != dev || (ks && (ks->device() != dev || vs->device() != dev)) ||
+      (slopes && slopes->device() != dev))
+    REFUSE(PyExc_ValueError, "query and cache must be on one device");
+  const c10::DeviceGuard guard(dev);
+  const at::Tensor qq = rows_ok(*q) ? *q : dense16(*q);
+  // laid out as the query is: what a projection wrote as (tokens, heads, D) comes back so for the next one
+  at::Tensor o = qq.is_non_overlapping_and_dense() ? at::empty_strided(qq.sizes(), qq.strides(), qq.options())
+                                                   : at::empty(qq.sizes(), qq.options());
+  at::Tensor lse = at::empty(qq.sizes().slice(0, 3), qq.options().dtype(at::kFloat));
+  int rc = FA_OK;
+  if (qq.numel()) {
+    at::Tensor ll, tt, qn, ss;
+    fa_prefill_call c{};
+    c.abi_version = FA_ABI_VERSION;
+    c.cache_dtype = ks ? FA_DTYPE_FP8_E4M3 : FA_DTYPE_BF16;
+    c.B = static_cast<int32_t>(B);
+    c.Hkv = static_cast<int32_t>(Hkv);
+    c.T = static_cast<int32_t>(T);
+    c.D = static_cast<int32_t>(D);
+    c.page_size = static_cast<int32_t>(k->size(2));
+    c.num_pages = static_cast<int32_t>(k->size(0));
+    c.max_pages = static_cast<int32_t>(pages);
+    c.kv_len = static_cast<int32_t>(cap);
+    c.window_left = static_cast<int32_t>(left);
+    c.window_right = static_cast<int32_t>(right);
+    c.scale = static_cast<float>(scale);
+    c.softcap = static_cast<float>(softcap);
+    c.alibi_slopes = slopes ? slopes->const_data_ptr<float>() : nullptr;
+    c.query = strided(qq);
+    c.out = strided(o);
+    c.out.data = o.mutable_data_ptr();
+    c.lse = lse.mutable_data_ptr<float>();
+    c.k_cache = k->const_data_ptr();
+    c.v_cache = v->const_data_ptr();
+    if (ks) {
+      c.k_scale = ks->const_data_ptr<float>();
+      c.v_scale = vs->const_data_ptr<float>();
+    }
+    if (table) c.page_table = (tt = row_ints(*table, dev)).const_data_ptr<int32_t>();
+    if (lens) c.kv_lens = (ll = row_ints(*lens, dev)).const_data_ptr<int32_t>();
+    if (ql) c.q_lens = (qn = row_ints(*ql, dev)).const_data_ptr<int32_t>();
+    if (starts) c.q_starts = (ss = row_ints(*starts, dev)).const_data_ptr<int32_t>();
+    const size_t bytes = g_prefill_ws(&c);
+    at::Tensor ws;
+    if (bytes) ws = at::empty({static_cast<int64_t>(bytes)}, qq.options().dtype(at::kByte));
+    rc = g_prefill(&c, bytes ? ws.mutable_data_ptr() : nullptr, bytes, stream_of(dev));
+  }
+  return Py_BuildValue("iNN", rc, THPVariable_Wrap(o), THPVariable_Wrap(lse));
+  END_HANDLE_TH_ERRORS
+}
+
+// A cache of latent vectors and the table of its rows.
+bool latent_ok(const at::Tensor& c, int64_t L, const at::Tensor* table, int64_t B) {
+  PyObject* value = PyExc_ValueError;
+  const char* bad = nullptr;
+  const int64_t R = c.dim() == 3 ? c.size(2) - L : 0;
+  if (c.scalar_type() != at::kBFloat16) {
+    value = PyExc_TypeError;
+    bad = "the cache must be bfloat16";
+  } else if (c.dim() != 3 || c.size(0) < 1 || c.size(1) < FA_KV_RUN || c.size(1) % FA_KV_RUN) {
+    bad = "the cache must be (num_pages, page_size, latent_dim + rope_dim), page_size a multiple of 32";
+  } else if ((L != 128 && L != 256 && L != 512) || (R != 32 && R != 64)) {
+    bad = "latent_dim must be 128, 256 or 512, rope_dim 32 or 64";
+  } else if (!c.is_contiguous()) {
+    bad = "the cache must be contiguous";
+  } else if (!sizes_fit(c)) {
+    bad = "the cache's sizes must be below 2^31";
+  } else if (!table) {
+    if (c.size(0) < B) bad = "without a page_table the cache has a page for every batch row";
+  } else if (table->dim() != 2 || table->size(0) != B || table->size(1) < 1) {
+    bad = "page_table must be (B, max_pages)";
+  } else if (table->scalar_type() != at::kInt && table->scalar_type() != at::kLong) {
+    value = PyExc_TypeError;
+    bad = "page_table must be int32 or int64";
+  }
+  if (bad) PyErr_SetString(value, bad);
+  return !bad;
+}
+
+// latent_append(cache, latent_dim, latent, key rope, kv_lens, table | None, new_lens | None, inv_freq | None, interleaved,
+//               scale, query rope | None) -> (status, query rope' | None)
+PyObject* py_latent_append(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  if (n != 11 || !g_latent_append) REFUSE(PyExc_TypeError, "latent_append takes 11 arguments, after bind_serve");
+  const at::Tensor *kc = tensor(a[0]), *x, *k, *lens, *table, *fresh, *f, *q;
+  const int64_t L = PyLong_AsLong(a[1]);
+  if (!kc || !(x = tensor(a[2])) || !(k = tensor(a[3])) || !(lens = tensor(a[4])) || !optional(a[5], &table) ||
+      !optional(a[6], &fresh) || !optional(a[7], &f) || !optional(a[10], &q))
+    return nullptr;
+  const int interleaved = PyObject_IsTrue(a[8]);
+  const double scale = PyFloat_AsDouble(a[9]);
+  if (PyErr_Occurred()) return nullptr;
+  if (x->dim() != 3 || k->dim() != 3 || (q && q->dim() != 4))
+    REFUSE(PyExc_ValueError, "latent and key_rope must be (B, T, dim), query_rope (B, H, T, rope_dim)");
+  if (x->scalar_type() != at::kBFloat16 || k->scalar_type() != at::kBFloat16 || (q && q->scalar_type() != at::kBFloat16))
+    REFUSE(PyExc_TypeError, "append_latent_cache takes bfloat16 latent, key_rope and query_rope");
+  const int64_t B = x->size(0), T = x->size(1);
+  if (!latent_ok(*kc, L, table, B)) return nullptr;
+  const int64_t R = kc->size(2) - L;
+  if (x->size(2) != L || k->size(0) != B || k->size(1) != T || k->size(2) != R ||
+      (q && (q->size(0) != B || q->size(2) != T || q->size(3) != R)))
+    REFUSE(PyExc_ValueError, "batch, length and dims of latent, key_rope, query_rope and cache must match");
+  if (q && !f) REFUSE(PyExc_ValueError, "query_rope is rotated with the keys: it needs rotary");
+  if (!lens_ok(lens, B, "kv_lens must have one entry per batch row") ||
+      !lens_ok(fresh, B, "new_lens must have one entry per batch row"))
+    return nullptr;
+  if (f && !freq_ok(*f, R)) REFUSE(PyExc_ValueError, "inv_freq must be a dense float64 vector with at most rope_dim / 2 entries");
+  if (f && f->size(0) % 8) REFUSE(PyExc_ValueError, "append_latent_cache takes a rotary_dim that is a multiple of 16");
+  if (!sizes_fit(*x) || (q && !sizes_fit(*q))) REFUSE(PyExc_ValueError, "sizes must be below 2^31");
+  const at::Device dev = kc->device();
+  if (!dev.is_cuda()) REFUSE(PyExc_ValueError, "the cache must be on the GPU");
+  if (x->device() != dev || k->device() != dev || (q && q->device() != dev) || (f && f->device() != dev))
+    REFUSE(PyExc_ValueError, "cache, tokens and inv_freq must be on one device");
+  const c10::DeviceGuard guard(dev);
+  at::Tensor out;
+  if (q) out = at::empty(q->sizes(), q->options());
+  int rc = FA_OK;
+  if (x->numel()) {
+    auto rows = [](const at::Tensor& t) {
+      const at::Tensor u = t.unsqueeze(1);
+      return rows_ok(u) ? u : dense16(u);
+    };
+    const at::Tensor xx = rows(*x), kk = rows(*k), ll = row_ints(*lens, dev);
+    at::Tensor tt, nn, qq;
+    fa_latent_append_call c{};
+    c.abi_version = FA_ABI_VERSION;
+    c.B = static_cast<int32_t>(B);
+    c.T = static_cast<int32_t>(T);
+    c.latent_dim = static_cast<int32_t>(L);
+    c.rope_dim = static_cast<int32_t>(R);
+    c.num_pages = static_cast<int32_t>(kc->size(0));
+    c.page_size = static_cast<int32_t>(kc->size(1));
+    c.max_pages = 1;
+    c.latent = strided(xx);
+    c.rope = strided(kk);
+    if (q && q->numel()) {
+      qq = rows_ok(*q) ? *q : dense16(*q);
+      c.query = strided(qq);
+      c.query_out = out.mutable_data_ptr();
+    }
+    c.cache = kc->mutable_data_ptr();
+    if (table) {
+      tt = row_ints(*table, dev);
+      c.page_table = tt.const_data_ptr<int32_t>();
+      c.max_pages = static_cast<int32_t>(tt.size(1));
+    }
+    c.kv_lens = ll.const_data_ptr<int32_t>();
+    if (fresh) c.new_lens = (nn = row_ints(*fresh, dev)).const_data_ptr<int32_t>();
+    if (f) {
+      c.rotary.inv_freq = f->const_data_ptr<double>();
+      c.rotary.pairs = static_cast<int32_t>(f->size(0));
+      c.rotary.interleaved = interleaved;
+      c.rotary.scale = static_cast<float>(scale);
+    }
+    rc = g_latent_append(&c, stream_of(dev));
+    if (rc == FA_OK) written(*kc);
+  }
+  if (!q) return Py_BuildValue("iO", rc, Py_None);
+  return Py_BuildValue("iN", rc, THPVariable_Wrap(out));
+  END_HANDLE_TH_ERRORS
+}
+
+// latent_decode(query, query rope, cache, latent_dim, scale, kv_lens | None, table | None, q_lens | None, left, right,
+//               kv_len | None) -> (status, o, lse)
+PyObject* py_latent_decode(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  if (n != 11 || !g_latent) REFUSE(PyExc_TypeError, "latent_decode takes 11 arguments, after bind_serve");
+  const at::Tensor *q = tensor(a[0]), *qr, *kc, *lens, *table, *ql;
+  if (!q || !(qr = tensor(a[1])) || !(kc = tensor(a[2])) || !optional(a[5], &lens) || !optional(a[6], &table) ||
+      !optional(a[7], &ql))
+    return nullptr;
+  const int64_t L = PyLong_AsLong(a[3]);
+  const double scale = PyFloat_AsDouble(a[4]);
+  const int64_t left = window(a[8]), right = window(a[9]);
+  const int64_t kv_len = a[10] == Py_None ? 0 : PyLong_AsLong(a[10]);
+  if (PyErr_Occurred()) return nullptr;
+  if (q->dim() != 4 || qr->dim() != 4) REFUSE(PyExc_ValueError, "query must be (B, H, T, latent_dim), query_rope (B, H, T, rope_dim)");
+  if (q->scalar_type() != at::kBFloat16 || qr->scalar_type() != at::kBFloat16)
+    REFUSE(PyExc_TypeError, "flex_decode_latent takes bfloat16 query and query_rope");
+  const int64_t B = q->size(0), H = q->size(1), T = q->size(2);
+  if (!latent_ok(*kc, L, table, B)) return nullptr;
+  if (q->size(3) != L || qr->size(0) != B || qr->size(1) != H || qr->size(2) != T || qr->size(3) != kc->size(2) - L)
+    REFUSE(PyExc_ValueError, "sizes of query, query_rope and cache do not match");
+  if (!lens_ok(lens, B, "kv_lens must have one entry per batch row") ||
+      !lens_ok(ql, B, "query_lens must have one entry per batch row"))
+    return nullptr;
+  if (!(scale >= FLT_MIN && scale <= FLT_MAX)) REFUSE(PyExc_ValueError, "scale must be a positive normal float32 number");
+  const int64_t pages = table ? table->size(1) : 1, all = pages * kc->size(1);
+  if (a[10] != Py_None && (kv_len < 1 || kv_len > all)) REFUSE(PyExc_ValueError, "kv_len must be in [1, max_pages * page_size]");
+  const int64_t cap = kv_len ? kv_len : all;
+  if (!sizes_fit(*q) || pages > kMaxSize || cap > kMaxSize) REFUSE(PyExc_ValueError, "sizes must be below 2^31");
+  const at::Device dev = q->device();
+  if (!dev.is_cuda()) REFUSE(PyExc_ValueError, "query and cache must be on the GPU");
+  if (qr->device() != dev || kc->device() != dev) REFUSE(PyExc_ValueError, "query and cache must be on one device");
+  const c10::DeviceGuard guard(dev);
+  at::Tensor o = at::empty(q->sizes(), q->options());
+  at::Tensor lse = at::empty(q->sizes().slice(0, 3), q->options().dtype(at::kFloat));
+  int rc = FA_OK;
+  if (q->numel()) {
+    const at::Tensor qq = rows_ok(*q) ? *q : dense16(*q), rr = rows_ok(*qr) ? *qr : dense16(*qr);
+    at::Tensor ll, tt, qn;
+    fa_latent_call c{};
+    c.abi_version = FA_ABI_VERSION;
+    c.B = static_cast<int32_t>(B);
+    c.T = static_cast<int32_t>(T);
+    c.latent_dim = static_cast<int32_t>(L);
+    c.rope_dim = static_cast<int32_t>(kc->size(2) - L);
+    c.page_size = static_cast<int32_t>(kc->size(1));
+    c.num_pages = static_cast<int32_t>(kc->size(0));
+    c.max_pages = static_cast<int32_t>(pages);
+    c.kv_len = static_cast<int32_t>(cap);
+    c.window_left = static_cast<int32_t>(left);
+    c.window_right = static_cast<int32_t>(right);
+    c.scale = static_cast<float>(scale);
+    c.query = strided(qq);
+    c.query_rope = strided(rr);
+    c.o = o.mutable_data_ptr();
+    c.lse = lse.mutable_data_ptr<float>();
+    c.cache = kc->const_data_ptr();
+    if (table) c.page_table = (tt = row_ints(*table, dev)).const_data_ptr<int32_t>();
+    if (lens) c.kv_lens = (ll = row_ints(*lens, dev)).const_data_ptr<int32_t>();
+    if (ql) c.q_lens = (qn = row_ints(*ql, dev)).const_data_ptr<int32_t>();
+    const size_t bytes = g_latent_ws(&c);
+    at::Tensor ws;
+    if (bytes) ws = at::empty({static_cast<int64_t>(bytes)}, q->options().dtype(at::kByte));
+    rc = g_latent(&c, bytes ? ws.mutable_data_ptr() : nullptr, bytes, stream_of(dev));
+  }
+  return Py_BuildValue("iNN", rc, THPVariable_Wrap(o), THPVariable_Wrap(lse));
+  END_HANDLE_TH_ERRORS
+}
+
+// The tensors of a call on pages: dense, of as many pages each, on one device.
+bool paged_tensors(PyObject* list, std::vector<const at::Tensor*>* t, std::vector<fa_paged_tensor>* out) {
+  if (!PyList_Check(list) || PyList_GET_SIZE(list) < 1) {
+    PyErr_SetString(PyExc_TypeError, "expected a list of tensors");
+    return false;
+  }
+  for (Py_ssize_t i = 0; i < PyList_GET_SIZE(list); ++i) {
+    const at::Tensor* x = tensor(PyList_GET_ITEM(list, i));
+    if (!x) return false;
+    const char* bad = nullptr;
+    if (x->dim() < 2 || x->numel() == 0 || !x->is_contiguous()) bad = "a cache's tensors must be dense (num_pages, ...)";
+    else if (x->size(0) > kMaxSize) bad = "sizes must be below 2^31";
+    else if (!t->empty() && x->size(0) != t->front()->size(0)) bad = "the caches must have as many pages each";
+    else if (!t->empty() && x->device() != t->front()->device()) bad = "the caches must be on one device";
+    if (bad) {
+      PyErr_SetString(PyExc_ValueError, bad);
+      return false;
+    }
+    t->push_back(x);
+    out->push_back({const_cast<void*>(x->const_data_ptr()), x->numel() / x->size(0) * x->element_size()});
+  }
+  return true;
+}
+
+// copy_pages(tensors, src, dst) -> status
+PyObject* py_copy_pages(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  if (n != 3 || !g_copy_pages) REFUSE(PyExc_TypeError, "copy_pages takes 3 arguments, after bind_serve");
+  std::vector<const at::Tensor*> t;
+  std::vector<fa_paged_tensor> p;
+  if (!paged_tensors(a[0], &t, &p)) return nullptr;
+  const at::Tensor *src = tensor(a[1]), *dst;
+  if (!src || !(dst = tensor(a[2]))) return nullptr;
+  for (const at::Tensor* x : {src, dst}) {
+    if (x->scalar_type() != at::kInt && x->scalar_type() != at::kLong) REFUSE(PyExc_TypeError, "page ids must be int32 or int64");
+    if (x->dim() != 1 || x->size(0) != src->size(0) || x->size(0) > kMaxSize)
+      REFUSE(PyExc_ValueError, "src and dst must be vectors of one length");
+  }
+  const at::Device dev = t[0]->device();
+  if (!dev.is_cuda()) REFUSE(PyExc_ValueError, "the caches must be on the GPU");
+  int rc = FA_OK;
+  if (src->size(0)) {
+    const c10::DeviceGuard guard(dev);
+    const at::Tensor s = row_ints(*src, dev), d = row_ints(*dst, dev);
+    rc = g_copy_pages(p.data(), static_cast<int32_t>(p.size()), static_cast<int32_t>(t[0]->size(0)), s.const_data_ptr<int32_t>(),
+                      d.const_data_ptr<int32_t>(), static_cast<int32_t>(s.size(0)), stream_of(dev));
+    if (rc == FA_OK)
+      for (const at::Tensor* x : t) written(*x);
+  }
+  return PyLong_FromLong(rc);
+  END_HANDLE_TH_ERRORS
+}
+
+// page_plan(fork, tensors, page_size, table, kv_lens, parents | None, room | None, room_all, keep | None)
+//   -> (status, table', lens' | None, count)
+PyObject* py_page_plan(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  if (n != 9 || !g_fork) REFUSE(PyExc_TypeError, "page_plan takes 9 arguments, after bind_serve");
+  const bool fork = PyObject_IsTrue(a[0]);
+  std::vector<const at::Tensor*> t;
+  std::vector<fa_paged_tensor> p;
+  if (!paged_tensors(a[1], &t, &p)) return nullptr;
+  const int64_t page_size = PyLong_AsLong(a[2]), room_all = PyLong_AsLong(a[7]);
+  const at::Tensor *table = tensor(a[3]), *lens, *parents, *room, *keep;
+  if (!table || !(lens = tensor(a[4])) || !optional(a[5], &parents) || !optional(a[6], &room) || !optional(a[8], &keep)) return nullptr;
+  if (PyErr_Occurred()) return nullptr;
+  const int64_t pages = t[0]->size(0);
+  if (table->scalar_type() != at::kInt && table->scalar_type() != at::kLong)
+    REFUSE(PyExc_TypeError, "page_table must be int32 or int64");
+  if (table->dim() != 2 || table->size(0) < 1 || table->size(1) < 1) REFUSE(PyExc_ValueError, "page_table must be (B, max_pages)");
+  const int64_t B = table->size(0), M = table->size(1);
+  if (!lens_ok(lens, B, "kv_lens must have one entry per row of the page table")) return nullptr;
+  if (parents && ((parents->scalar_type() != at::kInt && parents->scalar_type() != at::kLong)))
+    REFUSE(PyExc_TypeError, "parents must be int32 or int64");
+  if (parents && (parents->dim() != 1 || parents->size(0) < 1)) REFUSE(PyExc_ValueError, "parents must be a vector of at least one row");
+  const int64_t N = parents ? parents->size(0) : B;
+  if (!lens_ok(room, N, "room must be a number or have one entry per row")) return nullptr;
+  if (room_all < 0 || room_all > kMaxSize) REFUSE(PyExc_ValueError, "room must not be negative, and below 2^31");
+  if (keep && keep->scalar_type() != at::kBool) REFUSE(PyExc_TypeError, "keep must be a bool tensor");
+  if (keep && (keep->dim() != 1 || keep->size(0) != pages)) REFUSE(PyExc_ValueError, "keep must have one entry per page");
+  if (!sizes_fit(*table) || N > kMaxSize || page_size > kMaxSize) REFUSE(PyExc_ValueError, "sizes must be below 2^31");
+  const at::Device dev = t[0]->device();
+  if (!dev.is_cuda()) REFUSE(PyExc_ValueError, "the caches must be on the GPU");
+  if (keep && keep->device() != dev) REFUSE(PyExc_ValueError, "keep must be on the caches' device");
+  const c10::DeviceGuard guard(dev);
+  const at::Tensor tt = row_ints(*table, dev), ll = row_ints(*lens, dev);
+  at::Tensor pp, rr, kk;
+  fa_page_plan_call c{};
+  c.abi_version = FA_ABI_VERSION;
+  c.B = static_cast<int32_t>(B);
+  c.N = static_cast<int32_t>(N);
+  c.max_pages = static_cast<int32_t>(M);
+  c.page_size = static_cast<int32_t>(page_size);
+  c.num_pages = static_cast<int32_t>(pages);
+  c.room_all = static_cast<int32_t>(room_all);
+  c.page_table = tt.const_data_ptr<int32_t>();
+  c.kv_lens = ll.const_data_ptr<int32_t>();
+  if (parents) c.parents = (pp = row_ints(*parents, dev)).const_data_ptr<int32_t>();
+  if (room) c.room = (rr = row_ints(*room, dev)).const_data_ptr<int32_t>();
+  if (keep) c.keep = static_cast<const uint8_t*>((kk = keep->contiguous()).const_data_ptr());
+  const auto ints = tt.options();
+  at::Tensor out = at::empty({N, M}, ints), count = at::empty({}, ints), olens;
+  c.out_table = out.mutable_data_ptr<int32_t>();
+  c.out_count = count.mutable_data_ptr<int32_t>();
+  if (fork) c.out_lens = (olens = at::empty({N}, ints)).mutable_data_ptr<int32_t>();
+  c.tensors = p.data();
+  c.tensor_count = static_cast<int32_t>(p.size());
+  const size_t bytes = (fork ? g_fork_ws : g_compact_ws)(&c);
+  at::Tensor ws = at::empty({static_cast<int64_t>(std::max<size_t>(bytes, 16))}, ints.dtype(at::kByte));
+  const int rc = (fork ? g_fork : g_compact)(&c, ws.mutable_data_ptr(), bytes, stream_of(dev));
+  if (rc == FA_OK)
+    for (const at::Tensor* x : t) written(*x);
+  if (!fork) return Py_BuildValue("iNON", rc, THPVariable_Wrap(out), Py_None, THPVariable_Wrap(count));
+  return Py_BuildValue("iNNN", rc, THPVariable_Wrap(out), THPVariable_Wrap(olens), THPVariable_Wrap(count));
+  END_HANDLE_TH_ERRORS
+}
+
 PyCFunction fast(PyObject* (*f)(PyObject*, PyObject* const*, Py_ssize_t)) {
   return reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)(void)>(f));
 }
@@ -596,6 +1029,12 @@ PyMethodDef methods[] = {
     {"rotary", fast(py_rotary), METH_FASTCALL, nullptr},
     {"append", fast(py_append), METH_FASTCALL, nullptr},
     {"decode", fast(py_decode), METH_FASTCALL, nullptr},
+    {"bind_serve", fast(py_bind_serve), METH_FASTCALL, nullptr},
+    {"prefill", fast(py_prefill), METH_FASTCALL, nullptr},
+    {"latent_append", fast(py_latent_append), METH_FASTCALL, nullptr},
+    {"latent_decode", fast(py_latent_decode), METH_FASTCALL, nullptr},
+    {"copy_pages", fast(py_copy_pages), METH_FASTCALL, nullptr},
+    {"page_plan", fast(py_page_plan), METH_FASTCALL, nullptr},
     {nullptr, nullptr, 0, nullptr}};
 
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_launch", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};

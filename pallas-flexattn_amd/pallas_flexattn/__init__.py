@@ -41,6 +41,9 @@ from pallas_flexattn.block_mask import (
 from pallas_flexattn.fp8 import Fp8Tensor, dequantize_fp8, flex_attention_fp8, quantize_fp8
 from pallas_flexattn.rotary import Rotary, apply_rotary, rotary_embedding
 from pallas_flexattn.kv_cache import Fp8KVCache, append_kv_cache, create_fp8_kv_cache, flex_decode_fp8
+from pallas_flexattn.prefill import flex_prefill
+from pallas_flexattn.latent import LatentKVCache, append_latent_cache, create_latent_cache, flex_decode_latent
+from pallas_flexattn.kv_pages import compact_kv_pages, copy_kv_pages, fork_kv_rows
 from pallas_flexattn.kernel_tuner import (
     get_optimal_params,
     get_kernel_config,
@@ -80,6 +83,14 @@ __all__ = [
     "create_fp8_kv_cache",
     "append_kv_cache",
     "flex_decode_fp8",
+    "flex_prefill",
+    "LatentKVCache",
+    "create_latent_cache",
+    "append_latent_cache",
+    "flex_decode_latent",
+    "copy_kv_pages",
+    "fork_kv_rows",
+    "compact_kv_pages",
     "flash_attention_bwd_preprocess",
     "flash_attention_bwd_dkv",
     "flash_attention_bwd_dq",

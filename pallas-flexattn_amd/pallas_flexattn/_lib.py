@@ -107,6 +107,46 @@ class FaFp8Cache(ctypes.Structure):
                 ("kv_lens", _pi32), ("q_lens", _pi32)]
 
 
+class FaPrefillCall(ctypes.Structure):
+    """Mirror of ``struct fa_prefill_call`` (include/flexattn.h)."""
+    _fields_ = [("abi_version", _i32), ("cache_dtype", _i32), ("B", _i32), ("Hkv", _i32), ("T", _i32), ("D", _i32),
+                ("page_size", _i32), ("max_pages", _i32), ("num_pages", _i32), ("kv_len", _i32), ("window_left", _i32),
+                ("window_right", _i32), ("scale", ctypes.c_float), ("softcap", ctypes.c_float), ("alibi_slopes", _pf),
+                ("query", FaStrided), ("out", FaStrided), ("lse", _pf), ("k_cache", ctypes.c_void_p),
+                ("v_cache", ctypes.c_void_p), ("k_scale", _pf), ("v_scale", _pf), ("page_table", _pi32), ("kv_lens", _pi32),
+                ("q_lens", _pi32), ("q_starts", _pi32)]
+
+
+class FaLatentAppendCall(ctypes.Structure):
+    """Mirror of ``struct fa_latent_append_call`` (include/flexattn.h)."""
+    _fields_ = [("abi_version", _i32), ("B", _i32), ("T", _i32), ("latent_dim", _i32), ("rope_dim", _i32),
+                ("page_size", _i32), ("max_pages", _i32), ("num_pages", _i32), ("latent", FaStrided), ("rope", FaStrided),
+                ("query", FaStrided), ("query_out", ctypes.c_void_p), ("cache", ctypes.c_void_p), ("page_table", _pi32),
+                ("kv_lens", _pi32), ("new_lens", _pi32), ("rotary", FaRotary)]
+
+
+class FaLatentCall(ctypes.Structure):
+    """Mirror of ``struct fa_latent_call`` (include/flexattn.h)."""
+    _fields_ = [("abi_version", _i32), ("B", _i32), ("T", _i32), ("latent_dim", _i32), ("rope_dim", _i32),
+                ("page_size", _i32), ("max_pages", _i32), ("num_pages", _i32), ("kv_len", _i32), ("window_left", _i32),
+                ("window_right", _i32), ("scale", ctypes.c_float), ("query", FaStrided), ("query_rope", FaStrided),
+                ("o", ctypes.c_void_p), ("lse", _pf), ("cache", ctypes.c_void_p), ("page_table", _pi32), ("kv_lens", _pi32),
+                ("q_lens", _pi32)]
+
+
+class FaPagedTensor(ctypes.Structure):
+    """Mirror of ``struct fa_paged_tensor`` (include/flexattn.h)."""
+    _fields_ = [("data", ctypes.c_void_p), ("page_bytes", ctypes.c_int64)]
+
+
+class FaPagePlanCall(ctypes.Structure):
+    """Mirror of ``struct fa_page_plan_call`` (include/flexattn.h)."""
+    _fields_ = [("abi_version", _i32), ("B", _i32), ("N", _i32), ("max_pages", _i32), ("page_size", _i32),
+                ("num_pages", _i32), ("room_all", _i32), ("page_table", _pi32), ("kv_lens", _pi32), ("parents", _pi32),
+                ("room", _pi32), ("keep", ctypes.c_void_p), ("out_table", _pi32), ("out_lens", _pi32), ("out_count", _pi32),
+                ("tensors", ctypes.POINTER(FaPagedTensor)), ("tensor_count", _i32)]
+
+
 EXPORTED = ("fa_fwd", "fa_fwd_fp8", "fa_fwd_fp8_q16", "fa_quantize_fp8", "fa_quantize_fp8_kv", "fa_fwd_host", "fa_bwd_preprocess_host", "fa_bwd_dkdv_host",
             "fa_bwd_dq_host", "fa_bwd_host", "fa_fwd_splitkv", "fa_fwd_splitkv_workspace_bytes", "fa_fwd_kvcache",
             "fa_fwd_kvcache_workspace_bytes", "fa_bwd", "fa_bwd_workspace_bytes", "fa_bwd_split",
@@ -116,7 +156,9 @@ EXPORTED = ("fa_fwd", "fa_fwd_fp8", "fa_fwd_fp8_q16", "fa_quantize_fp8", "fa_qua
             "fa_mods_compile", "fa_mods_free_blob", "fa_mods_load", "fa_mods_unload", "fa_mods_fwd", "fa_mods_bwd",
             "fa_mods_bwd_dkdv", "fa_mods_bwd_dq", "fa_mods_source_hash",
             "fa_apply_rotary", "fa_kv_append", "fa_fwd_kvcache_fp8", "fa_fwd_kvcache_fp8_workspace_bytes",
-            "fa_int64_to_int32")
+            "fa_int64_to_int32", "fa_prefill", "fa_prefill_workspace_bytes", "fa_latent_append", "fa_latent_decode",
+            "fa_latent_decode_workspace_bytes", "fa_copy_pages", "fa_fork_rows", "fa_fork_rows_workspace_bytes",
+            "fa_compact_pages", "fa_compact_pages_workspace_bytes")
 
 MODS_MASK, MODS_SCORE, MODS_BUILTIN_SCORE, MODS_GENERAL = 1, 2, 4, 8
 
@@ -218,6 +260,17 @@ def load():
     lib.fa_fwd_kvcache_fp8_workspace_bytes.restype = ctypes.c_size_t
     lib.fa_int64_to_int32.argtypes = [v, v, ctypes.c_int64, v]
     lib.fa_int64_to_int32.restype = i
+    for name, call in (("fa_prefill", FaPrefillCall), ("fa_latent_decode", FaLatentCall), ("fa_fork_rows", FaPagePlanCall),
+                       ("fa_compact_pages", FaPagePlanCall)):
+        f, size = getattr(lib, name), getattr(lib, name + "_workspace_bytes")
+        f.argtypes = [ctypes.POINTER(call), v, ctypes.c_size_t, v]
+        f.restype = i
+        size.argtypes = [ctypes.POINTER(call)]
+        size.restype = ctypes.c_size_t
+    lib.fa_latent_append.argtypes = [ctypes.POINTER(FaLatentAppendCall), v]
+    lib.fa_latent_append.restype = i
+    lib.fa_copy_pages.argtypes = [ctypes.POINTER(FaPagedTensor), i32, i32, v, v, i32, v]
+    lib.fa_copy_pages.restype = i
     lib.fa_strerror.argtypes = [ctypes.c_int]
     lib.fa_strerror.restype = ctypes.c_char_p
     lib.fa_mods_source_hash.argtypes = []
@@ -253,6 +306,10 @@ def launcher():
         ext.bind_cache(*(ctypes.cast(f, ctypes.c_void_p).value for f in (
             lib.fa_apply_rotary, lib.fa_kv_append, lib.fa_fwd_kvcache_fp8, lib.fa_fwd_kvcache_fp8_workspace_bytes,
             lib.fa_int64_to_int32, lib.fa_strerror)))
+        ext.bind_serve(*(ctypes.cast(f, ctypes.c_void_p).value for f in (
+            lib.fa_prefill, lib.fa_prefill_workspace_bytes, lib.fa_latent_append, lib.fa_latent_decode,
+            lib.fa_latent_decode_workspace_bytes, lib.fa_copy_pages, lib.fa_fork_rows, lib.fa_fork_rows_workspace_bytes,
+            lib.fa_compact_pages, lib.fa_compact_pages_workspace_bytes)))
         _launch = ext
     return _launch
 

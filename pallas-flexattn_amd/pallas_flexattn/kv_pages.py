@@ -1,0 +1,93 @@
+"""The pages of paged KV caches (not in the reference): copying, forking, compacting and freeing them, on the
+GPU and without synchronisation.
+
+Every function takes one cache or a list of caches (the layers of a model) that share page tables: an
+:class:`Fp8KVCache`, the bf16 (key, value) tensors, or a :class:`LatentKVCache`, of equal page
+counts and sizes.  Nothing but the tables and lengths says which pages are in use: those that a row's tokens
+fill, and those that the caller holds for something else (``keep``, (num_pages,) bool: a prefix cache).  All others are
+free, so a row that is not taken over is freed by that.
+
+Page ids, tables and lengths are int32 (read as they are) or int64; what comes back is int32.
+"""
+from . import _lib
+from .flash_attn import _torch
+from .kv_cache import Fp8KVCache, _rows
+from .latent import LatentKVCache
+
+
+def _tensors(caches):
+    """The tensors of a cache or of several, and their page size."""
+    if isinstance(caches, (Fp8KVCache, LatentKVCache)) or (isinstance(caches, tuple) and len(caches) == 2 and
+                                                            all(hasattr(x, "data_ptr") for x in caches)):
+        caches = [caches]
+    if not isinstance(caches, (list, tuple)) or not caches:
+        raise TypeError("caches must be a cache or a list of caches")
+    out, pages = [], set()
+    for c in caches:
+        if isinstance(c, LatentKVCache):
+            parts, dim, at = (c.data,), 3, 1
+        elif isinstance(c, Fp8KVCache) or (isinstance(c, (list, tuple)) and len(c) == 2):
+            parts, dim, at = tuple(c), 4, 2
+        else:
+            raise TypeError("a cache is an Fp8KVCache, a LatentKVCache or a (key, value) pair of tensors")
+        for i, x in enumerate(parts):
+            if not hasattr(x, "data_ptr"):
+                raise TypeError("a cache is made of tensors")
+            if x.dim() != (3 if i > 1 else dim):
+                raise ValueError("key and value are (num_pages, Hkv, page_size, D), latent vectors (num_pages, page_size, dim)")
+            if i < 2:
+                pages.add(x.shape[at])
+        out += parts
+    if len(pages) != 1:
+        raise ValueError("the caches must have one page size")
+    return out, pages.pop()
+
+
+def copy_kv_pages(caches, src, dst) -> None:
+    """Copies page ``src[i]`` to page ``dst[i]`` in every cache, in place (``src``, ``dst``: vectors of page ids on the
+    GPU).  Pairs with an id outside the cache are left out, so a vector may be padded with -1.  The pages ``dst``
+    must be distinct, and none of them among ``src``."""
+    tensors, _ = _tensors(caches)
+    rc = _lib.launcher().copy_pages(tensors, _rows(src, tensors[0]), _rows(dst, tensors[0]))
+    if rc:
+        _lib.check(rc)
+
+
+def _room(room, like):
+    return (None, room) if isinstance(room, int) else (_rows(room, like), 0)
+
+
+def fork_kv_rows(caches, page_table, kv_lens, parents=None, room=0, keep=None):
+    """Rows that go on from other rows -> (page_table, kv_lens, free): the beams of a search after a step, samples of one
+    prompt, a batch some of whose rows ended, or (``parents`` None: each row from itself) just room for the next tokens.
+
+    Row b of the result has the tokens of row ``parents[b]`` of ``page_table`` (B, max_pages) and ``kv_lens`` (B,); a
+    parent outside [0, B) gives an empty row.  Pages that a row's tokens fill are shared by all that have them.  A last page that they fill in
+    part becomes the row's own, to be appended to: the first row that ends in it keeps it, unless another one has the whole of it or it
+    is in ``keep``; the others get a copy, in every cache.  Behind its tokens a row gets pages for ``room`` (a
+    number, or one per row) more, as far as the table goes; the entries behind those are -1.
+
+    Copies and room come from the free pages, lowest first, row by row: pages that neither the result's rows nor ``keep``
+    hold.  ``free`` (int32, on the GPU) is how many are left; where it is negative so many were lacking, and
+    the entries that lack one are -1 (tokens of a copy that could not be made are lost: look before going on).
+    Page ids outside the cache stay as they are."""
+    tensors, page_size = _tensors(caches)
+    per_row, number = _room(room, tensors[0])
+    rc, table, lens, free = _lib.launcher().page_plan(True, tensors, page_size, page_table, _rows(kv_lens, tensors[0]),
+                                                      _rows(parents, tensors[0]), per_row, number, keep)
+    if rc:
+        _lib.check(rc)
+    return table, lens, free
+
+
+def compact_kv_pages(caches, page_table, kv_lens, room: int = 0, keep=None):
+    """Moves the pages in use to the front -> (page_table, used): with n pages in use (that a row's tokens and ``room`` more
+    fill, or ``keep`` holds), those with ids from n on that ``keep`` does not hold move, in every cache, to the
+    free ids below n, both in ascending order.  ``used`` (int32, on the GPU) is n; pages that ``keep`` holds stay where they
+    are.  Entries past a row's tokens and room are -1, page ids outside the cache stay as they are."""
+    tensors, page_size = _tensors(caches)
+    rc, table, _, used = _lib.launcher().page_plan(False, tensors, page_size, page_table, _rows(kv_lens, tensors[0]), None,
+                                                   None, room, keep)
+    if rc:
+        _lib.check(rc)
+    return table, used
