@@ -233,6 +233,7 @@ int decode_args(const fa_params* p, const fa_fp8_cache* kv, int cus, fa::DecodeA
                p->B * (long long)p->Hkv * rows > (1 << 26) - 4;
   // At most four pieces per unit (two where the rows are equally long: decode_unit).
   a->pieces = 4 * cus;
+  a->pieces_even = a->pieces / 2;
   // At least 16 tiles a piece, four per wave, so that the merge stays short (8 of 500
   // 16.5 us, with 8 tiles 18.8); 8 where that makes at most 16 pieces (8 of 126 12.4, 11.8).
   a->least = tiles <= 128 ? 8 : 16;

@@ -55,6 +55,7 @@ struct DecodeArgs {
   const float* alibi;
   int rt;            // query blocks per kv head
   int pieces, least; // what decode_chunk takes
+  int pieces_even;   // pieces where all rows are equally long
   // by_item: a workgroup takes one whole item, nothing is shared.  Else the
   // workspace holds the rows' first units and slots (2 (B + 1) ints) and the slots'
   // O (16 NQ, D) and (m, l) (16 NQ, 2)
@@ -235,7 +236,7 @@ __device__ __forceinline__ DecodeUnit decode_piece_unit(const DecodeArgs& a, int
   // pieces differ by up to half, twice as many come out more even (GPU time with two / four:
   // 8 equal rows of 32768 keys 97 / 99 us, 32 of 3840 49.8 / 51.7, 32 mixed to 8192 59.8 / 54.9,
   // D = 64 32 mixed to 9000 48 / 42).
-  const int pieces = __all(same) ? a.pieces / 2 : a.pieces;
+  const int pieces = __all(same) ? a.pieces_even : a.pieces;
   const int total = __builtin_amdgcn_readlane(wave_scan(sum), 63) * each;
   int chunk = decode_chunk(total, pieces, a.least);
   int p[kRows], units, slots, iu;  // pieces per item, this lane's units and slots

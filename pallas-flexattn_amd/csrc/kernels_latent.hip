@@ -11,7 +11,7 @@ static void run_latent(const LatentArgs& a, int nb, hipStream_t s) {
   switch (nb) {
     case 1: hipLaunchKernelGGL((latent_decode_kernel<L, R, 1>), grid, dim3(256), 0, s, a); break;
     case 2: hipLaunchKernelGGL((latent_decode_kernel<L, R, 2>), grid, dim3(256), 0, s, a); break;
-    default: hipLaunchKernelGGL((latent_decode_kernel<L, R, 4>), grid, dim3(512), 0, s, a); break;
+    default: hipLaunchKernelGGL((latent_decode_kernel<L, R, 4>), grid, dim3(256), 0, s, a); break;
   }
 }
 
@@ -22,8 +22,8 @@ int launch_latent<FA_KERNELS_L>(const LatentArgs& a, int R, int nb, hipStream_t 
   else run_latent<L, 64>(a, nb, s);
   const int rc = launch_status();
   if (rc || a.d.by_item) return rc;
-  const long long units = (long long)a.d.B * a.d.g * a.d.Sq * (L / 128);
-  hipLaunchKernelGGL((latent_merge<L>), dim3((unsigned)((units + 3) / 4)), dim3(256), 0, s, a.d, 16 * nb);
+  const long long units = (long long)a.d.B * a.d.g * a.d.Sq * (L >= 256 ? L / 256 : 1);
+  hipLaunchKernelGGL((latent_merge<L>), dim3((unsigned)((units + 3) / 4)), dim3(256), 0, s, a.d, a.rt, 16 * nb);
   return launch_status();
 }
 

@@ -8,7 +8,8 @@ namespace fa {
 constexpr int kLatentKeys = 64;  // keys of a tile: two runs of 32, each in one page
 
 struct LatentArgs {
-  DecodeArgs d;  // the partition (Hkv = 1, tiles of 32 keys), lengths, page table, windows, workspace, o, lse
+  DecodeArgs d;  // the partition (Hkv = rt = 1, tiles of 32 keys), lengths, page table, windows, workspace, o, lse
+  int rt;        // row blocks of a batch row
   const uint16_t* cache;  // (num_pages, page_size, L + R)
   const void *q, *qr;     // bf16; element strides of (row, head, query)
   long long qsb, qsh, qst, rsb, rsh, rst;

@@ -184,19 +184,21 @@ int latent_args(const fa_latent_call* c, int cus, fa::LatentArgs* a, LatentLayou
   d.win_right = c->window_right < 0 || c->window_right >= c->T - 1 ? -1 : c->window_right;
   d.scale = c->scale;
   d.scale_log2 = c->scale * fa::kLog2e;
-  d.rt = (int)rt;
+  d.rt = 1;
+  a->rt = (int)rt;
   a->cache = static_cast<const uint16_t*>(c->cache);
   a->q = c->query.data;
   a->qsb = c->query.stride_b, a->qsh = c->query.stride_h, a->qst = c->query.stride_t;
   a->qr = c->query_rope.data;
   a->rsb = c->query_rope.stride_b, a->rsh = c->query_rope.stride_h, a->rst = c->query_rope.stride_t;
   d.by_item = tiles <= 8 || (items >= cus && tiles <= 128) || c->B > 64 * fa::kMostLaneRows || c->B * rows > (1 << 22);
-  d.pieces = 2 * cus;
-  d.least = 8;
-  const long long grid = d.by_item ? items : fa::decode_grid(items, (int)tiles, d.pieces, d.least);
+  d.pieces = d.pieces_even = (int)std::max(1ll, cus / rt);
+  d.least = 2;
+  const long long units = d.by_item ? c->B : fa::decode_grid(c->B, (int)tiles, d.pieces, d.least);
+  const long long grid = rt > 1 ? (units + 7) / 8 * 8 * rt : units;
   if (grid > 0x7fffffll) return FA_ERR_SHAPE;
   d.grid = (int)grid;
-  const size_t slots = d.by_item ? 0 : (size_t)fa::decode_slots(grid, d.pieces) * 16 * L->nb;
+  const size_t slots = d.by_item ? 0 : (size_t)fa::decode_slots(units, d.pieces) * rt * 16 * L->nb;
   L->part = ((2 * (size_t)c->B + 2) * sizeof(int) + 255) & ~(size_t)255;
   L->ml = L->part + slots * c->latent_dim * sizeof(float);
   L->bytes = d.by_item ? 0 : L->ml + slots * 2 * sizeof(float);
