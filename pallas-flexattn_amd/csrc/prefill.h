@@ -94,18 +94,459 @@ __device__ __forceinline__ void tanh16(f32x16& x) {
 // bf16 pairs: bits 15 and 31 set where the half is an infinity or a NaN
 __device__ __forceinline__ uint32_t wild_halves(uint32_t w) { return ((w & 0x7f807f80u) + 0x00800080u) & 0x80008000u; }
 
+// The rows of a wave, one per lane (the two lane halves hold one row's other elements): Q, the running softmax and O.
 template <int D, bool kFp8, bool kMods, bool kPacked>
-__global__ __launch_bounds__(256, 2) void prefill_kernel(PrefillArgs a) {
+struct PrefillWave {
   using E = Elt<uint16_t>;
   using frag = E::frag;
+  static constexpr int RB = 2 * D, KCH = D / 8, KSTEPS = D / 16, DT = D / 32;
+  static constexpr float kSpill = 65536.0f;
+  frag qf[KSTEPS];
+  f32x16 oacc[DT];
+  float m, l;
+  KeySpan see;  // keys that the row sees ([0, 2^31 - 1]: a row that is not there, whose results are not written)
+  int qpos;
+  float mod_scale, mod_slope, sl2;  // scores in log2 units are sl2 times what the products hold (modified: see below)
+  int koff[KSTEPS], voff[DT];       // LDS offsets in tiles of keys (K's rows lane % 32 in perm23 order; V's transposing reads)
+
+  struct Row {
+    int qi, hq;
+    bool valid, live;
+  };
+  // (Computed again where the walk is over: kept, it would cost the walk registers, and a spilled one is read back only
+  // behind all copies under way.)
+  __device__ __forceinline__ static Row row(const PrefillArgs& a, const PrefillItem& it, int r) {
+    asm volatile("" : "+v"(r));
+    const int rows = it.nq * a.g;
+    Row x;
+    x.valid = r < rows;
+    const int c = x.valid ? r : rows - 1;
+    x.qi = c / a.g;
+    x.hq = c - x.qi * a.g;
+    x.live = x.valid && x.qi < it.ql;
+    return x;
+  }
+
+  // r: the lane's row of the item's batch row and kv head hk
+  __device__ __forceinline__ void init(const PrefillArgs& a, const PrefillItem& it, int hk, int r, int lane) {
+    const Row x = row(a, it, r);
+    const int hh = lane >> 5;
+    qpos = it.have - it.ql + x.qi;
+    see = key_span(qpos, it.have, a.win_left, a.win_right);
+    if (!x.live) see = KeySpan{0, 0x7fffffff};
+    const uint16_t* qp = static_cast<const uint16_t*>(a.q) + (kPacked ? 0 : it.b) * a.qsb + (hk * a.g + x.hq) * a.qsh +
+                         (long long)(it.tok + x.qi) * a.qst + 8 * hh;
+#pragma unroll
+    for (int s = 0; s < KSTEPS; ++s) qf[s] = *reinterpret_cast<const u32x4*>(qp + 16 * s);
+#pragma unroll
+    for (int s = 0; s < KSTEPS; ++s) qf[s] = x.live ? qf[s] : u32x4{0u, 0u, 0u, 0u};  // (padded tokens may be anything)
+    const float slope = kMods && a.alibi ? a.alibi[hk * a.g + x.hq] : 0.f;
+    const float mod_in = a.softcap > 0.f ? 1.0f / a.softcap : 1.0f;
+    mod_scale = a.scale * mod_in;
+    mod_slope = slope * mod_in;
+    sl2 = kMods ? (a.softcap > 0.f ? a.softcap : 1.0f) * kLog2e : a.scale_log2;
+    m = -INFINITY;
+    l = 0.f;
+#pragma unroll
+    for (int i = 0; i < DT; ++i)
+#pragma unroll
+      for (int e = 0; e < 16; ++e) oacc[i][e] = 0.f;
+    drain();
+    RowTileOffsets<D> kt;
+    kt.init(lane);
+#pragma unroll
+    for (int s = 0; s < KSTEPS; ++s) koff[s] = kt.aoff[s];
+#pragma unroll
+    for (int i = 0; i < DT; ++i) voff[i] = fwd_voff_t<D>(lane, i);
+  }
+  __device__ __forceinline__ void drain() {
+#pragma unroll
+    for (int i = 0; i < DT; ++i) mfma_drain<'v'>(oacc[i]);
+  }
+
+  // With modifiers: (scale q k + slope (key - position)) mod_in, of which a soft-cap's tanh; mod_out is taken with the exponent
+  template <int NSUB>
+  __device__ __forceinline__ void modify(const PrefillArgs& a, f32x16* s, int kbase, int hh) const {
+#pragma unroll
+    for (int j = 0; j < NSUB; ++j) {
+      const float first = mod_slope * (float)(kbase + 32 * j + 8 * hh - qpos);
+#pragma unroll
+      for (int e = 0; e < 16; ++e) s[j][e] = fmaf(s[j][e], mod_scale, fmaf(mod_slope, (float)acc_row(e, 0), first));
+      if (a.softcap > 0.f) tanh16(s[j]);
+    }
+  }
+  template <int NSUB>
+  __device__ __forceinline__ void mask(f32x16* s, int kbase, int hh) const {
+    if (__all(see.lo <= kbase && see.hi >= kbase + 32 * NSUB - 1)) return;
+#pragma unroll
+    for (int j = 0; j < NSUB; ++j) {
+      const int base = kbase + 32 * j + 8 * hh;
+      const uint32_t bits = interval_bits(see.lo - base, see.hi - base);
+#pragma unroll
+      for (int e = 0; e < 16; ++e) s[j][e] = keep_bit(s[j][e], bits, acc_row(e, 0), -INFINITY);
+    }
+  }
+  template <int NSUB>
+  __device__ __forceinline__ float exps(const f32x16* s, frag* pf, float ref) const {
+    float r0 = 0.f, r1 = 0.f;
+#pragma unroll
+    for (int c = 0; c < 2 * NSUB; ++c) {
+      float x[8];
+#pragma unroll
+      for (int t = 0; t < 8; ++t) x[t] = fast_exp2(fmaf(s[c >> 1][8 * (c & 1) + t], sl2, -ref));
+      pf[c] = E::pack(x);
+#pragma unroll
+      for (int t = 0; t < 8; t += 2) {
+        r0 += x[t];
+        r1 += x[t + 1];
+      }
+    }
+    return r0 + r1;
+  }
+  template <int NSUB>
+  __device__ __forceinline__ void softmax(const f32x16* s, frag* pf) {
+    float rs = exps<NSUB>(s, pf, m == -INFINITY ? 0.f : m);
+    if (__any(!(rs <= kSpill) || m == -INFINITY)) {
+      float mx = -INFINITY;
+#pragma unroll
+      for (int j = 0; j < NSUB; ++j)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) mx = fmaxf(mx, s[j][e]);
+      const float mnew = fmaxf(m, pair_max(mx) * sl2);
+      if (__any(mnew > m)) {
+        const float alpha = fast_exp2(m - (mnew == -INFINITY ? 0.f : mnew));
+        l *= alpha;
+        drain();
+#pragma unroll
+        for (int i = 0; i < DT; ++i)
+#pragma unroll
+          for (int e = 0; e < 16; ++e) oacc[i][e] *= alpha;
+        drain();
+        m = mnew;
+      }
+      rs = exps<NSUB>(s, pf, m == -INFINITY ? 0.f : m);
+    }
+    l += rs;
+  }
+  // Gives the rows that see the keys (of the 16 from k0 on, as bits) the infinities and NaN that were taken out of their
+  // values, read from the cache again so that nothing has to be kept for it: products of the largest finite numbers where they
+  // were with 2^16 for each row and visible key overflow to infinity, of both signs to NaN, and leave the other
+  // rows as they are.  (As products because any other change of O made the compiler copy it for every tile.)
+  __device__ __forceinline__ void patch(const PrefillArgs& a, int b, int hk, int k0, int keys, int lane) {
+    const int run = k0 / kTileKeys, pg = run / a.page_runs;  // (of a page that is there: its values were read)
+    const int page = a.page_table ? scalar_load(a.page_table + (size_t)b * a.max_pages, pg) : b;
+    const size_t row = ((size_t)(page * a.Hkv + hk) * a.page_runs + (run - pg * a.page_runs)) * kTileKeys + k0 % kTileKeys;
+    asm volatile("" : "+v"(lane));  // (addresses not kept for the whole walk)
+    const int first = 8 * (lane >> 5);
+    frag seen;
+#pragma unroll
+    for (int y = 0; y < 4; ++y) {
+      const int key = k0 + first + 2 * y;
+      seen[y] = (key >= see.lo && key <= see.hi ? 0x4780u : 0u) | (key + 1 >= see.lo && key + 1 <= see.hi ? 0x47800000u : 0u);
+    }
+#pragma unroll
+    for (int i = 0; i < DT; ++i) {
+      frag up = E::zero(), down = E::zero();
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const bool here = (keys >> (first + e)) & 1;  // (a key past the row's end is in the page all the same)
+        const size_t at = (row + first + e) * D + 32 * i + (lane & 31);
+        bool plus, minus;
+        if constexpr (kFp8) {
+          plus = minus = (static_cast<uint8_t>(a.v[at]) & 0x7f) == 0x7f;
+        } else {
+          const uint32_t v = *reinterpret_cast<const uint16_t*>(a.v + 2 * at);
+          const bool nan = (v & 0x7fffu) > 0x7f80u;
+          plus = nan || v == 0x7f80u;
+          minus = nan || v == 0xff80u;
+        }
+        up[e >> 1] |= (here && plus ? 0x7f7fu : 0u) << (16 * (e & 1));
+        down[e >> 1] |= (here && minus ? 0xff7fu : 0u) << (16 * (e & 1));
+      }
+      mfma_acc<'v', true>(oacc[i], up, seen);
+      mfma_acc<'v', true>(oacc[i], down, seen);
+    }
+  }
+};
+// Takes infinities and NaN out of 1 KB of a V tile in LDS; returns whether this lane's 16 bytes had any.
+__device__ __forceinline__ bool tame(char* at) {
+  u32x4 x = *reinterpret_cast<u32x4*>(at);
+  uint32_t bad = 0u;
+#pragma unroll
+  for (int y = 0; y < 4; ++y) {
+    const uint32_t odd = wild_halves(x[y]) >> 15;  // bits 0 and 16
+    bad |= odd;
+    x[y] &= ~(odd * 0xffffu);
+  }
+  if (bad) *reinterpret_cast<u32x4*>(at) = x;
+  return bad != 0u;
+}
+
+// What a split leaves of a row for the join: m = -inf, nothing (a NaN sum has seen something, whatever the maximum says).
+__device__ __forceinline__ float2 split_ml(float m, float l, bool live) {
+  return !live ? make_float2(-INFINITY, 0.f) : l == l ? make_float2(m, l) : make_float2(0.f, l);
+}
+
+// Where keys lie: lane i holds, for the keys first + step i .. of a batch row, their run (-1: none, or a bad page) and its scales.
+template <bool kFp8>
+struct RunTable {
+  int run = -1;
+  float ks = 1.f, vs = 1.f;
+  __device__ __forceinline__ void load(const PrefillArgs& a, int b, int hk, int have, long long key, long long end) {
+    run = -1;
+    ks = vs = 1.f;
+    if (key < end && key < have) {
+      const int r = (int)(key / kTileKeys), pg = r / a.page_runs;
+      const int page = pg >= a.max_pages ? -1 : a.page_table ? a.page_table[(size_t)b * a.max_pages + pg] : b;
+      if (page >= 0 && page < a.num_pages) {
+        run = (page * a.Hkv + hk) * a.page_runs + (r - pg * a.page_runs);
+        if constexpr (kFp8) {
+          ks = a.ks[run];
+          vs = a.vs[run];
+        }
+      }
+    }
+  }
+  __device__ __forceinline__ static float lane(float x, int i) {
+    return __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(x), i));
+  }
+};
+
+// Items of at most 32 rows (the single tokens of a mixed batch, short chunks): bound by the reads of the cache, so each wave walks
+// every fourth 32-key tile by itself, in a quarter of the LDS, without barriers; the waves join at the end.
+template <int D, bool kFp8, bool kMods, bool kPacked>
+__device__ __forceinline__ void prefill_thin(const PrefillArgs& a, const PrefillItem& it, int hk, int split, TileSpan ts, char* lds) {
+  using W = PrefillWave<D, kFp8, kMods, kPacked>;
+  using frag = typename W::frag;
+  constexpr int RB = W::RB, KCH = W::KCH, DT = W::DT, KSTEPS = W::KSTEPS, TB = 32 * RB;
+  constexpr int IPT = TB / 1024;               // LDS DMA instructions per tile and tensor
+  constexpr int CL = D / 32, PR = D / 16;      // 16-byte loads of codes per lane and tensor, and per row
+  __shared__ float2 tml[4][32];
+  const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int lr = lane & 31, hh = lane >> 5;
+  const int have = it.have;
+  char* kl = lds + w * (2 * TB);
+  char* vl = kl + TB;
+  W x;
+  x.init(a, it, hk, it.row0 + lr, lane);
+  // this wave's tiles: t0 + w, + 4, ..
+  const int t0 = 2 * ts.t0, t1 = imin(2 * ts.t1, (have + 31) / 32);
+  const int n = t1 > t0 + w ? (t1 - t0 - w + 3) / 4 : 0;
+  RunTable<kFp8> tab;
+  int base = -64;
+  auto find = [&](int i) {  // -> lane of tile i
+    if (i - base >= 64) {
+      base = i;
+      tab.load(a, it.b, hk, have, (long long)(t0 + w + 4 * (i + lane)) * 32, (long long)t1 * 32);
+    }
+    return i - base;
+  };
+  auto rsrc = [&](const char* p, int i, int row_bytes) {
+    const int at = find(i), run = __builtin_amdgcn_readlane(tab.run, at);
+    const uint32_t bytes = run < 0 ? 0u : (uint32_t)imin(32, have - (t0 + w + 4 * i) * 32) * row_bytes;
+    return make_rsrc(p + (size_t)imax(run, 0) * kTileKeys * row_bytes, bytes);
+  };
+  [[maybe_unused]] uint32_t dma[IPT];
+  [[maybe_unused]] u32x4 kc[CL], vc[CL];
+  [[maybe_unused]] float ksc = 1.f, vsc = 1.f;
+  auto load_k = [&](int i) {
+    const i32x4 rs = rsrc(a.k, i, kFp8 ? D : RB);
+    if constexpr (kFp8) {
+      ksc = RunTable<kFp8>::lane(tab.ks, i - base);
+#pragma unroll
+      for (int u = 0; u < CL; ++u) kc[u] = buf_load16(rs, (u * 64 + lane) * 16);
+    } else {
+#pragma unroll
+      for (int u = 0; u < IPT; ++u) dma16(rs, (int)(dma[u] & 0xffffu), kl + u * 1024, u == 0);
+    }
+  };
+  auto load_v = [&](int i) {
+    const i32x4 rs = rsrc(a.v, i, kFp8 ? D : RB);
+    if constexpr (kFp8) {
+      vsc = RunTable<kFp8>::lane(tab.vs, i - base);
+#pragma unroll
+      for (int u = 0; u < CL; ++u) vc[u] = buf_load16(rs, (u * 64 + lane) * 16);
+    } else {
+#pragma unroll
+      for (int u = 0; u < IPT; ++u) dma16(rs, (int)(dma[u] >> 16), vl + u * 1024, u == 0);
+    }
+  };
+  auto store = [&](const u32x4* c, float sc, char* tile, auto val) {  // codes of 16 elements a load, as bf16
+#pragma unroll
+    for (int u = 0; u < CL; ++u) {
+      const int at = u * 64 + lane, row = at / PR, ch = 2 * (at % PR);
+#pragma unroll
+      for (int y = 0; y < 2; ++y) {
+        const uint32_t c0 = c[u][2 * y], c1 = c[u][2 * y + 1];
+        const int slot = (ch + y) ^ (decltype(val)::value ? tr_swz<KCH>(row) : chunk_swz<KCH>(row));
+        *reinterpret_cast<u32x4*>(tile + row * RB + slot * 16) =
+            u32x4{cvt_e4m3_lo(c0, sc), cvt_e4m3_hi(c0, sc), cvt_e4m3_lo(c1, sc), cvt_e4m3_hi(c1, sc)};
+      }
+    }
+  };
+  if constexpr (!kFp8) {
+#pragma unroll
+    for (int u = 0; u < IPT; ++u)
+      dma[u] = (uint32_t)tile_dma_offset<D, 32, 1>(lane, 0, u) | (uint32_t)tile_dma_offset<D, 32, 1, true>(lane, 0, u) << 16;
+  }
+  if (n) {
+    load_k(0);
+    load_v(0);
+  }
+  for (int i = 0; i < n; ++i) {
+    const int kbase = (t0 + w + 4 * i) * 32;
+    const bool more = i + 1 < n;
+    if constexpr (kFp8) {
+      store(kc, ksc, kl, False{});
+      if (more) load_k(i + 1);
+    } else {
+      wait_vmem_but<IPT>();  // (V's copies may still be under way)
+    }
+    f32x16 s[1];
+#pragma unroll
+    for (int e = 0; e < 16; ++e) s[0][e] = 0.f;
+#pragma unroll
+    for (int k = 0; k < KSTEPS; ++k) s[0] = W::E::mma(*reinterpret_cast<const u32x4*>(kl + x.koff[k]), x.qf[k], s[0]);
+    __builtin_amdgcn_sched_barrier(0);
+    if constexpr (!kFp8) {
+      if (more) load_k(i + 1);  // (K's reads are done: the products have them)
+    }
+    if constexpr (kMods) x.template modify<1>(a, s, kbase, hh);
+    x.template mask<1>(s, kbase, hh);
+    frag pf[2];
+    x.template softmax<1>(s, pf);
+    if constexpr (kFp8) {
+      store(vc, vsc, vl, True{});
+      if (more) load_v(i + 1);
+    } else {
+      if (more) wait_vmem_but<IPT>();
+      else wait_vmem();
+    }
+    // values that are not finite, where a row does not see all keys of the tile
+    int keys[2] = {0, 0};
+    if (!__all(x.see.lo <= kbase && x.see.hi >= imin(kbase + 32, have) - 1)) {
+#pragma unroll
+      for (int u = 0; u < IPT; ++u) {
+        const unsigned long long bad = __ballot(tame(vl + u * 1024 + lane * 16));
+        for (unsigned long long z = bad; z; z &= z - 1) {
+          const int key = (u * 64 + __builtin_ctzll(z)) / KCH;
+          keys[key >> 4] |= 1 << (key & 15);
+        }
+      }
+    }
+#pragma unroll
+    for (int d = 0; d < DT; ++d)
+#pragma unroll
+      for (int c = 0; c < 2; ++c) {
+        const uint2 lo = lds_read_tr16(vl + x.voff[d] + (16 * c) * RB), hi = lds_read_tr16(vl + x.voff[d] + (16 * c + 4) * RB);
+        mfma_acc<'v', true>(x.oacc[d], u32x4{lo.x, lo.y, hi.x, hi.y}, pf[c]);
+      }
+    __builtin_amdgcn_sched_barrier(0);
+    if (keys[0]) x.patch(a, it.b, hk, kbase, keys[0], lane);
+    if (keys[1]) x.patch(a, it.b, hk, kbase + 16, keys[1], lane);
+    if constexpr (!kFp8) {
+      if (more) load_v(i + 1);
+    }
+  }
+  x.drain();
+  // join: M = max m, L = sum l 2^(m - M), O = sum O 2^(m - M)
+  const float lt = pair_sum(x.l);
+  if (hh == 0) tml[w][lr] = make_float2(x.m, lt);
+  __syncthreads();
+  float M = -INFINITY;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) M = fmaxf(M, tml[i][lr].x);
+  const float c = x.m == -INFINITY ? 0.f : fast_exp2(x.m - M);
+  constexpr int RC = D / 4;  // 16-byte chunks of a float32 row, swizzled by the row
+  char* mine = lds + w * (32 * 4 * D);
+#pragma unroll
+  for (int i = 0; i < DT; ++i)
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      f32x4 y;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) y[e] = c == 0.f ? 0.f : x.oacc[i][4 * j + e] * c;
+      *reinterpret_cast<f32x4*>(mine + lr * (4 * D) + (((8 * i + 2 * j + hh) ^ (lr & (RC - 1))) * 16)) = y;
+    }
+  __syncthreads();
+  constexpr int CW = D / 8;  // columns of a thread, eight threads a row
+  const int orow = tid / 8, col = (tid % 8) * CW;
+  float L = 0.f;
+  M = -INFINITY;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) M = fmaxf(M, tml[i][orow].x);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) L += tml[i][orow].x == -INFINITY ? tml[i][orow].y : tml[i][orow].y * fast_exp2(tml[i][orow].x - M);
+  f32x4 o[CW / 4];
+#pragma unroll
+  for (int k = 0; k < CW / 4; ++k) {
+    const int at = orow * (4 * D) + (((col / 4 + k) ^ (orow & (RC - 1))) * 16);
+    const f32x4* p = reinterpret_cast<const f32x4*>(lds + at);
+    o[k] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const f32x4 y = p[i * (32 * 4 * D) / 16];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) o[k][e] += y[e];
+    }
+  }
+  const int rows = it.nq * a.g;
+  const auto me = W::row(a, it, it.row0 + orow);
+  if (me.valid) {
+    const size_t at = ((size_t)(kPacked ? 0 : it.b) * a.Hq + hk * a.g + me.hq) * a.Sq + it.tok + me.qi;
+    if (a.n_splits > 1) {
+      const size_t all = (size_t)(kPacked ? 1 : a.B) * a.Hq * a.Sq;
+      float* po = a.part + ((size_t)split * all + at) * D + col;
+#pragma unroll
+      for (int k = 0; k < CW / 4; ++k) *reinterpret_cast<f32x4*>(po + 4 * k) = o[k];
+      if (col == 0)
+        *reinterpret_cast<float2*>(a.part + (size_t)a.n_splits * all * D + ((size_t)split * all + at) * 2) =
+            split_ml(M, L, me.live);
+    } else {
+      const bool none = !me.live || L == 0.f;  // (NaN is passed on)
+      const float inv = none ? 0.f : 1.0f / L;
+      uint16_t* po = static_cast<uint16_t*>(a.o) + (kPacked ? 0 : it.b) * a.osb + (hk * a.g + me.hq) * a.osh +
+                     (long long)(it.tok + me.qi) * a.ost + col;
+#pragma unroll
+      for (int k = 0; k < CW / 4; ++k) {
+        const u32x2 y{pack_bf16x2(o[k][0] * inv, o[k][1] * inv), pack_bf16x2(o[k][2] * inv, o[k][3] * inv)};
+        *reinterpret_cast<u32x2*>(po + 4 * k) = none ? u32x2{0u, 0u} : y;
+      }
+      if (col == 0) a.lse[at] = none ? -INFINITY : (M + log2f(L)) * kLn2;
+    }
+  }
+  // the item's further rows are padded tokens
+  const int left = imin(rows - it.row0, kPrefillRows);
+  for (int z = 32 + orow; z < left; z += 32) {
+    const auto pad = W::row(a, it, it.row0 + z);
+    const size_t at = ((size_t)(kPacked ? 0 : it.b) * a.Hq + hk * a.g + pad.hq) * a.Sq + it.tok + pad.qi;
+    if (a.n_splits > 1) {
+      const size_t all = (size_t)(kPacked ? 1 : a.B) * a.Hq * a.Sq;
+      if (col == 0)
+        *reinterpret_cast<float2*>(a.part + (size_t)a.n_splits * all * D + ((size_t)split * all + at) * 2) = make_float2(-INFINITY, 0.f);
+    } else {
+      uint16_t* po = static_cast<uint16_t*>(a.o) + (kPacked ? 0 : it.b) * a.osb + (hk * a.g + pad.hq) * a.osh +
+                     (long long)(it.tok + pad.qi) * a.ost + col;
+#pragma unroll
+      for (int k = 0; k < CW / 4; ++k) *reinterpret_cast<u32x2*>(po + 4 * k) = u32x2{0u, 0u};
+      if (col == 0) a.lse[at] = -INFINITY;
+    }
+  }
+}
+
+template <int D, bool kFp8, bool kMods, bool kPacked>
+__global__ __launch_bounds__(256, D == 128 ? 2 : 3) void prefill_kernel(PrefillArgs a) {
+  using W = PrefillWave<D, kFp8, kMods, kPacked>;
+  using E = typename W::E;
+  using frag = typename W::frag;
   constexpr int BN = kPrefillKeys, NW = 4;
-  constexpr int RB = 2 * D, KCH = D / 8, KSTEPS = D / 16, NSUB = BN / 32, DT = D / 32, NC = BN / 16;
+  constexpr int RB = W::RB, KCH = W::KCH, KSTEPS = W::KSTEPS, DT = W::DT, NSUB = BN / 32, NC = BN / 16;
   constexpr int TILE = BN * RB;
   constexpr int IPW = TILE / 1024 / NW;      // LDS DMA instructions per wave and tensor
   constexpr int WR = BN / NW;                // keys that a wave brings
   constexpr int CL = D >= 64 ? D / 64 : 1;   // 16-byte loads of codes per wave and tensor
   __shared__ __attribute__((aligned(1024))) char lds[4 * TILE];  // K_0, K_1, V_0, V_1
-  __shared__ int wild[2][NW];                // a tile holds values that are not finite (where that matters)
+  __shared__ int wild[2][NW];                // keys of a tile (of each wave's 16) with values that are not finite, where that matters
 
   const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int lr = lane & 31, hh = lane >> 5;
@@ -123,70 +564,42 @@ __global__ __launch_bounds__(256, 2) void prefill_kernel(PrefillArgs a) {
     const SplitRange sr = split_range(ts.t1 - ts.t0, split, a.n_splits, 0);
     ts = TileSpan{ts.t0 + sr.it0, ts.t0 + sr.it1};
   }
-
-  // this lane's row
-  const int r = it.row0 + 32 * w + lr;
-  const bool valid = r < rows;
-  const int qi = (valid ? r : rows - 1) / a.g, hq = (valid ? r : rows - 1) - qi * a.g;
-  const int h = hk * a.g + hq;
-  const bool live = valid && qi < it.ql;
-  const int qpos = have - it.ql + qi;
-  KeySpan see = key_span(qpos, have, a.win_left, a.win_right);
-  if (!live) see = KeySpan{0, 0x7fffffff};  // (its results are not written: nothing to mask)
-  const bool wave_live = __any(live);
-  const float slope = kMods && a.alibi ? a.alibi[h] : 0.f;
-
-  frag qf[KSTEPS];
-  {
-    const uint16_t* qp = static_cast<const uint16_t*>(a.q) + (kPacked ? 0 : it.b) * a.qsb + h * a.qsh + (long long)(it.tok + qi) * a.qst;
-#pragma unroll
-    for (int s = 0; s < KSTEPS; ++s) qf[s] = ld16(qp + (2 * s + hh) * 8, live);
+  if (it.ql * a.g - it.row0 <= 32) {
+    prefill_thin<D, kFp8, kMods, kPacked>(a, it, hk, split, ts, lds);
+    return;
   }
+  W x;
+  x.init(a, it, hk, it.row0 + 32 * w + lr, lane);
 
-  // Where a tile's keys lie: lane i holds, of tile base + i, the run of this wave's 16 keys (-1: none, or a bad page; keys of a
-  // run that are past the row's end read as zeros) and its scales.
-  int tab_base = ts.t0 - 64, run_l = -1;
-  float ks_l = 1.f, vs_l = 1.f;
-  auto table = [&](int t0) {
-    tab_base = t0;
-    run_l = -1;
-    ks_l = vs_l = 1.f;
-    const long long key = (long long)(t0 + lane) * BN + WR * w;
-    if (t0 + lane < ts.t1 && key < have) {
-      const int run = (int)(key / kTileKeys), pg = run / a.page_runs;
-      const int page = pg >= a.max_pages ? -1 : a.page_table ? a.page_table[(size_t)it.b * a.max_pages + pg] : it.b;
-      if (page >= 0 && page < a.num_pages) {
-        run_l = (page * a.Hkv + hk) * a.page_runs + (run - pg * a.page_runs);
-        if constexpr (kFp8) {
-          ks_l = a.ks[run_l];
-          vs_l = a.vs[run_l];
-        }
-      }
-    }
-  };
-  // Byte offset of this wave's 16 keys of tile t (rows of `row` bytes) and how many bytes of them are there.
+  // This wave's 16 keys of tile t: their byte offset (rows of `row` bytes) and how many bytes of them are there (the others read as
+  // zeros).
+  RunTable<kFp8> tab;
+  int tab_base = ts.t0 - 64;
   struct Place {
     size_t at;
     uint32_t bytes;
     float ksc, vsc;
   };
   auto place = [&](int t, int row) {
-    if (t - tab_base >= 64) table(t);
+    if (t - tab_base >= 64) {
+      tab_base = t;
+      tab.load(a, it.b, hk, have, (long long)(t + lane) * BN + WR * w, (long long)ts.t1 * BN);
+    }
     const int i = t - tab_base;
-    const int run = __builtin_amdgcn_readlane(run_l, i);
+    const int run = __builtin_amdgcn_readlane(tab.run, i);
     Place p;
     p.at = ((size_t)imax(run, 0) * kTileKeys + (WR * w) % kTileKeys) * row;
     p.bytes = run < 0 ? 0u : (uint32_t)imin(WR, have - (t * BN + WR * w)) * row;
     p.ksc = p.vsc = 1.f;
     if constexpr (kFp8) {
-      p.ksc = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(ks_l), i));
-      p.vsc = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(vs_l), i));
+      p.ksc = RunTable<kFp8>::lane(tab.ks, i);
+      p.vsc = RunTable<kFp8>::lane(tab.vs, i);
     }
     return p;
   };
 
   // bf16: copies straight to LDS
-  [[maybe_unused]] int dma_k[IPW], dma_v[IPW];
+  [[maybe_unused]] uint32_t dma[IPW];  // lane offsets: K's in the lower half, V's in the upper
   struct Copy {
     i32x4 rk, rv;
     char *kl, *vl;
@@ -197,8 +610,10 @@ __global__ __launch_bounds__(256, 2) void prefill_kernel(PrefillArgs a) {
                 lds + (2 + buf) * TILE + w * (IPW * 1024)};
   };
   [[maybe_unused]] auto copy_one = [&](const Copy& c, int i) {
-    if (i < IPW) dma16(c.rk, dma_k[i], c.kl + i * 1024, i == 0);
-    else dma16(c.rv, dma_v[i - IPW], c.vl + (i - IPW) * 1024, i == IPW);
+    uint32_t off = dma[i % IPW];
+    asm volatile("" : "+v"(off));  // (not unpacked ahead of the loop)
+    if (i < IPW) dma16(c.rk, (int)(off & 0xffffu), c.kl + i * 1024, i == 0);
+    else dma16(c.rv, (int)(off >> 16), c.vl + (i - IPW) * 1024, i == IPW);
   };
   // e4m3: codes in registers, sixteen of a row per load
   [[maybe_unused]] u32x4 kc[CL], vc[CL];
@@ -215,26 +630,26 @@ __global__ __launch_bounds__(256, 2) void prefill_kernel(PrefillArgs a) {
       vc[u] = buf_load16(rv, (u * 64 + lane) * 16);
     }
   };
-  [[maybe_unused]] auto codes_store = [&](int buf) {
+  // (in 2 CL parts: load u of K and of V)
+  [[maybe_unused]] auto codes_store = [&](int buf, int part) {
+    const int u = part >> 1;
+    const bool val = part & 1;
+    const int c = u * 64 + lane, row = WR * w + c / PR, ch = 2 * (c % PR);
+    if (D < 64 && lane >= 32) return;  // (D = 32: the 16 rows take 32 loads)
 #pragma unroll
-    for (int u = 0; u < CL; ++u) {
-      const int c = u * 64 + lane, row = WR * w + c / PR, ch = 2 * (c % PR);
-      if (D < 64 && lane >= 32) break;  // (D = 32: the 16 rows take 32 loads)
-#pragma unroll
-      for (int x = 0; x < 2; ++x) {
-        const uint32_t k0 = kc[u][2 * x], k1 = kc[u][2 * x + 1], v0 = vc[u][2 * x], v1 = vc[u][2 * x + 1];
-        *reinterpret_cast<u32x4*>(lds + buf * TILE + row * RB + (((ch + x) ^ chunk_swz<KCH>(row)) * 16)) =
-            u32x4{cvt_e4m3_lo(k0, ksc), cvt_e4m3_hi(k0, ksc), cvt_e4m3_lo(k1, ksc), cvt_e4m3_hi(k1, ksc)};
-        *reinterpret_cast<u32x4*>(lds + (2 + buf) * TILE + row * RB + (((ch + x) ^ tr_swz<KCH>(row)) * 16)) =
-            u32x4{cvt_e4m3_lo(v0, vsc), cvt_e4m3_hi(v0, vsc), cvt_e4m3_lo(v1, vsc), cvt_e4m3_hi(v1, vsc)};
-      }
+    for (int y = 0; y < 2; ++y) {
+      const uint32_t c0 = val ? vc[u][2 * y] : kc[u][2 * y], c1 = val ? vc[u][2 * y + 1] : kc[u][2 * y + 1];
+      const float sc = val ? vsc : ksc;
+      const int slot = (ch + y) ^ (val ? tr_swz<KCH>(row) : chunk_swz<KCH>(row));
+      *reinterpret_cast<u32x4*>(lds + ((val ? 2 : 0) + buf) * TILE + row * RB + slot * 16) =
+          u32x4{cvt_e4m3_lo(c0, sc), cvt_e4m3_hi(c0, sc), cvt_e4m3_lo(c1, sc), cvt_e4m3_hi(c1, sc)};
     }
   };
   if constexpr (!kFp8) {
 #pragma unroll
     for (int u = 0; u < IPW; ++u) {
-      dma_k[u] = tile_dma_offset<D, BN, NW>(lane, w, u) - WR * w * RB;
-      dma_v[u] = tile_dma_offset<D, BN, NW, true>(lane, w, u) - WR * w * RB;
+      dma[u] = (uint32_t)(tile_dma_offset<D, BN, NW>(lane, w, u) - WR * w * RB) |
+               (uint32_t)(tile_dma_offset<D, BN, NW, true>(lane, w, u) - WR * w * RB) << 16;
     }
   }
   // Keys that all of the item's rows see: a tile with others among its keys has to keep a value that is not finite
@@ -247,124 +662,18 @@ __global__ __launch_bounds__(256, 2) void prefill_kernel(PrefillArgs a) {
   auto look = [&](int t, int buf) {
     if (!cut(t)) return;
     if (lane == 0) wild[buf][w] = 0;
+    int l0 = lane;
+    asm volatile("" : "+v"(l0));
 #pragma unroll
-    for (int u = 0; u < IPW; ++u) {
-      u32x4* at = reinterpret_cast<u32x4*>(lds + (2 + buf) * TILE + (w * IPW + u) * 1024 + lane * 16);
-      u32x4 x = *at;
-      uint32_t bad = 0u;
-#pragma unroll
-      for (int y = 0; y < 4; ++y) {
-        const uint32_t odd = wild_halves(x[y]) >> 15;  // bits 0 and 16
-        bad |= odd;
-        x[y] &= ~(odd * 0xffffu);
-      }
-      if (bad) {
-        *at = x;
-        atomicOr(&wild[buf][w], 1 << ((u * 64 + lane) / KCH));
-      }
-    }
-  };
-
-  RowTileOffsets<D> kt;
-  kt.init(lane);
-  int voff[DT];
-#pragma unroll
-  for (int i = 0; i < DT; ++i) voff[i] = fwd_voff_t<D>(lane, i);
-
-  f32x16 oacc[DT];
-#pragma unroll
-  for (int i = 0; i < DT; ++i)
-#pragma unroll
-    for (int e = 0; e < 16; ++e) oacc[i][e] = 0.f;
-#pragma unroll
-  for (int i = 0; i < DT; ++i) mfma_drain<'v'>(oacc[i]);
-  // Adds what look() took out of a key's value to the rows that see the key: infinities, and NaN.  (From the
-  // cache, so that nothing has to be kept for it.)
-  auto patch = [&](int key) {
-    const int run = key / kTileKeys, pg = run / a.page_runs;  // (of a page that is there: its values were read)
-    const int page = a.page_table ? scalar_load(a.page_table + (size_t)it.b * a.max_pages, pg) : it.b;
-    const size_t row = ((size_t)(page * a.Hkv + hk) * a.page_runs + (run - pg * a.page_runs)) * kTileKeys + key % kTileKeys;
-    const bool sees = key >= see.lo && key <= see.hi;
-#pragma unroll
-    for (int i = 0; i < DT; ++i) mfma_drain<'v'>(oacc[i]);
-#pragma unroll
-    for (int i = 0; i < DT; ++i)
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const size_t at = row * D + 32 * i + 8 * j + 4 * hh;
-        float x[4];
-        if constexpr (kFp8) {
-          const uint32_t y = nan_codes(*reinterpret_cast<const uint32_t*>(a.v + at));
-#pragma unroll
-          for (int e = 0; e < 4; ++e) x[e] = (y >> (8 * e + 7)) & 1u ? __builtin_nanf("") : 0.f;
-        } else {
-          const u32x2 y = *reinterpret_cast<const u32x2*>(a.v + 2 * at);
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const uint32_t z = y[e >> 1];
-            const float v = e & 1 ? bf16_hi(z) : bf16_lo(z);
-            x[e] = fabsf(v) < INFINITY ? 0.f : v;
-          }
-        }
-#pragma unroll
-        for (int e = 0; e < 4; ++e) oacc[i][4 * j + e] += sees ? x[e] : 0.f;
-      }
-#pragma unroll
-    for (int i = 0; i < DT; ++i) mfma_drain<'v'>(oacc[i]);
-  };
-
-  constexpr float kSpill = 65536.0f;
-  float m = -INFINITY, l = 0.f;
-  const float sl2 = kMods ? 1.0f : a.scale_log2;  // (with modifiers the scores are in log2 units already)
-  const float mod_in = a.softcap > 0.f ? 1.0f / a.softcap : 1.0f;
-  const float mod_out = (a.softcap > 0.f ? a.softcap : 1.0f) * kLog2e;
-  auto exps = [&](const f32x16* s, frag* pf, float ref) {
-    float r0 = 0.f, r1 = 0.f;
-#pragma unroll
-    for (int c = 0; c < NC; ++c) {
-      float x[8];
-#pragma unroll
-      for (int t = 0; t < 8; ++t) x[t] = fast_exp2(fmaf(s[c >> 1][8 * (c & 1) + t], sl2, -ref));
-      pf[c] = E::pack(x);
-#pragma unroll
-      for (int t = 0; t < 8; t += 2) {
-        r0 += x[t];
-        r1 += x[t + 1];
-      }
-    }
-    return r0 + r1;
-  };
-  auto softmax = [&](const f32x16* s, frag* pf) {
-    float rs = exps(s, pf, m == -INFINITY ? 0.f : m);
-    if (__any(!(rs <= kSpill) || m == -INFINITY)) {
-      float mx = -INFINITY;
-#pragma unroll
-      for (int j = 0; j < NSUB; ++j)
-#pragma unroll
-        for (int e = 0; e < 16; ++e) mx = fmaxf(mx, s[j][e]);
-      const float mnew = fmaxf(m, pair_max(mx) * sl2);
-      if (__any(mnew > m)) {
-        const float alpha = fast_exp2(m - (mnew == -INFINITY ? 0.f : mnew));
-        l *= alpha;
-#pragma unroll
-        for (int i = 0; i < DT; ++i) mfma_drain<'v'>(oacc[i]);
-#pragma unroll
-        for (int i = 0; i < DT; ++i)
-#pragma unroll
-          for (int e = 0; e < 16; ++e) oacc[i][e] *= alpha;
-#pragma unroll
-        for (int i = 0; i < DT; ++i) mfma_drain<'v'>(oacc[i]);
-        m = mnew;
-      }
-      rs = exps(s, pf, m == -INFINITY ? 0.f : m);
-    }
-    l += rs;
+    for (int u = 0; u < IPW; ++u)
+      if (tame(lds + (2 + buf) * TILE + (w * IPW + u) * 1024 + l0 * 16)) atomicOr(&wild[buf][w], 1 << ((u * 64 + l0) / KCH));
   };
 
   if (ts.t0 < ts.t1) {
     if constexpr (kFp8) {
       codes_load(ts.t0);
-      codes_store(0);
+#pragma unroll
+      for (int i = 0; i < 2 * CL; ++i) codes_store(0, i);
     } else {
       const Copy c = copy_plan(ts.t0, 0);
 #pragma unroll
@@ -375,8 +684,44 @@ __global__ __launch_bounds__(256, 2) void prefill_kernel(PrefillArgs a) {
   if (ts.t0 < ts.t1) look(ts.t0, 0);
   __syncthreads();
 
-  auto step = [&](int t, auto buf_c) {
-    constexpr int buf = decltype(buf_c)::value;
+  // The tiles that some row of this wave sees are [w0, w1): the wave only brings its part of the others.  (Three walks, so that
+  // O is in no branch: the compiler kept it twice where it was.)
+  const bool sees = x.see.hi >= x.see.lo && x.see.hi != 0x7fffffff;
+  int w0 = sees ? x.see.lo / BN : 0x7fffffff;
+  int w1 = sees ? x.see.hi / BN + 1 : 0;
+#pragma unroll
+  for (int d = 1; d < 64; d <<= 1) {
+    w0 = imin(w0, __shfl_xor(w0, d, 64));
+    w1 = imax(w1, __shfl_xor(w1, d, 64));
+  }
+  w0 = __builtin_amdgcn_readfirstlane(imin(imax(w0, ts.t0), ts.t1));
+  w1 = __builtin_amdgcn_readfirstlane(imin(imax(w1, w0), ts.t1));
+  int buf = 0;
+  // the end of a tile: the next one's keys are there, and everyone has left this one
+  auto turn = [&](int t) {
+    const bool more = t + 1 < ts.t1;
+    if constexpr (!kFp8) wait_vmem();
+    if (more) look(t + 1, buf ^ 1);
+    __syncthreads();
+    buf ^= 1;
+  };
+  auto pass = [&](int t) {
+    if (t + 1 < ts.t1) {
+      if constexpr (kFp8) {
+        codes_load(t + 1);
+#pragma unroll
+        for (int i = 0; i < 2 * CL; ++i) codes_store(buf ^ 1, i);
+      } else {
+        const Copy c = copy_plan(t + 1, buf ^ 1);
+#pragma unroll
+        for (int i = 0; i < 2 * IPW; ++i) copy_one(c, i);
+      }
+    }
+    turn(t);
+  };
+  for (int t = ts.t0; t < w0; ++t) pass(t);
+  int toggle = buf * TILE;  // of the LDS offsets: the buffers are a power of two apart
+  for (int t = w0; t < w1; ++t) {
     const int kbase = t * BN;
     const bool more = t + 1 < ts.t1;
     [[maybe_unused]] Copy nc;
@@ -384,135 +729,108 @@ __global__ __launch_bounds__(256, 2) void prefill_kernel(PrefillArgs a) {
       if constexpr (kFp8) codes_load(t + 1);
       else nc = copy_plan(t + 1, buf ^ 1);
     }
-    // a tile that no row of this wave sees only passes by
-    const bool run = wave_live && __any(live && see.lo < kbase + BN && see.hi >= kbase);
-    if (!kFp8 && !run && more) {
 #pragma unroll
-      for (int i = 0; i < 2 * IPW; ++i) copy_one(nc, i);
-    }
-    if (run) {  // wave-uniform
-      const char* kl = lds + buf * TILE;
-      const char* vl = lds + (2 + buf) * TILE;
-      f32x16 s[NSUB];
+    for (int k = 0; k < KSTEPS; ++k) x.koff[k] ^= toggle;
 #pragma unroll
-      for (int j = 0; j < NSUB; ++j)
+    for (int i = 0; i < DT; ++i) x.voff[i] ^= toggle;
+    toggle = TILE;
+    const char* kl = lds;
+    const char* vl = lds + 2 * TILE;
+    f32x16 s[NSUB];
 #pragma unroll
-        for (int e = 0; e < 16; ++e) s[j][e] = 0.f;
-      constexpr int KPF = 2, KR = KPF + 1;  // K fragments ahead of their products
-      frag ka[KR][NSUB];
-      __builtin_amdgcn_s_setprio(1);
+    for (int j = 0; j < NSUB; ++j)
 #pragma unroll
-      for (int x = 0; x < KPF; ++x)
+      for (int e = 0; e < 16; ++e) s[j][e] = 0.f;
+    constexpr int KPF = 2, KR = KPF + 1;  // K fragments ahead of their products
+    frag ka[KR][NSUB];
+    __builtin_amdgcn_s_setprio(1);
 #pragma unroll
-        for (int j = 0; j < NSUB; ++j) ka[x][j] = *reinterpret_cast<const u32x4*>(kl + j * 32 * RB + kt.aoff[x]);
+    for (int k = 0; k < KPF; ++k)
 #pragma unroll
-      for (int x = 0; x < KSTEPS; ++x) {
-        if (x + KPF < KSTEPS) {
+      for (int j = 0; j < NSUB; ++j) ka[k][j] = *reinterpret_cast<const u32x4*>(kl + j * 32 * RB + x.koff[k]);
 #pragma unroll
-          for (int j = 0; j < NSUB; ++j) ka[(x + KPF) % KR][j] = *reinterpret_cast<const u32x4*>(kl + j * 32 * RB + kt.aoff[x + KPF]);
-        }
+    for (int k = 0; k < KSTEPS; ++k) {
+      if (k + KPF < KSTEPS) {
 #pragma unroll
-        for (int j = 0; j < NSUB; ++j) s[j] = E::mma(ka[x % KR][j], qf[x], s[j]);
-        if constexpr (!kFp8) {  // this step's share of the next tile's copies
-#pragma unroll
-          for (int i = 0; i < 2 * IPW; ++i)
-            if (i * KSTEPS / (2 * IPW) == x && more) copy_one(nc, i);
-        }
-        __builtin_amdgcn_sched_barrier(0);
+        for (int j = 0; j < NSUB; ++j) ka[(k + KPF) % KR][j] = *reinterpret_cast<const u32x4*>(kl + j * 32 * RB + x.koff[k + KPF]);
       }
-      __builtin_amdgcn_s_setprio(0);
-      if constexpr (kMods) {
 #pragma unroll
-        for (int j = 0; j < NSUB; ++j) {
-          const float first = (float)(kbase + 32 * j + 8 * hh - qpos);
+      for (int j = 0; j < NSUB; ++j) s[j] = E::mma(ka[k % KR][j], x.qf[k], s[j]);
+      if constexpr (!kFp8) {  // this step's share of the next tile's copies
 #pragma unroll
-          for (int e = 0; e < 16; ++e) s[j][e] = fmaf(slope, first + (float)acc_row(e, 0), s[j][e] * a.scale) * mod_in;
-          if (a.softcap > 0.f) tanh16(s[j]);
-#pragma unroll
-          for (int e = 0; e < 16; ++e) s[j][e] *= mod_out;
-        }
+        for (int i = 0; i < 2 * IPW; ++i)
+          if (i * KSTEPS / (2 * IPW) == k && more) copy_one(nc, i);
       }
-      const bool whole = __all(see.lo <= kbase && see.hi >= kbase + BN - 1);
-      if (!whole) {
-#pragma unroll
-        for (int j = 0; j < NSUB; ++j) {
-          const int base = kbase + 32 * j + 8 * hh;
-          const uint32_t bits = interval_bits(see.lo - base, see.hi - base);
-#pragma unroll
-          for (int e = 0; e < 16; ++e) s[j][e] = keep_bit(s[j][e], bits, acc_row(e, 0), -INFINITY);
-        }
-      }
-      frag vt[2][NC];
-      auto load_vt = [&](int i) {
-#pragma unroll
-        for (int c = 0; c < NC; ++c) {
-          const uint2 lo = lds_read_tr16(vl + voff[i] + (16 * c) * RB);
-          const uint2 hi = lds_read_tr16(vl + voff[i] + (16 * c + 4) * RB);
-          vt[i & 1][c] = u32x4{lo.x, lo.y, hi.x, hi.y};
-        }
-      };
-      load_vt(0);
-      frag pf[NC];
-      softmax(s, pf);
-      // the 2 wait states that an MFMA needs after a VALU write of its operand, once for all of P
-      static_assert(NC == 4, "P fragments");
-      asm volatile("s_nop 1" : "+v"(pf[0]), "+v"(pf[1]), "+v"(pf[2]), "+v"(pf[3]));
-      __builtin_amdgcn_s_setprio(1);
       __builtin_amdgcn_sched_barrier(0);
+    }
+    __builtin_amdgcn_s_setprio(0);
+    if constexpr (kMods) x.template modify<NSUB>(a, s, kbase, hh);
+    x.template mask<NSUB>(s, kbase, hh);
+    frag vt[2][NC];
+    auto load_vt = [&](int i) {
 #pragma unroll
-      for (int i = 0; i < DT; ++i) {
-        if (i + 1 < DT) load_vt(i + 1);
-#pragma unroll
-        for (int c = 0; c < NC; ++c) mfma_acc<'v', false>(oacc[i], vt[i & 1][c], pf[c]);
-        __builtin_amdgcn_sched_barrier(0);
+      for (int c = 0; c < NC; ++c) {
+        const uint2 lo = lds_read_tr16(vl + x.voff[i] + (16 * c) * RB);
+        const uint2 hi = lds_read_tr16(vl + x.voff[i] + (16 * c + 4) * RB);
+        vt[i & 1][c] = u32x4{lo.x, lo.y, hi.x, hi.y};
       }
-      __builtin_amdgcn_s_setprio(0);
-      if (cut(t)) {
-        for (int x = 0; x < NW; ++x) {
-          for (int keys = __builtin_amdgcn_readfirstlane(wild[buf][x]); keys; keys &= keys - 1) patch(kbase + WR * x + __builtin_ctz(keys));
-        }
+    };
+    load_vt(0);
+    frag pf[NC];
+    x.template softmax<NSUB>(s, pf);
+    // the 2 wait states that an MFMA needs after a VALU write of its operand, once for all of P
+    static_assert(NC == 4, "P fragments");
+    asm volatile("s_nop 1" : "+v"(pf[0]), "+v"(pf[1]), "+v"(pf[2]), "+v"(pf[3]));
+    __builtin_amdgcn_s_setprio(1);
+    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+    for (int i = 0; i < DT; ++i) {
+      if (i + 1 < DT) load_vt(i + 1);
+#pragma unroll
+      for (int c = 0; c < NC; ++c) mfma_acc<'v', false>(x.oacc[i], vt[i & 1][c], pf[c]);
+      if constexpr (kFp8) {  // the next tile's codes have come by now
+#pragma unroll
+        for (int p = 0; p < 2 * CL; ++p)
+          if (p * DT / (2 * CL) == i && more) codes_store(buf ^ 1, p);
+      }
+      __builtin_amdgcn_sched_barrier(0);
+    }
+    __builtin_amdgcn_s_setprio(0);
+    if (cut(t)) {
+      for (int y = 0; y < NW; ++y) {
+        const int keys = __builtin_amdgcn_readfirstlane(wild[buf][y]);
+        if (keys) x.patch(a, it.b, hk, kbase + WR * y, keys, lane);
       }
     }
-    if constexpr (kFp8) {
-      if (more) codes_store(buf ^ 1);
-    } else {
-      wait_vmem();
-    }
-    if (more) look(t + 1, buf ^ 1);
-    __syncthreads();
-  };
-  int t = ts.t0;
-  for (; t + 1 < ts.t1; t += 2) {
-    step(t, Int<0>{});
-    step(t + 1, Int<1>{});
+    turn(t);
   }
-  if (t < ts.t1) step(t, Int<0>{});
+  for (int t = w1; t < ts.t1; ++t) pass(t);
 
-#pragma unroll
-  for (int i = 0; i < DT; ++i) mfma_drain<'v'>(oacc[i]);
-  const float lt = pair_sum(l);
+  x.drain();
+  const float lt = pair_sum(x.l);
+  const auto me = W::row(a, it, it.row0 + 32 * w + lr);
   // row of lse (and of the partial results)
-  const size_t at = ((size_t)(kPacked ? 0 : it.b) * a.Hq + h) * a.Sq + it.tok + qi;
+  const size_t at = ((size_t)(kPacked ? 0 : it.b) * a.Hq + hk * a.g + me.hq) * a.Sq + it.tok + me.qi;
   if (a.n_splits > 1) {
     const size_t all = (size_t)(kPacked ? 1 : a.B) * a.Hq * a.Sq;
-    if (valid) {
+    if (me.valid) {
       float* po = a.part + ((size_t)split * all + at) * D;
-      if (ts.t0 < ts.t1 && live) {  // (else m = -inf says that there is no O)
+      if (ts.t0 < ts.t1 && me.live) {  // (else m = -inf says that there is no O)
 #pragma unroll
         for (int i = 0; i < DT; ++i)
 #pragma unroll
           for (int j = 0; j < 4; ++j)
             *reinterpret_cast<f32x4*>(po + 32 * i + 8 * j + 4 * hh) =
-                f32x4{oacc[i][4 * j], oacc[i][4 * j + 1], oacc[i][4 * j + 2], oacc[i][4 * j + 3]};
+                f32x4{x.oacc[i][4 * j], x.oacc[i][4 * j + 1], x.oacc[i][4 * j + 2], x.oacc[i][4 * j + 3]};
       }
       if (hh == 0)
         *reinterpret_cast<float2*>(a.part + (size_t)a.n_splits * all * D + ((size_t)split * all + at) * 2) =
-            live ? make_float2(m, lt) : make_float2(-INFINITY, 0.f);
+            split_ml(x.m, lt, me.live);
     }
     return;
   }
   // O through the wave's part of the (now idle) tiles, so that a store writes whole row segments
-  const bool none = !live || lt == 0.f;  // (NaN is passed on)
+  const bool none = !me.live || lt == 0.f;  // (NaN is passed on)
   const float inv = none ? 0.f : 1.0f / lt;
   constexpr int RPI = 64 / KCH;
   char* stage = lds + w * (32 * RB);
@@ -521,73 +839,68 @@ __global__ __launch_bounds__(256, 2) void prefill_kernel(PrefillArgs a) {
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
       const int c = 4 * i + j;
-      const u32x2 x{pack_bf16x2(oacc[i][4 * j] * inv, oacc[i][4 * j + 1] * inv),
-                    pack_bf16x2(oacc[i][4 * j + 2] * inv, oacc[i][4 * j + 3] * inv)};
-      *reinterpret_cast<u32x2*>(stage + lr * RB + ((c ^ (lr % KCH)) * 16) + hh * 8) = none ? u32x2{0u, 0u} : x;
+      const u32x2 y{pack_bf16x2(x.oacc[i][4 * j] * inv, x.oacc[i][4 * j + 1] * inv),
+                    pack_bf16x2(x.oacc[i][4 * j + 2] * inv, x.oacc[i][4 * j + 3] * inv)};
+      *reinterpret_cast<u32x2*>(stage + lr * RB + ((c ^ (lr % KCH)) * 16) + hh * 8) = none ? u32x2{0u, 0u} : y;
     }
   const int c = lane % KCH;
 #pragma unroll
   for (int k = 0; k < 32 / RPI; ++k) {
     const int rr = k * RPI + lane / KCH, row = it.row0 + 32 * w + rr;
-    const u32x4 x = *reinterpret_cast<const u32x4*>(stage + rr * RB + ((c ^ (rr % KCH)) * 16));
+    const u32x4 y = *reinterpret_cast<const u32x4*>(stage + rr * RB + ((c ^ (rr % KCH)) * 16));
     if (row < rows) {
       const int i = row / a.g, hr = row - i * a.g;
       uint16_t* o = static_cast<uint16_t*>(a.o) + (kPacked ? 0 : it.b) * a.osb + (hk * a.g + hr) * a.osh + (long long)(it.tok + i) * a.ost;
-      *reinterpret_cast<u32x4*>(o + c * 8) = x;
+      *reinterpret_cast<u32x4*>(o + c * 8) = y;
     }
   }
-  if (valid && hh == 0) a.lse[at] = none ? -INFINITY : (m + log2f(lt)) * kLn2;
+  if (me.valid && hh == 0) a.lse[at] = none ? -INFINITY : (x.m + log2f(lt)) * kLn2;
 }
 
-// The splits of a row: M = max m_s, L = sum l_s 2^(m_s - M), O = sum O_s 2^(m_s - M) / L.  A wave per row;
-// lane s of 64 holds split s's factor, the columns go over the lanes.
+// The splits of a row: M = max m_s, L = sum l_s 2^(m_s - M), O = sum O_s 2^(m_s - M) / L.  Four columns a thread, D / 4
+// threads a row, so that a wave has several rows under way; the factors come from the cache twice.
 template <int D>
 __global__ __launch_bounds__(256) void prefill_merge(PrefillArgs a, long long rows) {
-  constexpr int CPL = D >= 64 ? D / 64 : 1, DEEP = 8;
-  const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
-  const long long row = (long long)blockIdx.x * 4 + w;
+  constexpr int TPR = D / 4, DEEP = 4;
+  const long long row = ((long long)blockIdx.x * 256 + threadIdx.x) / TPR;
   if (row >= rows) return;
-  const int n = a.n_splits;
-  const float* ml = a.part + (size_t)n * rows * D;
-  const int col = lane * CPL < D ? lane * CPL : 0;
-  float2 x = make_float2(-INFINITY, 0.f);
-  if (lane < n) x = *reinterpret_cast<const float2*>(ml + ((size_t)lane * rows + row) * 2);
-  float M = x.x;
+  const int n = a.n_splits, col = 4 * (threadIdx.x % TPR);
+  const float2* ml = reinterpret_cast<const float2*>(a.part + (size_t)n * rows * D) + row;
+  const float* part = a.part + (size_t)row * D + col;
+  float M = -INFINITY;
+  for (int s0 = 0; s0 < n; s0 += 8) {
+    float x[8];
 #pragma unroll
-  for (int d = kPrefillSplits / 2; d >= 1; d >>= 1) M = fmaxf(M, __shfl_xor(M, d));
-  M = __shfl(M, 0);
-  const float c = x.x == -INFINITY ? 0.f : fast_exp2(x.x - M);
-  float L = x.y * c;
+    for (int u = 0; u < 8; ++u) x[u] = ml[(size_t)imin(s0 + u, n - 1) * rows].x;
 #pragma unroll
-  for (int d = kPrefillSplits / 2; d >= 1; d >>= 1) L += __shfl_xor(L, d);
-  L = __shfl(L, 0);
-  float acc[CPL];
-#pragma unroll
-  for (int k = 0; k < CPL; ++k) acc[k] = 0.f;
+    for (int u = 0; u < 8; ++u) M = fmaxf(M, x[u]);
+  }
+  f32x4 acc = {0.f, 0.f, 0.f, 0.f};
+  float L = 0.f;
   for (int s0 = 0; s0 < n; s0 += DEEP) {
-    float y[DEEP][CPL];
+    float2 x[DEEP];
+    f32x4 y[DEEP];
 #pragma unroll
     for (int u = 0; u < DEEP; ++u) {
-      const float* p = a.part + ((size_t)imin(s0 + u, n - 1) * rows + row) * D + col;
-#pragma unroll
-      for (int k = 0; k < CPL; ++k) y[u][k] = p[k];
+      const size_t s = imin(s0 + u, n - 1);
+      x[u] = ml[s * rows];
+      y[u] = *reinterpret_cast<const f32x4*>(part + s * rows * D);
     }
 #pragma unroll
     for (int u = 0; u < DEEP; ++u) {
-      const float cs = __shfl(c, (s0 + u) & 63);
-      const bool there = s0 + u < n && !(cs == 0.f);  // (a split without a visible key has no O; NaN is passed on)
+      const bool there = s0 + u < n && x[u].x != -INFINITY;  // (a split without a visible key has no O)
+      const float c = there ? fast_exp2(x[u].x - M) : 0.f;
+      L = there ? fmaf(x[u].y, c, L) : L;
 #pragma unroll
-      for (int k = 0; k < CPL; ++k) acc[k] = there ? fmaf(y[u][k], cs, acc[k]) : acc[k];
+      for (int k = 0; k < 4; ++k) acc[k] = there ? fmaf(y[u][k], c, acc[k]) : acc[k];
     }
   }
-  const float inv = L == 0.f ? 0.f : 1.0f / L;
-  if (lane * CPL < D) {
-    const long long tok = row % a.Sq, bh = row / a.Sq;
-    uint16_t* o = static_cast<uint16_t*>(a.o) + (bh / a.Hq) * a.osb + (bh % a.Hq) * a.osh + tok * a.ost + col;
-    if constexpr (CPL == 2) *reinterpret_cast<uint32_t*>(o) = L == 0.f ? 0u : pack_bf16x2(acc[0] * inv, acc[CPL - 1] * inv);
-    else *o = L == 0.f ? (uint16_t)0 : (uint16_t)(pack_bf16x2(acc[0] * inv, 0.f) & 0xffffu);
-  }
-  if (lane == 0) a.lse[row] = L == 0.f ? -INFINITY : (M + log2f(L)) * kLn2;
+  const float inv = L == 0.f ? 0.f : 1.0f / L;  // (NaN is passed on)
+  const long long tok = row % a.Sq, bh = row / a.Sq;
+  uint16_t* o = static_cast<uint16_t*>(a.o) + (bh / a.Hq) * a.osb + (bh % a.Hq) * a.osh + tok * a.ost + col;
+  *reinterpret_cast<u32x2*>(o) =
+      L == 0.f ? u32x2{0u, 0u} : u32x2{pack_bf16x2(acc[0] * inv, acc[1] * inv), pack_bf16x2(acc[2] * inv, acc[3] * inv)};
+  if (col == 0) a.lse[row] = L == 0.f ? -INFINITY : (M + log2f(L)) * kLn2;
 }
 
 }  // namespace fa
