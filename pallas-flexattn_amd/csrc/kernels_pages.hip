@@ -14,9 +14,8 @@ int launch_copy_pages(const CopyArgs& a, hipStream_t s) {
 
 int launch_page_plan(const PagePlan& a, bool fork, hipStream_t s) {
   if (!a.marks) {
-    const size_t lds = (size_t)a.num_pages * sizeof(int);
-    if (fork) hipLaunchKernelGGL((page_plan_kernel<true>), dim3(1), dim3(kPlanThreads), lds, s, a);
-    else hipLaunchKernelGGL((page_plan_kernel<false>), dim3(1), dim3(kPlanThreads), lds, s, a);
+    if (fork) hipLaunchKernelGGL(fork_plan_kernel, dim3(1), dim3(kPlanThreads), 0, s, a);
+    else hipLaunchKernelGGL(compact_plan_kernel, dim3(1), dim3(kPlanThreads), 0, s, a);
     return launch_status();
   }
   const unsigned rows = (unsigned)((a.N + 3) / 4), wide = rows < 2048u ? rows : 2048u;

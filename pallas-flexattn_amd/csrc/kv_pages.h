@@ -6,9 +6,9 @@
 // kCopyTensors, in pieces of kCopyPiece bytes, four 16-byte loads a thread before its stores.
 //
 // Plans are bound by latency: a chain of a few dependent reads (parent, length, page
-// id), a mark per page, and ranks of the free pages.  Where the marks fit in LDS one
+// id), a mark per page, and ranks of the free pages.  Where marks and rows fit in LDS one
 // workgroup does all of it in one launch; else the marks lie in the workspace and three
-// launches follow each other.  A mark is the smallest claim on its page, so no result
+// launches (a compaction: four) follow each other.  A mark is the smallest claim on its page, so no result
 // depends on the order of the atomics.
 #pragma once
 #include "common.h"
@@ -78,27 +78,20 @@ __device__ __forceinline__ int block_scan(int x, int* part, int* all) {
   return before + s - x;
 }
 
-// The marks of the pages: in LDS, or in the workspace (atomics and reads past the
-// caches: other workgroups write them too).
-template <bool kLds>
+// The marks of the pages in the workspace (atomics and reads past the caches: other workgroups write them too).
 struct Marks {
   int* p;
   __device__ __forceinline__ void set(int i, int x) const { p[i] = x; }
   __device__ __forceinline__ void claim(int i, int x) const { atomicMin(&p[i], x); }
-  __device__ __forceinline__ int get(int i) const {
-    if constexpr (kLds) return p[i];
-    else return __hip_atomic_load(&p[i], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-  }
+  __device__ __forceinline__ int get(int i) const { return __hip_atomic_load(&p[i], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); }
 };
 
-template <class M>
-__device__ __forceinline__ void marks_init(const PagePlan& a, const M& m, int tid, int stride) {
+__device__ __forceinline__ void marks_init(const PagePlan& a, const Marks& m, int tid, int stride) {
   for (int i = tid; i < a.num_pages; i += stride) m.set(i, a.keep && a.keep[i] ? kPageHeld : kPageFree);
 }
 
 // Rows wave, wave + waves, ..: the entries that a row keeps go into the new table, whole pages and last ones are claimed.
-template <class M>
-__device__ __forceinline__ void fork_mark(const PagePlan& a, const M& m, int wave, int waves) {
+__device__ __forceinline__ void fork_mark(const PagePlan& a, const Marks& m, int wave, int waves) {
   const int lane = threadIdx.x & 63;
   for (int b = wave; b < a.N; b += waves) {
     const ForkRow r = fork_row(a, b);
@@ -114,8 +107,7 @@ __device__ __forceinline__ void fork_mark(const PagePlan& a, const M& m, int wav
 }
 
 // One workgroup: which rows need fresh pages, the free ones in ascending order, and who gets which.
-template <class M>
-__device__ __forceinline__ void fork_assign(const PagePlan& a, const M& m, int* part) {
+__device__ __forceinline__ void fork_assign(const PagePlan& a, const Marks& m, int* part) {
   const int tid = threadIdx.x;
   int need = 0;  // of all rows so far
   for (int b0 = 0; b0 < a.N; b0 += kPlanThreads) {
@@ -182,8 +174,7 @@ __device__ __forceinline__ void fork_assign(const PagePlan& a, const M& m, int* 
 }
 
 // Every page id that a row names is claimed as used (kPageUsed; what others hold keeps its mark).
-template <class M>
-__device__ __forceinline__ void compact_mark(const PagePlan& a, const M& m, int wave, int waves) {
+__device__ __forceinline__ void compact_mark(const PagePlan& a, const Marks& m, int wave, int waves) {
   const int lane = threadIdx.x & 63;
   for (int b = wave; b < a.N; b += waves) {
     const ForkRow r = fork_row(a, b);
@@ -196,8 +187,7 @@ __device__ __forceinline__ void compact_mark(const PagePlan& a, const M& m, int 
 }
 
 // One workgroup: pages past the number in use move to the free ones before it; a mark becomes its page's new id.
-template <class M>
-__device__ __forceinline__ void compact_assign(const PagePlan& a, const M& m, int* part) {
+__device__ __forceinline__ void compact_assign(const PagePlan& a, const Marks& m, int* part) {
   const int tid = threadIdx.x;
   int n = 0;
   for (int i = tid; i < a.num_pages; i += kPlanThreads) n += m.get(i) != kPageFree;
@@ -232,8 +222,7 @@ __device__ __forceinline__ void compact_assign(const PagePlan& a, const M& m, in
   }
 }
 
-template <class M>
-__device__ __forceinline__ void compact_write(const PagePlan& a, const M& m, int wave, int waves) {
+__device__ __forceinline__ void compact_write(const PagePlan& a, const Marks& m, int wave, int waves) {
   const int lane = threadIdx.x & 63;
   for (int b = wave; b < a.N; b += waves) {
     const ForkRow r = fork_row(a, b);
@@ -249,46 +238,184 @@ __device__ __forceinline__ void compact_write(const PagePlan& a, const M& m, int
   }
 }
 
-template <bool kFork>
-__global__ __launch_bounds__(kPlanThreads) void page_plan_kernel(PagePlan a) {
-  extern __shared__ int marks[];
+// f(i, x[i]) of i < n over the workgroup's threads, eight loads x(i) under way at a time.
+template <class X, class F>
+__device__ __forceinline__ void plan_each(int n, int tid, X x, F f) {
+  for (int i0 = tid; i0 < n; i0 += 8 * kPlanThreads) {
+    int y[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) y[j] = i0 + j * kPlanThreads < n ? x(i0 + j * kPlanThreads) : 0;
+#pragma unroll
+    for (int j = 0; j < 8; ++j)
+      if (i0 + j * kPlanThreads < n) f(i0 + j * kPlanThreads, y[j]);
+  }
+}
+__device__ __forceinline__ void plan_marks(const PagePlan& a, int* marks, int tid) {
+  plan_each(a.num_pages, tid, [&](int i) { return a.keep ? (int)a.keep[i] : 0; },
+            [&](int i, int held) { marks[i] = held ? kPageHeld : kPageFree; });
+}
+
+// A small fork in one launch.  Rows are a thread's each at first (a row after the other in a wave took 2 us a row: three
+// reads that wait for each other), entries all threads' together; a free page's thread finds by its rank
+// the row that gets it and writes it there.  64 rows of 57 pages among 6000: 11.2 us with rows by waves and the free pages
+// in a list, 9.8 so (8 rows of one prompt 6).
+__global__ __launch_bounds__(kPlanThreads) void fork_plan_kernel(PagePlan a) {
+  __shared__ int marks[kPlanPages];
+  __shared__ int parent[kPlanRows], len[kPlanRows], want[kPlanRows], first[kPlanRows], last[kPlanRows];  // last: a page to copy, or -1
   __shared__ int part[kPlanThreads / 64];
-  const Marks<true> m{marks};
-  const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  marks_init(a, m, tid, kPlanThreads);
+  const int tid = threadIdx.x;
+  plan_marks(a, marks, tid);
+  ForkRow mine{0, 0, 0, 0, 0};
+  int id = -1;
+  if (tid < a.N) {
+    mine = fork_row(a, tid);
+    parent[tid] = mine.parent;
+    len[tid] = mine.len;
+    want[tid] = mine.want;
+    a.out_lens[tid] = mine.len;
+    if (mine.have > mine.whole) id = a.table[(size_t)mine.parent * a.max_pages + mine.whole];
+    if (id >= a.num_pages) id = -1;
+  }
   __syncthreads();
-  if constexpr (kFork) {
-    fork_mark(a, m, wave, kPlanThreads / 64);
-    __syncthreads();
-    fork_assign(a, m, part);
-  } else {
-    compact_mark(a, m, wave, kPlanThreads / 64);
-    __syncthreads();
-    compact_assign(a, m, part);
-    __syncthreads();
-    compact_write(a, m, wave, kPlanThreads / 64);
+  const int entries = a.N * a.max_pages;
+  plan_each(entries, tid,
+            [&](int i) {
+              const int b = i / a.max_pages, e = i - b * a.max_pages;
+              return (long long)e * a.page_size < len[b] ? a.table[(size_t)parent[b] * a.max_pages + e] : -1;
+            },
+            [&](int i, int x) {
+              const int b = i / a.max_pages, e = i - b * a.max_pages;
+              a.out_table[i] = x;
+              // (every claim on such a page says so or more)
+              if ((e + 1ll) * a.page_size <= len[b] && x >= 0 && x < a.num_pages) marks[x] = kPageHeld;
+            });
+  __syncthreads();
+  if (id >= 0) atomicMin(&marks[id], tid);
+  __syncthreads();
+  const bool copy = id >= 0 && marks[id] != tid;
+  int need;
+  const int at = block_scan(tid < a.N ? copy + mine.want - mine.have : 0, part, &need);
+  if (tid < a.N) {
+    first[tid] = at;
+    last[tid] = copy ? id : -1;
+  }
+  __syncthreads();
+  int free = 0;
+  for (int p0 = 0; p0 < a.num_pages; p0 += 4 * kPlanThreads) {
+    const int p = p0 + 4 * tid;
+    bool is[4];
+    int n = 0;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      is[j] = p + j < a.num_pages && marks[imin(p + j, kPlanPages - 1)] == kPageFree;
+      n += is[j];
+    }
+    int all;
+    int rank = free + block_scan(n, part, &all);
+    free += all;
+    if (rank >= need) continue;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      if (!is[j]) continue;
+      if (rank < need) {  // of the rows that begin there the last one: those before it need none
+        int lo = 0, hi = a.N;
+        while (hi - lo > 1) {
+          const int mid = (lo + hi) / 2;
+          if (first[mid] <= rank) lo = mid;
+          else hi = mid;
+        }
+        const int k = rank - first[lo], c = last[lo] >= 0;
+        const int whole = (unsigned)len[lo] / (unsigned)a.page_size, have = whole + ((unsigned)len[lo] % (unsigned)a.page_size != 0u);
+        a.out_table[(size_t)lo * a.max_pages + (c && k == 0 ? whole : have + k - c)] = p + j;
+        if (c && k == 0) a.pair_dst[lo] = p + j;
+      }
+      ++rank;
+    }
+  }
+  if (tid == 0) *a.out_count = free - need;
+  if (tid < a.N) {
+    a.pair_src[tid] = copy && at < free ? id : -1;
+    if (copy && at >= free) a.out_table[(size_t)tid * a.max_pages + mine.whole] = -1;  // none left
   }
 }
 
-// The same in launches of their own, the marks in the workspace.
+// A small compaction in one launch.
+__global__ __launch_bounds__(kPlanThreads) void compact_plan_kernel(PagePlan a) {
+  __shared__ int marks[kPlanPages];
+  __shared__ uint16_t list[kPlanPages / 2 + 1];
+  __shared__ int want[kPlanRows];
+  __shared__ int part[kPlanThreads / 64];
+  const int tid = threadIdx.x;
+  plan_marks(a, marks, tid);
+  if (tid < a.N) want[tid] = fork_row(a, tid).want;
+  __syncthreads();
+  const int entries = a.N * a.max_pages;
+  auto entry = [&](int i) {
+    const int b = i / a.max_pages;
+    return i - b * a.max_pages < want[b] ? a.table[i] : -1;
+  };
+  plan_each(entries, tid, entry, [&](int, int x) {
+    if (x >= 0 && x < a.num_pages) atomicMin(&marks[x], kPageUsed);
+  });
+  __syncthreads();
+  int n = 0;
+  for (int i = tid; i < a.num_pages; i += kPlanThreads) n += marks[i] != kPageFree;
+  int used;
+  block_scan(n, part, &used);
+  int slots = 0;
+  for (int p0 = 0; p0 < used; p0 += kPlanThreads) {
+    const int p = p0 + tid;
+    const bool is = p < used && marks[p] == kPageFree;
+    int all;
+    const int rank = slots + block_scan(is, part, &all);
+    if (is) list[rank] = (uint16_t)p;
+    slots += all;
+  }
+  __syncthreads();
+  int moved = 0;
+  for (int p0 = used / kPlanThreads * kPlanThreads; p0 < a.num_pages; p0 += kPlanThreads) {
+    const int p = p0 + tid;
+    const bool is = p >= used && p < a.num_pages && marks[p] == kPageUsed;
+    int all;
+    const int rank = moved + block_scan(is, part, &all);
+    if (is) {  // (pages in use past the number in use: no more than free ones before it)
+      const int to = list[rank];
+      a.pair_src[rank] = p;
+      a.pair_dst[rank] = to;
+      marks[p] = to;
+    }
+    moved += all;
+  }
+  if (tid == 0) {
+    *a.out_count = used;
+    *a.moved = moved;
+  }
+  __syncthreads();
+  plan_each(entries, tid, entry, [&](int i, int x) {
+    if (x >= used && x < a.num_pages && marks[x] >= 0) x = marks[x];  // (what others hold stays)
+    a.out_table[i] = x;
+  });
+}
+
+// Larger ones in launches of their own, the marks in the workspace.
 __global__ __launch_bounds__(256) void page_init_kernel(PagePlan a) {
-  marks_init(a, Marks<false>{a.marks}, blockIdx.x * 256 + threadIdx.x, gridDim.x * 256);
+  marks_init(a, Marks{a.marks}, blockIdx.x * 256 + threadIdx.x, gridDim.x * 256);
 }
 template <bool kFork>
 __global__ __launch_bounds__(256) void page_mark_kernel(PagePlan a) {
   const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
-  if constexpr (kFork) fork_mark(a, Marks<false>{a.marks}, blockIdx.x * 4 + wave, gridDim.x * 4);
-  else compact_mark(a, Marks<false>{a.marks}, blockIdx.x * 4 + wave, gridDim.x * 4);
+  if constexpr (kFork) fork_mark(a, Marks{a.marks}, blockIdx.x * 4 + wave, gridDim.x * 4);
+  else compact_mark(a, Marks{a.marks}, blockIdx.x * 4 + wave, gridDim.x * 4);
 }
 template <bool kFork>
 __global__ __launch_bounds__(kPlanThreads) void page_assign_kernel(PagePlan a) {
   __shared__ int part[kPlanThreads / 64];
-  if constexpr (kFork) fork_assign(a, Marks<false>{a.marks}, part);
-  else compact_assign(a, Marks<false>{a.marks}, part);
+  if constexpr (kFork) fork_assign(a, Marks{a.marks}, part);
+  else compact_assign(a, Marks{a.marks}, part);
 }
 __global__ __launch_bounds__(256) void page_write_kernel(PagePlan a) {
   const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
-  compact_write(a, Marks<false>{a.marks}, blockIdx.x * 4 + wave, gridDim.x * 4);
+  compact_write(a, Marks{a.marks}, blockIdx.x * 4 + wave, gridDim.x * 4);
 }
 
 }  // namespace fa

@@ -49,13 +49,13 @@ struct PrefillArgs;
 
 // Chunks of new tokens over a paged cache (kernels_prefill.hip: D = 32, 64 or 128; mods: ALiBi or a soft-cap), rows
 // over a cache of latent vectors (kernels_latent.hip: L = 128, 256 or 512, R = 32 or 64; nb: 16-row blocks per
-// work item, 1, 2 or 4), appends to it, and pages (kernels_pages.hip; marks null: in LDS, at most kPlanLds of them)
+// work item, 1, 2 or 4), appends to it, and pages (kernels_pages.hip; marks null: the plan of one workgroup)
 template <int D>
 int launch_prefill(const PrefillArgs& a, bool fp8, bool mods, hipStream_t s);
 template <int L>
 int launch_latent(const LatentArgs& a, int R, int nb, hipStream_t s);
 int launch_latent_append(const LatentAppendArgs& a, hipStream_t s);
-constexpr int kCopyGrid = 2048, kPlanLds = 15 * 1024;
+constexpr int kCopyGrid = 2048;
 int launch_copy_pages(const CopyArgs& a, hipStream_t s);
 int launch_page_plan(const PagePlan& a, bool fork, hipStream_t s);
 int launch_saturate(const int64_t* x, int32_t* y, long long n, hipStream_t s);

@@ -23,6 +23,10 @@ struct CopyArgs {
 // or others keep it.
 constexpr int kPageHeld = -1, kPageUsed = 0, kPageFree = 0x7fffffff;
 
+// What one workgroup does in one launch: marks and rows in LDS, and no more table entries than it reads in
+// the time of the other form's launches.
+constexpr int kPlanPages = 24 * 1024, kPlanRows = 1024, kPlanEntries = 1 << 15;
+
 struct PagePlan {
   const int *table, *kv_lens;  // (B, max_pages), (B)
   const int* parents;          // (N) or null: row b goes on from row b

@@ -78,7 +78,7 @@ FA_HD TileSpan tile_span(int have, int ql, int i0, int i1, int left, int right) 
 
 // Ranges of keys that an item is cut into: workgroups for about `want` where there are fewer items, each at least
 // kPrefillLeast tiles of the longest row, at most kPrefillSplits.
-constexpr int kPrefillSplits = 32, kPrefillLeast = 2;
+constexpr int kPrefillSplits = 32, kPrefillLeast = 1;
 FA_HD int prefill_splits(long long items, int most_tiles, int want) {
   if (items >= want) return 1;
   long long n = want / items;

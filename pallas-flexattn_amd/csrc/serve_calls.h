@@ -240,10 +240,8 @@ struct PlanLayout {
   size_t marks, first, list, src, dst, moved, bytes;
   int pairs;
 };
-// What one workgroup does in one launch: marks in LDS, and no more table entries than it reads in the time that the
-// other form's launches take.
 bool small_plan(const fa_page_plan_call* c) {
-  return c->num_pages <= fa::kPlanLds && (long long)c->N * c->max_pages <= (1 << 15);
+  return c->num_pages <= fa::kPlanPages && c->N <= fa::kPlanRows && (long long)c->N * c->max_pages <= fa::kPlanEntries;
 }
 int plan_args(const fa_page_plan_call* c, bool fork, fa::PagePlan* a, PlanLayout* L) {
   if (!c) return FA_ERR_NULL;

@@ -900,37 +900,63 @@ PyObject* py_latent_decode(PyObject*, PyObject* const* a, Py_ssize_t n) {
   END_HANDLE_TH_ERRORS
 }
 
-// The tensors of a call on pages: dense, of as many pages each, on one device.
-bool paged_tensors(PyObject* list, std::vector<const at::Tensor*>* t, std::vector<fa_paged_tensor>* out) {
-  if (!PyList_Check(list) || PyList_GET_SIZE(list) < 1) {
-    PyErr_SetString(PyExc_TypeError, "expected a list of tensors");
+// The tensors of a call on pages: those of one cache or of a list of them, dense, of as many pages each, on one device.
+// (Here and not in Python: the 32 tensors of eight layers took 9 us there.)
+struct Paged {
+  std::vector<const at::Tensor*> t;
+  std::vector<fa_paged_tensor> p;
+  int64_t page_size = 0;
+
+  bool refuse(PyObject* type, const char* text) {
+    PyErr_SetString(type, text);
     return false;
   }
-  for (Py_ssize_t i = 0; i < PyList_GET_SIZE(list); ++i) {
-    const at::Tensor* x = tensor(PyList_GET_ITEM(list, i));
-    if (!x) return false;
-    const char* bad = nullptr;
-    if (x->dim() < 2 || x->numel() == 0 || !x->is_contiguous()) bad = "a cache's tensors must be dense (num_pages, ...)";
-    else if (x->size(0) > kMaxSize) bad = "sizes must be below 2^31";
-    else if (!t->empty() && x->size(0) != t->front()->size(0)) bad = "the caches must have as many pages each";
-    else if (!t->empty() && x->device() != t->front()->device()) bad = "the caches must be on one device";
-    if (bad) {
-      PyErr_SetString(PyExc_ValueError, bad);
-      return false;
+  bool add(const at::Tensor& x, int64_t dims, int at) {  // at: the dimension of the page size (0: none)
+    if (x.dim() != dims) return refuse(PyExc_ValueError, "key and value are (num_pages, Hkv, page_size, D), latent vectors (num_pages, page_size, dim)");
+    if (x.numel() == 0 || !x.is_contiguous()) return refuse(PyExc_ValueError, "a cache's tensors must be dense and not empty");
+    if (!sizes_fit(x)) return refuse(PyExc_ValueError, "sizes must be below 2^31");
+    if (!t.empty() && x.size(0) != t.front()->size(0)) return refuse(PyExc_ValueError, "the caches must have as many pages each");
+    if (!t.empty() && x.device() != t.front()->device()) return refuse(PyExc_ValueError, "the caches must be on one device");
+    if (at) {
+      if (page_size && x.size(at) != page_size) return refuse(PyExc_ValueError, "the caches must have one page size");
+      page_size = x.size(at);
     }
-    t->push_back(x);
-    out->push_back({const_cast<void*>(x->const_data_ptr()), x->numel() / x->size(0) * x->element_size()});
+    t.push_back(&x);
+    p.push_back({const_cast<void*>(x.const_data_ptr()), x.numel() / x.size(0) * x.element_size()});
+    return true;
   }
-  return true;
-}
+  static bool sequence(PyObject* x) { return PyTuple_Check(x) || PyList_Check(x); }
+  // (key, value), (key, value, key scale, value scale) or (latent data, its length)
+  bool cache(PyObject* c) {
+    const char* const text = "a cache is an Fp8KVCache, a LatentKVCache or a (key, value) pair of tensors";
+    if (!sequence(c)) return refuse(PyExc_TypeError, text);
+    const Py_ssize_t n = PySequence_Fast_GET_SIZE(c);
+    PyObject** x = PySequence_Fast_ITEMS(c);
+    if (n == 2 && THPVariable_Check(x[0]) && PyLong_Check(x[1])) return add(THPVariable_Unpack(x[0]), 3, 1);
+    if (n != 2 && n != 4) return refuse(PyExc_TypeError, text);
+    for (Py_ssize_t i = 0; i < n; ++i) {
+      if (!THPVariable_Check(x[i])) return refuse(PyExc_TypeError, text);
+      if (!add(THPVariable_Unpack(x[i]), i < 2 ? 4 : 3, i < 2 ? 2 : 0)) return false;
+    }
+    return true;
+  }
+  bool read(PyObject* caches) {
+    if (!sequence(caches) || PySequence_Fast_GET_SIZE(caches) < 1)
+      return refuse(PyExc_TypeError, "caches must be a cache or a list of caches");
+    PyObject** x = PySequence_Fast_ITEMS(caches);
+    if (THPVariable_Check(x[0])) return cache(caches);
+    for (Py_ssize_t i = 0; i < PySequence_Fast_GET_SIZE(caches); ++i)
+      if (!cache(x[i])) return false;
+    return true;
+  }
+};
 
-// copy_pages(tensors, src, dst) -> status
+// copy_pages(caches, src, dst) -> status
 PyObject* py_copy_pages(PyObject*, PyObject* const* a, Py_ssize_t n) {
   HANDLE_TH_ERRORS
   if (n != 3 || !g_copy_pages) REFUSE(PyExc_TypeError, "copy_pages takes 3 arguments, after bind_serve");
-  std::vector<const at::Tensor*> t;
-  std::vector<fa_paged_tensor> p;
-  if (!paged_tensors(a[0], &t, &p)) return nullptr;
+  Paged c;
+  if (!c.read(a[0])) return nullptr;
   const at::Tensor *src = tensor(a[1]), *dst;
   if (!src || !(dst = tensor(a[2]))) return nullptr;
   for (const at::Tensor* x : {src, dst}) {
@@ -938,33 +964,33 @@ PyObject* py_copy_pages(PyObject*, PyObject* const* a, Py_ssize_t n) {
     if (x->dim() != 1 || x->size(0) != src->size(0) || x->size(0) > kMaxSize)
       REFUSE(PyExc_ValueError, "src and dst must be vectors of one length");
   }
-  const at::Device dev = t[0]->device();
+  const at::Device dev = c.t[0]->device();
   if (!dev.is_cuda()) REFUSE(PyExc_ValueError, "the caches must be on the GPU");
   int rc = FA_OK;
   if (src->size(0)) {
     const c10::DeviceGuard guard(dev);
     const at::Tensor s = row_ints(*src, dev), d = row_ints(*dst, dev);
-    rc = g_copy_pages(p.data(), static_cast<int32_t>(p.size()), static_cast<int32_t>(t[0]->size(0)), s.const_data_ptr<int32_t>(),
-                      d.const_data_ptr<int32_t>(), static_cast<int32_t>(s.size(0)), stream_of(dev));
+    rc = g_copy_pages(c.p.data(), static_cast<int32_t>(c.p.size()), static_cast<int32_t>(c.t[0]->size(0)),
+                      s.const_data_ptr<int32_t>(), d.const_data_ptr<int32_t>(), static_cast<int32_t>(s.size(0)), stream_of(dev));
     if (rc == FA_OK)
-      for (const at::Tensor* x : t) written(*x);
+      for (const at::Tensor* x : c.t) written(*x);
   }
   return PyLong_FromLong(rc);
   END_HANDLE_TH_ERRORS
 }
 
-// page_plan(fork, tensors, page_size, table, kv_lens, parents | None, room | None, room_all, keep | None)
+// page_plan(fork, caches, table, kv_lens, parents | None, room | None, room_all, keep | None)
 //   -> (status, table', lens' | None, count)
 PyObject* py_page_plan(PyObject*, PyObject* const* a, Py_ssize_t n) {
   HANDLE_TH_ERRORS
-  if (n != 9 || !g_fork) REFUSE(PyExc_TypeError, "page_plan takes 9 arguments, after bind_serve");
+  if (n != 8 || !g_fork) REFUSE(PyExc_TypeError, "page_plan takes 8 arguments, after bind_serve");
   const bool fork = PyObject_IsTrue(a[0]);
-  std::vector<const at::Tensor*> t;
-  std::vector<fa_paged_tensor> p;
-  if (!paged_tensors(a[1], &t, &p)) return nullptr;
-  const int64_t page_size = PyLong_AsLong(a[2]), room_all = PyLong_AsLong(a[7]);
-  const at::Tensor *table = tensor(a[3]), *lens, *parents, *room, *keep;
-  if (!table || !(lens = tensor(a[4])) || !optional(a[5], &parents) || !optional(a[6], &room) || !optional(a[8], &keep)) return nullptr;
+  Paged k;
+  if (!k.read(a[1])) return nullptr;
+  const std::vector<const at::Tensor*>& t = k.t;
+  const int64_t page_size = k.page_size, room_all = PyLong_AsLong(a[6]);
+  const at::Tensor *table = tensor(a[2]), *lens, *parents, *room, *keep;
+  if (!table || !(lens = tensor(a[3])) || !optional(a[4], &parents) || !optional(a[5], &room) || !optional(a[7], &keep)) return nullptr;
   if (PyErr_Occurred()) return nullptr;
   const int64_t pages = t[0]->size(0);
   if (table->scalar_type() != at::kInt && table->scalar_type() != at::kLong)
@@ -980,7 +1006,7 @@ PyObject* py_page_plan(PyObject*, PyObject* const* a, Py_ssize_t n) {
   if (room_all < 0 || room_all > kMaxSize) REFUSE(PyExc_ValueError, "room must not be negative, and below 2^31");
   if (keep && keep->scalar_type() != at::kBool) REFUSE(PyExc_TypeError, "keep must be a bool tensor");
   if (keep && (keep->dim() != 1 || keep->size(0) != pages)) REFUSE(PyExc_ValueError, "keep must have one entry per page");
-  if (!sizes_fit(*table) || N > kMaxSize || page_size > kMaxSize) REFUSE(PyExc_ValueError, "sizes must be below 2^31");
+  if (!sizes_fit(*table) || N > kMaxSize) REFUSE(PyExc_ValueError, "sizes must be below 2^31");
   const at::Device dev = t[0]->device();
   if (!dev.is_cuda()) REFUSE(PyExc_ValueError, "the caches must be on the GPU");
   if (keep && keep->device() != dev) REFUSE(PyExc_ValueError, "keep must be on the caches' device");
@@ -1005,8 +1031,8 @@ PyObject* py_page_plan(PyObject*, PyObject* const* a, Py_ssize_t n) {
   c.out_table = out.mutable_data_ptr<int32_t>();
   c.out_count = count.mutable_data_ptr<int32_t>();
   if (fork) c.out_lens = (olens = at::empty({N}, ints)).mutable_data_ptr<int32_t>();
-  c.tensors = p.data();
-  c.tensor_count = static_cast<int32_t>(p.size());
+  c.tensors = k.p.data();
+  c.tensor_count = static_cast<int32_t>(k.p.size());
   const size_t bytes = (fork ? g_fork_ws : g_compact_ws)(&c);
   at::Tensor ws = at::empty({static_cast<int64_t>(std::max<size_t>(bytes, 16))}, ints.dtype(at::kByte));
   const int rc = (fork ? g_fork : g_compact)(&c, ws.mutable_data_ptr(), bytes, stream_of(dev));

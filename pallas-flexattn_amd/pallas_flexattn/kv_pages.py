@@ -11,50 +11,25 @@ Page ids, tables and lengths are int32 (read as they are) or int64; what comes b
 """
 from . import _lib
 from .flash_attn import _torch
-from .kv_cache import Fp8KVCache, _rows
-from .latent import LatentKVCache
 
 
-def _tensors(caches):
-    """The tensors of a cache or of several, and their page size."""
-    if isinstance(caches, (Fp8KVCache, LatentKVCache)) or (isinstance(caches, tuple) and len(caches) == 2 and
-                                                            all(hasattr(x, "data_ptr") for x in caches)):
-        caches = [caches]
-    if not isinstance(caches, (list, tuple)) or not caches:
-        raise TypeError("caches must be a cache or a list of caches")
-    out, pages = [], set()
-    for c in caches:
-        if isinstance(c, LatentKVCache):
-            parts, dim, at = (c.data,), 3, 1
-        elif isinstance(c, Fp8KVCache) or (isinstance(c, (list, tuple)) and len(c) == 2):
-            parts, dim, at = tuple(c), 4, 2
-        else:
-            raise TypeError("a cache is an Fp8KVCache, a LatentKVCache or a (key, value) pair of tensors")
-        for i, x in enumerate(parts):
-            if not hasattr(x, "data_ptr"):
-                raise TypeError("a cache is made of tensors")
-            if x.dim() != (3 if i > 1 else dim):
-                raise ValueError("key and value are (num_pages, Hkv, page_size, D), latent vectors (num_pages, page_size, dim)")
-            if i < 2:
-                pages.add(x.shape[at])
-        out += parts
-    if len(pages) != 1:
-        raise ValueError("the caches must have one page size")
-    return out, pages.pop()
+def _ints(x, caches):
+    """Whole numbers as a tensor (a list or array is copied to the caches' device)."""
+    if x is None or hasattr(x, "data_ptr"):
+        return x
+    c = caches
+    while isinstance(c, (list, tuple)) and c:
+        c = c[0]
+    return _torch().as_tensor(x, device=getattr(c, "device", None))
 
 
 def copy_kv_pages(caches, src, dst) -> None:
     """Copies page ``src[i]`` to page ``dst[i]`` in every cache, in place (``src``, ``dst``: vectors of page ids on the
     GPU).  Pairs with an id outside the cache are left out, so a vector may be padded with -1.  The pages ``dst``
     must be distinct, and none of them among ``src``."""
-    tensors, _ = _tensors(caches)
-    rc = _lib.launcher().copy_pages(tensors, _rows(src, tensors[0]), _rows(dst, tensors[0]))
+    rc = _lib.launcher().copy_pages(caches, _ints(src, caches), _ints(dst, caches))
     if rc:
         _lib.check(rc)
-
-
-def _room(room, like):
-    return (None, room) if isinstance(room, int) else (_rows(room, like), 0)
 
 
 def fork_kv_rows(caches, page_table, kv_lens, parents=None, room=0, keep=None):
@@ -71,10 +46,9 @@ def fork_kv_rows(caches, page_table, kv_lens, parents=None, room=0, keep=None):
     hold.  ``free`` (int32, on the GPU) is how many are left; where it is negative so many were lacking, and
     the entries that lack one are -1 (tokens of a copy that could not be made are lost: look before going on).
     Page ids outside the cache stay as they are."""
-    tensors, page_size = _tensors(caches)
-    per_row, number = _room(room, tensors[0])
-    rc, table, lens, free = _lib.launcher().page_plan(True, tensors, page_size, page_table, _rows(kv_lens, tensors[0]),
-                                                      _rows(parents, tensors[0]), per_row, number, keep)
+    per_row, number = (None, room) if isinstance(room, int) else (_ints(room, caches), 0)
+    rc, table, lens, free = _lib.launcher().page_plan(True, caches, page_table, _ints(kv_lens, caches), _ints(parents, caches),
+                                                      per_row, number, keep)
     if rc:
         _lib.check(rc)
     return table, lens, free
@@ -85,9 +59,7 @@ def compact_kv_pages(caches, page_table, kv_lens, room: int = 0, keep=None):
     fill, or ``keep`` holds), those with ids from n on that ``keep`` does not hold move, in every cache, to the
     free ids below n, both in ascending order.  ``used`` (int32, on the GPU) is n; pages that ``keep`` holds stay where they
     are.  Entries past a row's tokens and room are -1, page ids outside the cache stay as they are."""
-    tensors, page_size = _tensors(caches)
-    rc, table, _, used = _lib.launcher().page_plan(False, tensors, page_size, page_table, _rows(kv_lens, tensors[0]), None,
-                                                   None, room, keep)
+    rc, table, _, used = _lib.launcher().page_plan(False, caches, page_table, _ints(kv_lens, caches), None, None, room, keep)
     if rc:
         _lib.check(rc)
     return table, used
