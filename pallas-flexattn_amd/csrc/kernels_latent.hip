@@ -23,7 +23,10 @@ int launch_latent<FA_KERNELS_L>(const LatentArgs& a, int R, int nb, hipStream_t 
   const int rc = launch_status();
   if (rc || a.d.by_item) return rc;
   const long long units = (long long)a.d.B * a.d.g * a.d.Sq * (L >= 256 ? L / 256 : 1);
-  hipLaunchKernelGGL((latent_merge<L>), dim3((unsigned)((units + 3) / 4)), dim3(256), 0, s, a.d, a.rt, 16 * nb);
+  if (units <= kMergeWide / 64)
+    hipLaunchKernelGGL((latent_merge<L, 4>), dim3((unsigned)units), dim3(256), 0, s, a.d, a.rt, 16 * nb);
+  else
+    hipLaunchKernelGGL((latent_merge<L, 1>), dim3((unsigned)((units + 3) / 4)), dim3(256), 0, s, a.d, a.rt, 16 * nb);
   return launch_status();
 }
 

@@ -20,7 +20,11 @@ int launch_prefill<FA_KERNELS_D>(const PrefillArgs& a, bool fp8, bool mods, hipS
   const int rc = launch_status();
   if (rc || a.n_splits == 1) return rc;
   const long long rows = (long long)(a.starts ? 1 : a.B) * a.Hq * a.Sq;
-  hipLaunchKernelGGL((prefill_merge<D>), dim3((unsigned)((rows * (D / 4) + 255) / 256)), dim3(256), 0, s, a, rows);
+  const long long threads = rows * (D / 4);
+  if (a.n_splits > 4 && threads <= kMergeWide)
+    hipLaunchKernelGGL((prefill_merge<D, 4>), dim3((unsigned)((threads + 63) / 64)), dim3(256), 0, s, a, rows);
+  else
+    hipLaunchKernelGGL((prefill_merge<D, 1>), dim3((unsigned)((threads + 255) / 256)), dim3(256), 0, s, a, rows);
   return launch_status();
 }
 

@@ -454,14 +454,15 @@ void latent_decode_kernel(LatentArgs a) {
 }
 
 // Items that several workgroups shared: M = max m, L = sum l 2^(m - M), O = sum O 2^(m - M) / L.  A wave per output
-// row and 64 C of its elements; lane s of 64 holds piece s's factor.
-template <int L>
+// row and 64 C of its elements, of which lane s of 64 holds piece s's factor; kWaves waves take every kWaves-th piece
+// of the same elements where few rows would leave one wave's loads one behind another.
+template <int L, int kWaves>
 __global__ __launch_bounds__(256) void latent_merge(DecodeArgs a, int rt, int rows_per) {
   constexpr int C = L >= 256 ? 4 : 2, DEEP = 8, PARTS = L / (64 * C);
   typedef float vec __attribute__((ext_vector_type(C)));
-  const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
+  const int lane = threadIdx.x & 63, w4 = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6), w = kWaves == 1 ? 0 : w4;
   const int RT = a.g * a.Sq;
-  const long long unit = (long long)blockIdx.x * 4 + w;
+  const long long unit = kWaves == 1 ? (long long)blockIdx.x * 4 + w4 : blockIdx.x;
   const long long orow = unit / PARTS;
   if (orow >= (long long)a.B * RT) return;
   const int b = (int)(orow / RT), row = (int)(orow - (long long)b * RT);
@@ -480,9 +481,9 @@ __global__ __launch_bounds__(256) void latent_merge(DecodeArgs a, int rt, int ro
     vec y[DEEP];
     auto load = [&](int i0) {
 #pragma unroll
-      for (int i = 0; i < DEEP; ++i) y[i] = *reinterpret_cast<const vec*>(a.part + at(p0 + min(i0 + i, np - 1)) * L + col);
+      for (int i = 0; i < DEEP; ++i) y[i] = *reinterpret_cast<const vec*>(a.part + at(p0 + min(i0 + kWaves * i, np - 1)) * L + col);
     };
-    load(0);  // ahead of the factors
+    load(w);  // ahead of the factors
     float mx = ml.x;
 #pragma unroll
     for (int d = 32; d >= 1; d >>= 1) mx = fmaxf(mx, __shfl_xor(mx, d));
@@ -494,16 +495,24 @@ __global__ __launch_bounds__(256) void latent_merge(DecodeArgs a, int rt, int ro
     S = S * old + ls;
     M = mnew;
     acc *= old;
-    for (int i0 = 0; i0 < np; i0 += DEEP) {
-      if (i0) load(i0);
+    for (int i0 = w; i0 < np; i0 += kWaves * DEEP) {
+      if (i0 != w) load(i0);
 #pragma unroll
       for (int i = 0; i < DEEP; ++i) {
-        const float ci = __shfl(c, (i0 + i) & 63);
-        const bool there = i0 + i < np && !(ci == 0.f);
+        const float ci = __shfl(c, (i0 + kWaves * i) & 63);
+        const bool there = i0 + kWaves * i < np && !(ci == 0.f);
 #pragma unroll
         for (int k = 0; k < C; ++k) acc[k] = there ? fmaf(y[i][k], ci, acc[k]) : acc[k];
       }
     }
+  }
+  if constexpr (kWaves > 1) {
+    __shared__ vec sum[kWaves][64];
+    sum[w][lane] = acc;
+    __syncthreads();
+    if (w) return;
+#pragma unroll
+    for (int i = 1; i < kWaves; ++i) acc += sum[i][lane];
   }
   const float inv = S == 0.f ? 0.f : 1.0f / S;
   uint32_t* o = reinterpret_cast<uint32_t*>(static_cast<uint16_t*>(a.o) + (size_t)orow * L + col);

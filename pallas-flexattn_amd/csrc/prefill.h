@@ -67,15 +67,27 @@ __device__ __forceinline__ PrefillItem prefill_item(const PrefillArgs& a, int re
   return it;
 }
 
-// tanh of a lane's 16 values (tanh8's choice of form)
+// tanh of a lane's 16 values, in the form that the wave's values allow (tanh8): here also a shorter polynomial below kTanhTiny
+// (minimax in x^2 too, within 1.7 2^-24 of the value), where a soft-cap well above the scores leaves them.
+constexpr float kTanhTiny = 0.35f;
+__device__ __forceinline__ float tanh_tiny(float x) {
+  const float y = x * x;
+  float p = fmaf(-0.04914850369095802f, y, 0.1329982578754425f);
+  p = fmaf(p, y, -0.33332663774490356f);
+  return fmaf(x * y, p, x);
+}
 __device__ __forceinline__ void tanh16(f32x16& x) {
-  float lo = INFINITY, hi = 0.f;
+  float hi = 0.f;
 #pragma unroll
-  for (int e = 0; e < 16; ++e) {
-    const float t = fabsf(x[e]);
-    lo = fminf(lo, t);
-    hi = fmaxf(hi, t);
+  for (int e = 0; e < 16; e += 2) hi = fmaxf(fmaxf(hi, fabsf(x[e])), fabsf(x[e + 1]));
+  if (!__any(hi >= kTanhTiny)) {
+#pragma unroll
+    for (int e = 0; e < 16; ++e) x[e] = tanh_tiny(x[e]);
+    return;
   }
+  float lo = INFINITY;
+#pragma unroll
+  for (int e = 0; e < 16; e += 2) lo = fminf(fminf(lo, fabsf(x[e])), fabsf(x[e + 1]));
   if (!__any(hi >= kTanhSmall)) {
 #pragma unroll
     for (int e = 0; e < 16; ++e) x[e] = tanh_small(x[e]);
@@ -858,49 +870,72 @@ __global__ __launch_bounds__(256, D == 128 ? 2 : 3) void prefill_kernel(PrefillA
 }
 
 // The splits of a row: M = max m_s, L = sum l_s 2^(m_s - M), O = sum O_s 2^(m_s - M) / L.  Four columns a thread, D / 4
-// threads a row, so that a wave has several rows under way; the factors come from the cache twice.
-template <int D>
+// threads a row, of which thread j holds split j's factor (and j + D / 4's, ..); kWaves waves take every kWaves-th split of the same
+// rows where few rows would leave one wave's loads one behind another.
+template <int D, int kWaves>
 __global__ __launch_bounds__(256) void prefill_merge(PrefillArgs a, long long rows) {
-  constexpr int TPR = D / 4, DEEP = 4;
-  const long long row = ((long long)blockIdx.x * 256 + threadIdx.x) / TPR;
-  if (row >= rows) return;
-  const int n = a.n_splits, col = 4 * (threadIdx.x % TPR);
-  const float2* ml = reinterpret_cast<const float2*>(a.part + (size_t)n * rows * D) + row;
-  const float* part = a.part + (size_t)row * D + col;
+  constexpr int TPR = D / 4, DEEP = 4, HELD = kPrefillSplits / TPR < 1 ? 1 : kPrefillSplits / TPR;
+  const int lane = threadIdx.x & 63, w = kWaves == 1 ? 0 : (int)threadIdx.x >> 6, j = lane % TPR;
+  const long long row = ((long long)blockIdx.x * (256 / kWaves) + (kWaves == 1 ? (int)threadIdx.x : lane)) / TPR;
+  const bool there = row < rows;
+  const long long r = there ? row : rows - 1;
+  const int n = a.n_splits, col = 4 * j;
+  const float2* ml = reinterpret_cast<const float2*>(a.part + (size_t)n * rows * D) + r;
+  const float* part = a.part + (size_t)r * D + col;
+  float2 x[HELD];
+  f32x4 y[DEEP];
+  auto load = [&](int s0) {
+#pragma unroll
+    for (int u = 0; u < DEEP; ++u) y[u] = *reinterpret_cast<const f32x4*>(part + (size_t)imin(s0 + kWaves * u, n - 1) * rows * D);
+  };
+#pragma unroll
+  for (int u = 0; u < HELD; ++u) x[u] = ml[(size_t)imin(j + TPR * u, n - 1) * rows];
+  load(w);  // ahead of the factors
   float M = -INFINITY;
-  for (int s0 = 0; s0 < n; s0 += 8) {
-    float x[8];
 #pragma unroll
-    for (int u = 0; u < 8; ++u) x[u] = ml[(size_t)imin(s0 + u, n - 1) * rows].x;
+  for (int u = 0; u < HELD; ++u) M = fmaxf(M, x[u].x);
 #pragma unroll
-    for (int u = 0; u < 8; ++u) M = fmaxf(M, x[u]);
+  for (int d = TPR / 2; d >= 1; d >>= 1) M = fmaxf(M, __shfl_xor(M, d));
+  float c[HELD], L = 0.f;
+#pragma unroll
+  for (int u = 0; u < HELD; ++u) {
+    const bool mine = j + TPR * u < n && x[u].x != -INFINITY;  // (a split without a visible key has no O)
+    c[u] = mine ? fast_exp2(x[u].x - M) : -1.f;
+    L += mine ? x[u].y * c[u] : 0.f;
   }
+#pragma unroll
+  for (int d = TPR / 2; d >= 1; d >>= 1) L += __shfl_xor(L, d);
   f32x4 acc = {0.f, 0.f, 0.f, 0.f};
-  float L = 0.f;
-  for (int s0 = 0; s0 < n; s0 += DEEP) {
-    float2 x[DEEP];
-    f32x4 y[DEEP];
+  for (int s0 = w; s0 < n; s0 += kWaves * DEEP) {
+    if (s0 != w) load(s0);
 #pragma unroll
     for (int u = 0; u < DEEP; ++u) {
-      const size_t s = imin(s0 + u, n - 1);
-      x[u] = ml[s * rows];
-      y[u] = *reinterpret_cast<const f32x4*>(part + s * rows * D);
-    }
+      const int s = s0 + kWaves * u;
+      float f = -1.f;
 #pragma unroll
-    for (int u = 0; u < DEEP; ++u) {
-      const bool there = s0 + u < n && x[u].x != -INFINITY;  // (a split without a visible key has no O)
-      const float c = there ? fast_exp2(x[u].x - M) : 0.f;
-      L = there ? fmaf(x[u].y, c, L) : L;
+      for (int h = 0; h < HELD; ++h) f = s / TPR == h ? __shfl(c[h], (lane & ~(TPR - 1)) + s % TPR) : f;
+      const bool has = s < n && f >= 0.f;
 #pragma unroll
-      for (int k = 0; k < 4; ++k) acc[k] = there ? fmaf(y[u][k], c, acc[k]) : acc[k];
+      for (int k = 0; k < 4; ++k) acc[k] = has ? fmaf(y[u][k], f, acc[k]) : acc[k];
     }
   }
+  if constexpr (kWaves > 1) {
+    __shared__ f32x4 sum[kWaves][64];
+    sum[w][lane] = acc;
+    __syncthreads();
+    if (w) return;
+#pragma unroll
+    for (int i = 1; i < kWaves; ++i)
+#pragma unroll
+      for (int k = 0; k < 4; ++k) acc[k] += sum[i][lane][k];
+  }
+  if (!there) return;
   const float inv = L == 0.f ? 0.f : 1.0f / L;  // (NaN is passed on)
   const long long tok = row % a.Sq, bh = row / a.Sq;
   uint16_t* o = static_cast<uint16_t*>(a.o) + (bh / a.Hq) * a.osb + (bh % a.Hq) * a.osh + tok * a.ost + col;
   *reinterpret_cast<u32x2*>(o) =
       L == 0.f ? u32x2{0u, 0u} : u32x2{pack_bf16x2(acc[0] * inv, acc[1] * inv), pack_bf16x2(acc[2] * inv, acc[3] * inv)};
-  if (col == 0) a.lse[row] = L == 0.f ? -INFINITY : (M + log2f(L)) * kLn2;
+  if (j == 0) a.lse[row] = L == 0.f ? -INFINITY : (M + log2f(L)) * kLn2;
 }
 
 }  // namespace fa
