@@ -7,7 +7,7 @@ namespace fa {
 
 template <int D, bool kFp8, bool kMods>
 static void run_prefill(const PrefillArgs& a, hipStream_t s) {
-  const dim3 grid(a.n_splits * a.tiles * a.Hkv);
+  const dim3 grid((unsigned)prefill_grid(a));
   if (a.starts) hipLaunchKernelGGL((prefill_kernel<D, kFp8, kMods, true>), grid, dim3(256), 0, s, a);
   else hipLaunchKernelGGL((prefill_kernel<D, kFp8, kMods, false>), grid, dim3(256), 0, s, a);
 }

@@ -299,6 +299,15 @@ __device__ __forceinline__ float2 split_ml(float m, float l, bool live) {
   return !live ? make_float2(-INFINITY, 0.f) : l == l ? make_float2(m, l) : make_float2(0.f, l);
 }
 
+// Row `row` of all `rows` in the join's list of maxima and sums, for the range that x is.  (An item with fewer ranges than others
+// says so: one range, whose results are written already, by a negative sum; else by an empty range at the end.)
+__device__ __forceinline__ void note_ml(const PrefillArgs& a, const PrefillRange& x, int D, size_t rows, size_t row, float2 ml) {
+  if (a.n_splits == 1) return;
+  float2* list = reinterpret_cast<float2*>(a.part + (size_t)a.n_splits * rows * D) + row;
+  list[x.split * rows] = x.ranges > 1 ? ml : make_float2(0.f, -1.f);
+  if (x.split == 0 && x.ranges > 1 && x.ranges < a.n_splits) list[x.ranges * rows] = make_float2(-INFINITY, 0.f);
+}
+
 // Where keys lie: lane i holds, for the keys first + step i .. of a batch row, their run (-1: none, or a bad page) and its scales.
 template <bool kFp8>
 struct RunTable {
@@ -327,7 +336,7 @@ struct RunTable {
 // Items of at most 32 rows (the single tokens of a mixed batch, short chunks): bound by the reads of the cache, so each wave walks
 // every fourth 32-key tile by itself, in a quarter of the LDS, without barriers; the waves join at the end.
 template <int D, bool kFp8, bool kMods, bool kPacked>
-__device__ __forceinline__ void prefill_thin(const PrefillArgs& a, const PrefillItem& it, int hk, int split, TileSpan ts, char* lds) {
+__device__ __forceinline__ void prefill_thin(const PrefillArgs& a, const PrefillItem& it, int hk, const PrefillRange& x0, TileSpan ts, char* lds) {
   using W = PrefillWave<D, kFp8, kMods, kPacked>;
   using frag = typename W::frag;
   constexpr int RB = W::RB, KCH = W::KCH, DT = W::DT, KSTEPS = W::KSTEPS, TB = 32 * RB;
@@ -503,17 +512,15 @@ __device__ __forceinline__ void prefill_thin(const PrefillArgs& a, const Prefill
     }
   }
   const int rows = it.nq * a.g;
+  const size_t all = (size_t)(kPacked ? 1 : a.B) * a.Hq * a.Sq;
   const auto me = W::row(a, it, it.row0 + orow);
   if (me.valid) {
     const size_t at = ((size_t)(kPacked ? 0 : it.b) * a.Hq + hk * a.g + me.hq) * a.Sq + it.tok + me.qi;
-    if (a.n_splits > 1) {
-      const size_t all = (size_t)(kPacked ? 1 : a.B) * a.Hq * a.Sq;
-      float* po = a.part + ((size_t)split * all + at) * D + col;
+    if (col == 0) note_ml(a, x0, D, all, at, split_ml(M, L, me.live));
+    if (x0.ranges > 1) {
+      float* po = a.part + ((size_t)x0.split * all + at) * D + col;
 #pragma unroll
       for (int k = 0; k < CW / 4; ++k) *reinterpret_cast<f32x4*>(po + 4 * k) = o[k];
-      if (col == 0)
-        *reinterpret_cast<float2*>(a.part + (size_t)a.n_splits * all * D + ((size_t)split * all + at) * 2) =
-            split_ml(M, L, me.live);
     } else {
       const bool none = !me.live || L == 0.f;  // (NaN is passed on)
       const float inv = none ? 0.f : 1.0f / L;
@@ -532,11 +539,8 @@ __device__ __forceinline__ void prefill_thin(const PrefillArgs& a, const Prefill
   for (int z = 32 + orow; z < left; z += 32) {
     const auto pad = W::row(a, it, it.row0 + z);
     const size_t at = ((size_t)(kPacked ? 0 : it.b) * a.Hq + hk * a.g + pad.hq) * a.Sq + it.tok + pad.qi;
-    if (a.n_splits > 1) {
-      const size_t all = (size_t)(kPacked ? 1 : a.B) * a.Hq * a.Sq;
-      if (col == 0)
-        *reinterpret_cast<float2*>(a.part + (size_t)a.n_splits * all * D + ((size_t)split * all + at) * 2) = make_float2(-INFINITY, 0.f);
-    } else {
+    if (col == 0) note_ml(a, x0, D, all, at, make_float2(-INFINITY, 0.f));
+    if (x0.ranges == 1) {
       uint16_t* po = static_cast<uint16_t*>(a.o) + (kPacked ? 0 : it.b) * a.osb + (hk * a.g + pad.hq) * a.osh +
                      (long long)(it.tok + pad.qi) * a.ost + col;
 #pragma unroll
@@ -562,22 +566,20 @@ __global__ __launch_bounds__(256, D == 128 ? 2 : 3) void prefill_kernel(PrefillA
 
   const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int lr = lane & 31, hh = lane >> 5;
-  const int items = a.tiles * a.Hkv;
-  const int split = a.n_splits > 1 ? (int)blockIdx.x / items : 0;
-  const int item = (int)blockIdx.x - split * items;
+  const PrefillRange range = prefill_range(a, blockIdx.x);
   // (kv heads fastest: with eight of them each XCD's L2 holds one head's keys)
-  const int rest = item / a.Hkv, hk = item - rest * a.Hkv;
+  const int rest = range.item / a.Hkv, hk = range.item - rest * a.Hkv;
   const PrefillItem it = prefill_item<kPacked>(a, rest);
   if (kPacked && it.b < 0) return;
   const int have = it.have, rows = it.nq * a.g;
   const int i_first = it.row0 / a.g, i_last = imin((it.row0 + kPrefillRows - 1) / a.g, it.ql - 1);
   TileSpan ts = tile_span(have, it.ql, i_first, i_last, a.win_left, a.win_right);
-  if (a.n_splits > 1) {
-    const SplitRange sr = split_range(ts.t1 - ts.t0, split, a.n_splits, 0);
+  if (range.ranges > 1) {
+    const SplitRange sr = split_range(ts.t1 - ts.t0, range.split, range.ranges, 0);
     ts = TileSpan{ts.t0 + sr.it0, ts.t0 + sr.it1};
   }
   if (it.ql * a.g - it.row0 <= 32) {
-    prefill_thin<D, kFp8, kMods, kPacked>(a, it, hk, split, ts, lds);
+    prefill_thin<D, kFp8, kMods, kPacked>(a, it, hk, range, ts, lds);
     return;
   }
   W x;
@@ -823,10 +825,11 @@ __global__ __launch_bounds__(256, D == 128 ? 2 : 3) void prefill_kernel(PrefillA
   const auto me = W::row(a, it, it.row0 + 32 * w + lr);
   // row of lse (and of the partial results)
   const size_t at = ((size_t)(kPacked ? 0 : it.b) * a.Hq + hk * a.g + me.hq) * a.Sq + it.tok + me.qi;
-  if (a.n_splits > 1) {
-    const size_t all = (size_t)(kPacked ? 1 : a.B) * a.Hq * a.Sq;
+  const size_t all = (size_t)(kPacked ? 1 : a.B) * a.Hq * a.Sq;
+  if (me.valid && hh == 0) note_ml(a, range, D, all, at, split_ml(x.m, lt, me.live));
+  if (range.ranges > 1) {
     if (me.valid) {
-      float* po = a.part + ((size_t)split * all + at) * D;
+      float* po = a.part + ((size_t)range.split * all + at) * D;
       if (ts.t0 < ts.t1 && me.live) {  // (else m = -inf says that there is no O)
 #pragma unroll
         for (int i = 0; i < DT; ++i)
@@ -835,9 +838,6 @@ __global__ __launch_bounds__(256, D == 128 ? 2 : 3) void prefill_kernel(PrefillA
             *reinterpret_cast<f32x4*>(po + 32 * i + 8 * j + 4 * hh) =
                 f32x4{x.oacc[i][4 * j], x.oacc[i][4 * j + 1], x.oacc[i][4 * j + 2], x.oacc[i][4 * j + 3]};
       }
-      if (hh == 0)
-        *reinterpret_cast<float2*>(a.part + (size_t)a.n_splits * all * D + ((size_t)split * all + at) * 2) =
-            split_ml(x.m, lt, me.live);
     }
     return;
   }
@@ -891,6 +891,7 @@ __global__ __launch_bounds__(256) void prefill_merge(PrefillArgs a, long long ro
 #pragma unroll
   for (int u = 0; u < HELD; ++u) x[u] = ml[(size_t)imin(j + TPR * u, n - 1) * rows];
   load(w);  // ahead of the factors
+  const bool whole = __shfl(x[0].y, lane & ~(TPR - 1)) < 0.f;  // (its one range has written it)
   float M = -INFINITY;
 #pragma unroll
   for (int u = 0; u < HELD; ++u) M = fmaxf(M, x[u].x);
@@ -929,7 +930,7 @@ __global__ __launch_bounds__(256) void prefill_merge(PrefillArgs a, long long ro
 #pragma unroll
       for (int k = 0; k < 4; ++k) acc[k] += sum[i][lane][k];
   }
-  if (!there) return;
+  if (!there || whole) return;
   const float inv = L == 0.f ? 0.f : 1.0f / L;  // (NaN is passed on)
   const long long tok = row % a.Sq, bh = row / a.Sq;
   uint16_t* o = static_cast<uint16_t*>(a.o) + (bh / a.Hq) * a.osb + (bh % a.Hq) * a.osh + tok * a.ost + col;

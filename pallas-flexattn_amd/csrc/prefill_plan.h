@@ -25,7 +25,8 @@ struct PrefillArgs {
   float scale, scale_log2, softcap;
   const float* alibi;
   int tiles;                // row tiles (of each kv head)
-  int n_splits;
+  int n_splits;             // most ranges that an item's keys are cut into;
+  int few;                  // the first so many items have one less
   float* part;              // n_splits > 1: (n_splits, rows, D), then (m, l) (n_splits, rows, 2); rows as lse's
 };
 
@@ -80,16 +81,33 @@ FA_HD TileSpan tile_span(int have, int ql, int i0, int i1, int left, int right) 
 // row in 63 pieces takes 3 us less, of 608 rows of 9 splits 0.7 us; of 1536 latent rows in 6 pieces 2.9 us more.
 constexpr long long kMergeWide = 1 << 17;
 
-// Ranges of keys that an item is cut into: workgroups for about `want` where there are fewer items, each at least
-// kPrefillLeast tiles of the longest row, at most kPrefillSplits.
+// Ranges of keys that an item is cut into where there are fewer items than `want`, the workgroups that run at a time: each at least
+// kPrefillLeast tiles of the longest row, at most kPrefillSplits.  If the items are `even`, the last of them get one range more, so
+// that `want` workgroups come out: 375 of 512 in one range each leave half the compute units with one workgroup and
+// half with two (8192 keys, D = 128: 237 us, 257 whole, 245 all in two).
 constexpr int kPrefillSplits = 32, kPrefillLeast = 1;
-FA_HD int prefill_splits(long long items, int most_tiles, int want) {
-  if (items >= want) return 1;
-  long long n = want / items;
-  const int most = most_tiles / kPrefillLeast;
-  if (n > most) n = most;
-  if (n > kPrefillSplits) n = kPrefillSplits;
-  return n < 1 ? 1 : (int)n;
+struct PrefillCut {
+  int n, few;  // ranges; the first `few` items have one less
+};
+FA_HD PrefillCut prefill_cut(long long items, int most_tiles, int want, bool even) {
+  if (items >= want) return PrefillCut{1, 0};
+  const int most = most_tiles / kPrefillLeast < kPrefillSplits ? most_tiles / kPrefillLeast : kPrefillSplits;
+  const long long n = want / items;
+  if (n >= most) return PrefillCut{most < 1 ? 1 : most, 0};
+  if (!even || items * n == want) return PrefillCut{(int)n, 0};
+  return PrefillCut{(int)n + 1, (int)(items * (n + 1) - want)};
+}
+// Workgroups of the call, and what workgroup x does: range `split` of the item's `ranges`.
+FA_HD long long prefill_grid(const PrefillArgs& a) { return (long long)a.tiles * a.Hkv * a.n_splits - a.few; }
+struct PrefillRange {
+  int item, split, ranges;
+};
+FA_HD PrefillRange prefill_range(const PrefillArgs& a, int x) {
+  if (a.n_splits == 1) return PrefillRange{x, 0, 1};
+  const int items = a.tiles * a.Hkv, split = x / items;
+  int item = x - split * items;
+  if (a.few && split == a.n_splits - 1) item += a.few;
+  return PrefillRange{item, split, a.n_splits - (item < a.few ? 1 : 0)};
 }
 
 }  // namespace fa

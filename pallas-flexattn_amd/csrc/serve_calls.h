@@ -68,12 +68,15 @@ int prefill_args(const fa_prefill_call* c, int cus, fa::PrefillArgs* a, PrefillL
   if (a->win_left >= 0)
     walk = std::min(walk, ((long long)a->win_left + fa::kPrefillRows / g + fa::kPrefillKeys) / fa::kPrefillKeys + 2);
   // Workgroups for all that run at a time, two per compute unit at D = 128, else three (300 items of D = 64, 8192 keys: 129 us in
-  // two ranges each, 164 whole).  Packed rows: the tiles that rows leave partly filled are not counted; with lengths: about half
-  // the rows are there (16 ragged rows, 512 items: 110 us in two ranges, 130 whole; where most of them are: 258, 242).
-  const long long full = packed ? std::max(1ll, (long long)c->T * g / fa::kPrefillRows) * c->Hkv
+  // two ranges each, 164 whole).  Packed rows: as many tiles as full ones, or as rows (31 of one token, 4200 keys: 63 us; in 32
+  // ranges, as for the tokens in one tile: 129); with lengths: about half the rows are there, which is not
+  // known (16 ragged rows, 512 items: 110 us in two ranges, 130 whole; where most of them are: 258, 242).
+  const long long full = packed ? std::max<long long>((long long)c->T * g / fa::kPrefillRows, std::min(c->B, c->T)) * c->Hkv
                                 : c->q_lens ? (items + 1) / 2 : items;
-  a->n_splits = fa::prefill_splits(full, (int)walk, (c->D == 128 ? 2 : 3) * cus);
-  if (items * a->n_splits > 0x7fffffll) a->n_splits = 1;
+  const fa::PrefillCut cut = fa::prefill_cut(full, (int)walk, (c->D == 128 ? 2 : 3) * cus, !c->q_lens);
+  const bool fits = items * cut.n <= 0x7fffffll;
+  a->n_splits = fits ? cut.n : 1;
+  a->few = fits ? cut.few : 0;
   const size_t rows = (size_t)(packed ? 1 : c->B) * Hq * c->T;
   if (rows > 0x7fffffffull) return FA_ERR_SHAPE;
   L->bytes = a->n_splits > 1 ? rows * a->n_splits * (c->D + 2) * sizeof(float) : 0;

@@ -107,8 +107,36 @@ static int rows() {
   return 0;
 }
 
+// Every range of every item in one workgroup; as many workgroups as are wanted where that can be.
+static int cuts() {
+  for (int n = 0; n < 4000; ++n) {
+    PrefillArgs a{};
+    a.tiles = (int)draw(1, 90);
+    a.Hkv = (int)draw(1, 9);
+    const int items = a.tiles * a.Hkv, tiles = (int)draw(1, 200), want = (int)draw(1, 800);
+    const int counted = (int)draw(1, items);  // (of packed rows not all tiles are)
+    const PrefillCut c = prefill_cut(counted, tiles, want, n % 3);
+    a.n_splits = c.n;
+    a.few = c.few;
+    if (c.n < 1 || c.n > kPrefillSplits || c.few < 0 || c.few > counted || (c.few && c.n < 2)) return fail("prefill_cut", c.n, c.few);
+    if (c.n > 1 && c.n > tiles) return fail("ranges of a walk", c.n, tiles);
+    if (n % 3 && counted == items && c.few && prefill_grid(a) != want) return fail("workgroups", prefill_grid(a), want);
+    std::vector<int> got((size_t)items * c.n, 0);
+    for (int x = 0; x < prefill_grid(a); ++x) {
+      const PrefillRange r = prefill_range(a, x);
+      if (r.item < 0 || r.item >= items || r.split < 0 || r.split >= r.ranges || r.ranges > c.n) return fail("prefill_range", x, r.item);
+      if (r.ranges != c.n - (r.item < c.few ? 1 : 0)) return fail("ranges", r.ranges, c.n);
+      ++got[(size_t)r.item * c.n + r.split];
+    }
+    for (int i = 0; i < items; ++i)
+      for (int k = 0; k < c.n; ++k)
+        if (got[(size_t)i * c.n + k] != (k < c.n - (i < c.few ? 1 : 0))) return fail("a range's workgroups", i, k);
+  }
+  return 0;
+}
+
 int main() {
-  if (spans() || packed() || rows()) return 1;
+  if (spans() || packed() || rows() || cuts()) return 1;
   std::printf("ok\n");
   return 0;
 }
