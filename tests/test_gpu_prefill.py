@@ -130,6 +130,37 @@ def test_packed(new, kind):
 
 
 @pytest.mark.parametrize("kind", ["bf16", "fp8"])
+@pytest.mark.parametrize("packed", [False, True])
+def test_items_of_unequal_ranges(kind, packed):
+    """300 items (packed: 304, the first of single tokens) where 512 run at a time: some in one range of keys, whose results the join
+    must leave, the others in two."""
+    import torch
+    import pallas_flexattn as pf
+    D, Hq, Hkv = 128, 16, 4
+    new = [1] * 5 + [33] + [800] * 3 if packed else [800] * 3
+    lens = [n + x for n, x in zip(new, (300, 0, 64, 1, 500, 100, 0, 77, 200) if packed else (0, 77, 200))]
+    c = _cache(kind, lens, Hkv, 64, D, 41)
+    if not packed:
+        q = _q(3, Hq, 800, D, 42)
+        o, lse = pf.flex_prefill(q, c.cache, c.lens, c.table, mask_mod=pf.causal_mask, enable_gqa=True, return_lse=True)
+        return _check(o, lse, q, c, lens, None, -1, 0)
+    starts = [0, *np.cumsum(new).tolist()]
+    q = _q(1, Hq, starts[-1] + 9, D, 42)
+    o, lse = pf.flex_prefill(q, c.cache, c.lens, c.table, mask_mod=pf.causal_mask, enable_gqa=True, return_lse=True,
+                             query_starts=torch.tensor(starts, device="cuda", dtype=torch.int32))
+    assert (o[:, :, starts[-1]:] == 0).all() and torch.isneginf(lse[:, :, starts[-1]:]).all()
+    for some in (range(6), range(6, 9)):
+        T = max(new[b] for b in some)
+        pad = torch.zeros(len(some), Hq, T, D, device="cuda", dtype=torch.bfloat16)
+        po, pl = torch.zeros_like(pad), torch.full((len(some), Hq, T), float("-inf"), device="cuda")
+        for i, b in enumerate(some):
+            pad[i, :, :new[b]] = q[0, :, starts[b]:starts[b + 1]]
+            po[i, :, :new[b]], pl[i, :, :new[b]] = o[0, :, starts[b]:starts[b + 1]], lse[0, :, starts[b]:starts[b + 1]]
+        part = type("Rows", (), {"rows": [x[some.start:some.stop] for x in c.rows]})
+        _check(po, pl, pad, part, [lens[b] for b in some], [new[b] for b in some], -1, 0)
+
+
+@pytest.mark.parametrize("kind", ["bf16", "fp8"])
 def test_query_lens(kind):
     """Padded rows of every length, to none, whose padding is NaN; lengths past the sizes and below zero."""
     import torch
