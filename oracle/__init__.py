@@ -25,6 +25,9 @@ would be marked "parity unpinned"; none is):
                     of the reference's tiled Pallas kernels (fwd ``flash_attn.py:59-108``,
                     bwd ``:168-407``) with the same bf16 cast points.  Used as the CPU
                     baseline and cross-checked against ``attention``.
+* ``pages``       — forks and compactions of paged rows in plain Python (no reference
+                    counterpart).  Pinned by the invariants that define them
+                    (``tests/test_pages_oracle.py``).
 * ``bf16``        — float32 -> bfloat16 round-to-nearest-even in numpy.
 * ``fp8``         — OCP e4m3 codec, the fp8 path's block quantisation and a
                     model of its P rounding (no reference counterpart: the
