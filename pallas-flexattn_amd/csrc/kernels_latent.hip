@@ -11,6 +11,7 @@ static void run_latent(const LatentArgs& a, int nb, hipStream_t s) {
   switch (nb) {
     case 1: hipLaunchKernelGGL((latent_decode_kernel<L, R, 1>), grid, dim3(256), 0, s, a); break;
     case 2: hipLaunchKernelGGL((latent_decode_kernel<L, R, 2>), grid, dim3(256), 0, s, a); break;
+    case 3: hipLaunchKernelGGL((latent_decode_kernel<L, R, 3>), grid, dim3(256), 0, s, a); break;
     default: hipLaunchKernelGGL((latent_decode_kernel<L, R, 4>), grid, dim3(256), 0, s, a); break;
   }
 }

@@ -56,6 +56,9 @@ __device__ __forceinline__ void mma_q(f32x4& c, u32x4 a, u32x4 b) {
   else asm("v_mfma_f32_16x16x32_bf16 %0, %1, %2, %0" : "+v"(c) : "v"(a), "v"(b));
 }
 __device__ __forceinline__ void mma_q_drain(f32x4& c, f32x4& d) { asm volatile("s_nop 7\n\ts_nop 7\n\ts_nop 3" : "+v"(c), "+v"(d)); }
+__device__ __forceinline__ void mma_q_drain(f32x4& c, f32x4& d, f32x4& e) {
+  asm volatile("s_nop 7\n\ts_nop 7\n\ts_nop 3" : "+v"(c), "+v"(d), "+v"(e));
+}
 __device__ __forceinline__ void mma_q_drain(f32x4& c, f32x4& d, f32x4& e, f32x4& f) {
   asm volatile("s_nop 7\n\ts_nop 7\n\ts_nop 3" : "+v"(c), "+v"(d), "+v"(e), "+v"(f));
 }
@@ -87,8 +90,8 @@ void latent_decode_kernel(LatentArgs a) {
   using X = LatentShape<L, R, NB>;
   constexpr int NW = X::NW, RB = X::RB, CH = X::CH, KS = X::KS, TILE = X::TILE, ROWS = X::ROWS, HI = X::HI, J = X::J;
   constexpr int DTW = X::DTW, BN = kLatentKeys;
-  constexpr int AHEAD = NB == 4 ? 2 : NB == 2 ? 5 : 8;  // LDS reads ahead of their products
-  constexpr int JS = NB == 4 ? J : 2 * J;  // copies that go between the products of S, the others between those of O
+  constexpr int AHEAD = NB >= 3 ? 2 : NB == 2 ? 5 : 8;  // LDS reads ahead of their products
+  constexpr int JS = NB >= 3 ? J : 2 * J;  // copies that go between the products of S, the others between those of O
   constexpr float kLazy = 8.0f;  // a maximum may be this stale (log2): P stays under 2^8
   __shared__ __attribute__((aligned(1024))) char lds[2 * TILE];
   __shared__ __attribute__((aligned(16))) char pbuf[ROWS * 128];
@@ -159,7 +162,7 @@ void latent_decode_kernel(LatentArgs a) {
   auto copy_one = [&](const Copy& c, int i) {
     const int x = i / J, j = i % J;
     uint32_t off = dma[j / 2];
-    if constexpr (NB == 4) asm volatile("" : "+v"(off));  // (not unpacked ahead of the loop)
+    if constexpr (NB >= 3) asm volatile("" : "+v"(off));  // (not unpacked ahead of the loop)
     off = j & 1 ? off >> 16 : off & 0xffffu;
     if ((j + 1) * NW <= HI || w + NW * j < HI) dma16(c.rs[x], (int)off, c.to + x * (kTileKeys * RB) + NW * j * 1024, j == 0);
   };
@@ -293,6 +296,7 @@ void latent_decode_kernel(LatentArgs a) {
       }
     }
     if constexpr (NB == 2) mma_q_drain(s[0], s[1]);
+    if constexpr (NB == 3) mma_q_drain(s[0], s[1], s[2]);
     if constexpr (NB == 4) mma_q_drain(s[0], s[1], s[2], s[3]);
     // lane: keys k0 + 16 w + 4 g + 0 .. 3
     const bool whole = k0 + BN <= kend && s1.lo <= k0 && s0.hi >= k0 + BN - 1;  // every row sees every key
@@ -367,7 +371,7 @@ void latent_decode_kernel(LatentArgs a) {
       auto val_frag = [&](int x) {
         const int t = x % DTW, at = (x / DTW) * (32 * RB) + (t / VN) * (32 * VN);
         uint32_t off = va[t % VN];
-        if constexpr (NB == 4) asm volatile("" : "+v"(off));
+        if constexpr (NB >= 3) asm volatile("" : "+v"(off));
         const uint2 lo = lds_read_tr16(tile + (off & 0xffffu) + at), hi = lds_read_tr16(tile + (off >> 16) + at);
         return u32x4{lo.x, lo.y, hi.x, hi.y};
       };

@@ -169,9 +169,10 @@ int latent_args(const fa_latent_call* c, int cus, fa::LatentArgs* a, LatentLayou
   const int left = c->window_left < 0 || c->window_left >= c->kv_len ? -1 : c->window_left;
   long long tiles = (c->kv_len + (long long)fa::kTileKeys - 1) / fa::kTileKeys;
   if (left >= 0) tiles = std::min(tiles, ((long long)left + c->T + fa::kTileKeys - 2) / fa::kTileKeys + 1);
-  // rows of an item: as many as there are, up to 64, so that a key is read for all of them at once
-  L->nb = rows <= 16 ? 1 : rows <= 32 ? 2 : 4;
-  const long long rt = (rows + 16 * L->nb - 1) / (16 * L->nb), items = c->B * rt;
+  // rows of an item: up to 64, so that a key is read for as many at once, and of one size (16 batch rows of 96 rows: 45.5 us
+  // in two blocks of 48, 49.4 in 64 and 32)
+  const long long rt = (rows + 63) / 64, items = c->B * rt;
+  L->nb = (int)(((rows + 15) / 16 + rt - 1) / rt);
   if (items * tiles > 0x7fffffffll - (1 << 20)) return FA_ERR_SHAPE;  // tile numbers of a call are 32 bits
   d.page_table = c->page_table;
   d.kv_lens = c->kv_lens;

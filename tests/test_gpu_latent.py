@@ -89,6 +89,13 @@ def test_decode(case):
     assert (pf.flex_decode_latent(q, qr, c.cache, 0.05, c.lens, c.table, mask_mod=mask) == o).all()
 
 
+@pytest.mark.parametrize("case", [([700, 90, 64], 32, 3, 512, 64, 64, (-1, 0)), ([400, 33], 24, 2, 256, 32, 32, (-1, 0)),
+                                  ([1500, 7, 0], 45, 2, 128, 64, 96, (300, 0)), ([5000], 72, 1, 512, 32, 128, None),
+                                  ([96, 95, 1], 37, 1, 256, 64, 32, (31, 3))], ids=range(5))
+def test_blocks_of_48_rows(case):
+    test_decode(case)
+
+
 @pytest.mark.parametrize("H", [4, 10, 40])  # one, two and four 16-row blocks
 def test_query_lens_and_what_is_not_there(H):
     """Padded rows to none, lengths past the table and below zero, page ids outside the cache (zero keys), kv_len, no table, 64-bit numbers."""
