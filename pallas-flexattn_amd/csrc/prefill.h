@@ -705,12 +705,11 @@ __global__ __launch_bounds__(256, D == 128 ? 2 : 3) void prefill_kernel(PrefillA
   // The tiles that some row of this wave sees are [w0, w1): the wave only brings its part of the others.  (Three walks, so that
   // O is in no branch: the compiler kept it twice where it was.)
   const bool sees = x.see.hi >= x.see.lo && x.see.hi != 0x7fffffff;
-  int w0 = sees ? x.see.lo / BN : 0x7fffffff;
-  int w1 = sees ? x.see.hi / BN + 1 : 0;
-#pragma unroll
-  for (int d = 1; d < 64; d <<= 1) {
-    w0 = imin(w0, __shfl_xor(w0, d, 64));
-    w1 = imax(w1, __shfl_xor(w1, d, 64));
+  const unsigned long long seen = __ballot(sees);  // (spans do not fall from one row to the next)
+  int w0 = 0x7fffffff, w1 = 0;
+  if (seen) {
+    w0 = __builtin_amdgcn_readlane(x.see.lo, __builtin_ctzll(seen)) / BN;
+    w1 = __builtin_amdgcn_readlane(x.see.hi, 63 - __builtin_clzll(seen)) / BN + 1;
   }
   w0 = __builtin_amdgcn_readfirstlane(imin(imax(w0, ts.t0), ts.t1));
   w1 = __builtin_amdgcn_readfirstlane(imin(imax(w1, w0), ts.t1));
