@@ -63,6 +63,9 @@ __device__ __forceinline__ void mma_q_drain(f32x4& c, f32x4& d, f32x4& e, f32x4&
   asm volatile("s_nop 7\n\ts_nop 7\n\ts_nop 3" : "+v"(c), "+v"(d), "+v"(e), "+v"(f));
 }
 
+// bits 0 and 16: whether w's two bf16 are infinities or NaN
+__device__ __forceinline__ uint32_t odd_halves(uint32_t w) { return (((w & 0x7f807f80u) + 0x00800080u) & 0x80008000u) >> 15; }
+
 // A workgroup's piece of work.  The partition (decode_index.h) is one of the batch rows' keys: the rt row blocks of a
 // batch row take the same pieces, in workgroups 8 apart, so that they run at one time on one XCD, and all but the first read the
 // keys from its L2.
@@ -96,7 +99,8 @@ void latent_decode_kernel(LatentArgs a) {
   __shared__ __attribute__((aligned(1024))) char lds[2 * TILE];
   __shared__ __attribute__((aligned(16))) char pbuf[ROWS * 128];
   __shared__ __attribute__((aligned(16))) float red[ROWS][4];
-  __shared__ __attribute__((aligned(16))) int over[4];
+  constexpr int kHigher = 1, kWild = 2;
+  __shared__ __attribute__((aligned(16))) int over[4];  // what each wave found in the tile: a higher maximum, values that are not finite
   __shared__ uint32_t wild[NW][2];  // keys of the tile with values that are not finite, as each wave found them
 
   const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -171,24 +175,30 @@ void latent_decode_kernel(LatentArgs a) {
   const KeySpan s0 = key_span(have - ql, have, p.win_left, p.win_right);
   const KeySpan s1 = key_span(have - 1, have, p.win_left, p.win_right);
   auto cut = [&](int k0) { return s1.lo > k0 || s0.hi < imin(k0 + BN, kend) - 1; };
-  auto look = [&](int k0, int buf) {  // between the products: taken out of this wave's part of the tile, and noted by key
-    if (!cut(k0)) return;
+  // (A wave's part of the tile holds pieces of all waves' keys: it may be changed only when every wave has read its own
+  // keys for S, so the values are noted by key first, and taken out behind the barrier that all waves meet at then.)
+  auto piece = [&](int buf, int x, int j) { return reinterpret_cast<u32x4*>(lds + buf * TILE + x * (kTileKeys * RB) + j * 1024 + lane * 16); };
+  auto note = [&](int k0, int buf) {  // -> whether this wave's part of a tile that is cut has such values
+    if (!cut(k0)) return 0;
     if (lane < 2) wild[w][lane] = 0;
+    bool found = false;
     for (int x = 0; x < 2; ++x)
       for (int j = w; j < HI; j += NW) {
-        u32x4* at = reinterpret_cast<u32x4*>(lds + buf * TILE + x * (kTileKeys * RB) + j * 1024 + lane * 16);
-        u32x4 v = *at;
-        uint32_t bad = 0u;
-#pragma unroll
-        for (int y = 0; y < 4; ++y) {
-          const uint32_t odd = (((v[y] & 0x7f807f80u) + 0x00800080u) & 0x80008000u) >> 15;  // bits 0 and 16
-          bad |= odd;
-          v[y] &= ~(odd * 0xffffu);
-        }
-        if (bad) {
-          *at = v;
+        const u32x4 v = *piece(buf, x, j);
+        if (odd_halves(v[0]) | odd_halves(v[1]) | odd_halves(v[2]) | odd_halves(v[3])) {
+          found = true;
           atomicOr(&wild[w][x], 1u << ((j * 64 + lane) / CH));
         }
+      }
+    return __any(found);
+  };
+  auto take_out = [&](int buf) {
+    for (int x = 0; x < 2; ++x)
+      for (int j = w; j < HI; j += NW) {
+        u32x4 v = *piece(buf, x, j);
+#pragma unroll
+        for (int y = 0; y < 4; ++y) v[y] &= ~(odd_halves(v[y]) * 0xffffu);
+        *piece(buf, x, j) = v;
       }
   };
   // LDS offsets: S's A operand (key 16 kg + r, chunk 4 s + g) for even and odd s, and O's (transposing reads:
@@ -336,12 +346,16 @@ void latent_decode_kernel(LatentArgs a) {
       top[n] = fmaxf(fmaxf(s[n][0], s[n][1]), fmaxf(s[n][2], s[n][3])) * p.scale_log2;
       higher = higher || top[n] > m[n] + kLazy;
     }
-    const int any = __any(higher);
+    const int any = (__any(higher) ? kHigher : 0) | (note(k0, buf) ? kWild : 0);
     if (lane == 0) over[w] = any;
-    look(k0, buf);
-    __syncthreads();
+    __syncthreads();  // every wave's scores are made: nobody reads the tile's keys for S any more
     const i32x4 ov = *reinterpret_cast<const i32x4*>(over);
-    if (__builtin_amdgcn_readfirstlane(ov[0] | ov[1] | ov[2] | ov[3])) {  // (the same in every wave)
+    const int todo = __builtin_amdgcn_readfirstlane(ov[0] | ov[1] | ov[2] | ov[3]);  // (the same in every wave)
+    if (todo & kWild) {
+      take_out(buf);
+      __syncthreads();
+    }
+    if (todo & kHigher) {
 #pragma unroll
       for (int n = 0; n < NB; ++n) {
         top[n] = quad_max(top[n]);
@@ -395,9 +409,9 @@ void latent_decode_kernel(LatentArgs a) {
         __builtin_amdgcn_sched_barrier(0);
       }
     }
-    if (cut(k0)) {
-      // A value that is not finite makes NaN of that element in the rows that see its key (the score that it gave
-      // is not finite either: nothing else can come out).  From the cache: nothing has to be kept for it.
+    if (todo & kWild) {
+      // A value that is not finite makes NaN of that element in the rows that see its key (the score that it gave, before
+      // it was taken out, is not finite either: nothing else can come out).  From the cache: nothing has to be kept for it.
       for (int x = 0; x < 2; ++x) {
         uint32_t keys = 0u;
         for (int y = 0; y < NW; ++y) keys |= wild[y][x];
