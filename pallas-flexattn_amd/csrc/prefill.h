@@ -251,7 +251,9 @@ struct PrefillWave {
   __device__ __forceinline__ void patch(const PrefillArgs& a, int b, int hk, int k0, int keys, int lane) {
     const int run = k0 / kTileKeys, pg = run / a.page_runs;  // (of a page that is there: its values were read)
     const int page = a.page_table ? scalar_load(a.page_table + (size_t)b * a.max_pages, pg) : b;
-    const size_t row = ((size_t)(page * a.Hkv + hk) * a.page_runs + (run - pg * a.page_runs)) * kTileKeys + k0 % kTileKeys;
+    const int at_run = (page * a.Hkv + hk) * a.page_runs + (run - pg * a.page_runs);
+    const size_t row = (size_t)at_run * kTileKeys + k0 % kTileKeys;
+    [[maybe_unused]] const float vsc = kFp8 ? __uint_as_float(scalar_load(reinterpret_cast<const int*>(a.vs), at_run)) : 1.f;
     asm volatile("" : "+v"(lane));  // (addresses not kept for the whole walk)
     const int first = 8 * (lane >> 5);
     frag seen;
@@ -267,15 +269,10 @@ struct PrefillWave {
       for (int e = 0; e < 8; ++e) {
         const bool here = (keys >> (first + e)) & 1;  // (a key past the row's end is in the page all the same)
         const size_t at = (row + first + e) * D + 32 * i + (lane & 31);
-        bool plus, minus;
-        if constexpr (kFp8) {
-          plus = minus = (static_cast<uint8_t>(a.v[at]) & 0x7f) == 0x7f;
-        } else {
-          const uint32_t v = *reinterpret_cast<const uint16_t*>(a.v + 2 * at);
-          const bool nan = (v & 0x7fffu) > 0x7f80u;
-          plus = nan || v == 0x7f80u;
-          minus = nan || v == 0xff80u;
-        }
+        uint32_t v;  // as the tile had it, in the upper half: a code is infinite, too, where its scale takes it past bf16
+        if constexpr (kFp8) v = cvt_e4m3_lo((uint32_t) static_cast<uint8_t>(a.v[at]) << 8, vsc);
+        else v = (uint32_t) * reinterpret_cast<const uint16_t*>(a.v + 2 * at) << 16;
+        const bool plus = __builtin_amdgcn_classf(__uint_as_float(v), 0x203), minus = __builtin_amdgcn_classf(__uint_as_float(v), 0x007);
         up[e >> 1] |= (here && plus ? 0x7f7fu : 0u) << (16 * (e & 1));
         down[e >> 1] |= (here && minus ? 0xff7fu : 0u) << (16 * (e & 1));
       }
@@ -824,12 +821,14 @@ __global__ __launch_bounds__(256, D == 128 ? 2 : 3) void prefill_kernel(PrefillA
   for (int t = w1; t < ts.t1; ++t) pass(t);
 
   x.drain();
+  // (computed again: kept through the walk, it is one register too many at D = 64)
+  const int le = __builtin_amdgcn_mbcnt_hi(~0u, __builtin_amdgcn_mbcnt_lo(~0u, 0u)), lre = le & 31, hhe = le >> 5;
   const float lt = pair_sum(x.l);
-  const auto me = W::row(a, it, it.row0 + 32 * w + lr);
+  const auto me = W::row(a, it, it.row0 + 32 * w + lre);
   // row of lse (and of the partial results)
   const size_t at = ((size_t)(kPacked ? 0 : it.b) * a.Hq + hk * a.g + me.hq) * a.Sq + it.tok + me.qi;
   const size_t all = (size_t)(kPacked ? 1 : a.B) * a.Hq * a.Sq;
-  if (me.valid && hh == 0) note_ml(a, range, D, all, at, split_ml(x.m, lt, me.live));
+  if (me.valid && hhe == 0) note_ml(a, range, D, all, at, split_ml(x.m, lt, me.live));
   if (range.ranges > 1) {
     if (me.valid) {
       float* po = a.part + ((size_t)range.split * all + at) * D;
@@ -838,7 +837,7 @@ __global__ __launch_bounds__(256, D == 128 ? 2 : 3) void prefill_kernel(PrefillA
         for (int i = 0; i < DT; ++i)
 #pragma unroll
           for (int j = 0; j < 4; ++j)
-            *reinterpret_cast<f32x4*>(po + 32 * i + 8 * j + 4 * hh) =
+            *reinterpret_cast<f32x4*>(po + 32 * i + 8 * j + 4 * hhe) =
                 f32x4{x.oacc[i][4 * j], x.oacc[i][4 * j + 1], x.oacc[i][4 * j + 2], x.oacc[i][4 * j + 3]};
       }
     }
@@ -856,12 +855,12 @@ __global__ __launch_bounds__(256, D == 128 ? 2 : 3) void prefill_kernel(PrefillA
       const int c = 4 * i + j;
       const u32x2 y{pack_bf16x2(x.oacc[i][4 * j] * inv, x.oacc[i][4 * j + 1] * inv),
                     pack_bf16x2(x.oacc[i][4 * j + 2] * inv, x.oacc[i][4 * j + 3] * inv)};
-      *reinterpret_cast<u32x2*>(stage + lr * RB + ((c ^ (lr % KCH)) * 16) + hh * 8) = none ? u32x2{0u, 0u} : y;
+      *reinterpret_cast<u32x2*>(stage + lre * RB + ((c ^ (lre % KCH)) * 16) + hhe * 8) = none ? u32x2{0u, 0u} : y;
     }
-  const int c = lane % KCH;
+  const int c = le % KCH;
 #pragma unroll
   for (int k = 0; k < 32 / RPI; ++k) {
-    const int rr = k * RPI + lane / KCH, row = it.row0 + 32 * w + rr;
+    const int rr = k * RPI + le / KCH, row = it.row0 + 32 * w + rr;
     const u32x4 y = *reinterpret_cast<const u32x4*>(stage + rr * RB + ((c ^ (rr % KCH)) * 16));
     if (row < rows) {
       const int i = row / a.g, hr = row - i * a.g;
@@ -869,7 +868,7 @@ __global__ __launch_bounds__(256, D == 128 ? 2 : 3) void prefill_kernel(PrefillA
       *reinterpret_cast<u32x4*>(o + c * 8) = y;
     }
   }
-  if (me.valid && hh == 0) a.lse[at] = none ? -INFINITY : (x.m + log2f(lt)) * kLn2;
+  if (me.valid && hhe == 0) a.lse[at] = none ? -INFINITY : (x.m + log2f(lt)) * kLn2;
 }
 
 // The splits of a row: M = max m_s, L = sum l_s 2^(m_s - M), O = sum O_s 2^(m_s - M) / L.  Four columns a thread, D / 4
