@@ -67,12 +67,11 @@ __device__ __forceinline__ void mma_q_drain(f32x4& c, f32x4& d, f32x4& e, f32x4&
 __device__ __forceinline__ uint32_t odd_halves(uint32_t w) { return (((w & 0x7f807f80u) + 0x00800080u) & 0x80008000u) >> 15; }
 
 // A workgroup's piece of work.  The partition (decode_index.h) is one of the batch rows' keys: the rt row blocks of a
-// batch row take the same pieces, in workgroups 8 apart, so that they run at one time on one XCD, and all but the first read the
-// keys from its L2.
+// batch row take the same pieces (latent_plan.h).
 __device__ __forceinline__ DecodeUnit latent_unit(const LatentArgs& a, int wg, bool first_wave) {
   const DecodeArgs& d = a.d;  // (rt = 1)
-  const int slot = wg / 8, xcd = wg % 8;
-  const int piece = a.rt > 1 ? slot / a.rt * 8 + xcd : wg, block = a.rt > 1 ? slot % a.rt : 0;
+  const LatentPlace at = latent_place(wg, a.rt, a.near);
+  const int piece = at.piece, block = at.block;
   DecodeUnit u;
   if (d.by_item && piece >= d.B) {
     u.b = -1;

@@ -1,6 +1,7 @@
 // Kernel arguments of the calls on a cache of latent vectors (latent.h, latent_append.h).
 #pragma once
 #include "decode_fp8.h"
+#include "latent_plan.h"
 #include "rotary.h"
 
 namespace fa {
@@ -10,6 +11,7 @@ constexpr int kLatentKeys = 64;  // keys of a tile: two runs of 32, each in one 
 struct LatentArgs {
   DecodeArgs d;  // the partition (Hkv = rt = 1, tiles of 32 keys), lengths, page table, windows, workspace, o, lse
   int rt;        // row blocks of a batch row
+  bool near;     // where they run (latent_place)
   const uint16_t* cache;  // (num_pages, page_size, L + R)
   const void *q, *qr;     // bf16; element strides of (row, head, query)
   long long qsb, qsh, qst, rsb, rsh, rst;

@@ -202,7 +202,8 @@ int latent_args(const fa_latent_call* c, int cus, fa::LatentArgs* a, LatentLayou
   d.pieces = d.pieces_even = (int)std::max(1ll, cus / rt);
   d.least = 2;
   const long long units = d.by_item ? c->B : fa::decode_grid(c->B, (int)tiles, d.pieces, d.least);
-  const long long grid = rt > 1 ? (units + 7) / 8 * 8 * rt : units;
+  a->near = fa::latent_near(units, (int)rt);
+  const long long grid = fa::latent_grid(units, (int)rt, a->near);
   if (grid > 0x7fffffll) return FA_ERR_SHAPE;
   d.grid = (int)grid;
   const size_t slots = d.by_item ? 0 : (size_t)fa::decode_slots(units, d.pieces) * rt * 16 * L->nb;
