@@ -51,9 +51,17 @@ def create_fp8_kv_cache(num_pages: int, kv_heads: int, page_size: int, head_dim:
     return Fp8KVCache(*codes, *scales)
 
 
+def _whole(x, device):
+    """Whole numbers as a tensor (a list or array is copied to ``device``; an empty one has no type of its own)."""
+    if x is None or hasattr(x, "data_ptr"):
+        return x
+    t = _torch().as_tensor(x, device=device)
+    return t if t.numel() else t.int()
+
+
 def _rows(x, like):
     """Per-row integers as a tensor (a list or array is copied to ``like``'s device)."""
-    return x if x is None or hasattr(x, "data_ptr") else _torch().as_tensor(x, device=like.device)
+    return _whole(x, like.device)
 
 
 def append_kv_cache(cache, key, value, kv_lens, page_table=None, new_lens=None, rotary: Optional[Rotary] = None,

@@ -10,17 +10,15 @@ free, so a row that is not taken over is freed by that.
 Page ids, tables and lengths are int32 (read as they are) or int64; what comes back is int32.
 """
 from . import _lib
-from .flash_attn import _torch
+from .kv_cache import _whole
 
 
 def _ints(x, caches):
     """Whole numbers as a tensor (a list or array is copied to the caches' device)."""
-    if x is None or hasattr(x, "data_ptr"):
-        return x
     c = caches
     while isinstance(c, (list, tuple)) and c:
         c = c[0]
-    return _torch().as_tensor(x, device=getattr(c, "device", None))
+    return _whole(x, getattr(c, "device", None))
 
 
 def copy_kv_pages(caches, src, dst) -> None:
