@@ -9,6 +9,8 @@ free, so a row that is not taken over is freed by that.
 
 Page ids, tables and lengths are int32 (read as they are) or int64; what comes back is int32.
 """
+from numbers import Integral
+
 from . import _lib
 from .kv_cache import _whole
 
@@ -44,7 +46,7 @@ def fork_kv_rows(caches, page_table, kv_lens, parents=None, room=0, keep=None):
     hold.  ``free`` (int32, on the GPU) is how many are left; where it is negative so many were lacking, and
     the entries that lack one are -1 (tokens of a copy that could not be made are lost: look before going on).
     Page ids outside the cache stay as they are."""
-    per_row, number = (None, room) if isinstance(room, int) else (_ints(room, caches), 0)
+    per_row, number = (None, int(room)) if isinstance(room, Integral) else (_ints(room, caches), 0)
     rc, table, lens, free = _lib.launcher().page_plan(True, caches, page_table, _ints(kv_lens, caches), _ints(parents, caches),
                                                       per_row, number, keep)
     if rc:
