@@ -439,8 +439,9 @@ int fa_int64_to_int32(const int64_t *x, int32_t *y, int64_t n, void *stream);
  * kv_lens[b] - q_lens[b] + i, which is what the window and ALiBi refer to.  query is
  * (B, Hq, T, D) bf16; queries i >= q_lens[b] give o = 0 and lse = -inf, as do queries that see no key.
  * Packed (q_starts set, q_lens null): query is (1, Hq, T, D), row b's queries are its tokens
- * q_starts[b] .. q_starts[b + 1] - 1; q_starts (B + 1) begins with 0 and does not fall; tokens
- * behind its last entry give o = 0 and lse = -inf.  out: like query, strides of its own; lse float32, dense.
+ * q_starts[b] .. q_starts[b + 1] - 1; q_starts (B + 1) begins with 0 and does not fall (an entry below
+ * an earlier one counts as the highest before it); tokens behind its last entry, and before its first, give o = 0 and
+ * lse = -inf.  out: like query, strides of its own; lse float32, dense.
  * cache_dtype FA_DTYPE_BF16: fa_fwd_kvcache's layout; FA_DTYPE_FP8_E4M3: struct fa_fp8_cache's (powers of two as
  * scales).  page_size is a multiple of 32, D = 32, 64 or 128, rows are 16-byte aligned.  Page ids
  * outside the cache read as zero keys.  What no query sees may hold anything; a value that is not finite

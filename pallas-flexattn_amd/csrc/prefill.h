@@ -30,6 +30,17 @@
 
 namespace fa {
 
+// inclusive maximum over the lanes of a wave, of numbers that are not negative (as wave_scan)
+__device__ __forceinline__ int wave_max_scan(int x) {
+  x = imax(x, __builtin_amdgcn_update_dpp(0, x, 0x111, 0xf, 0xf, false));
+  x = imax(x, __builtin_amdgcn_update_dpp(0, x, 0x112, 0xf, 0xf, false));
+  x = imax(x, __builtin_amdgcn_update_dpp(0, x, 0x114, 0xf, 0xf, false));
+  x = imax(x, __builtin_amdgcn_update_dpp(0, x, 0x118, 0xf, 0xf, false));
+  x = imax(x, __builtin_amdgcn_update_dpp(0, x, 0x142, 0xa, 0xf, false));
+  x = imax(x, __builtin_amdgcn_update_dpp(0, x, 0x143, 0xc, 0xf, false));
+  return x;
+}
+
 // An item's rows [row0, row0 + kPrefillRows) of `rows` = g nq: queries i >= ql see nothing.
 struct PrefillItem {
   int b, row0, nq, ql, have, tok;  // tok: the row's first token (packed)
@@ -45,12 +56,15 @@ __device__ __forceinline__ PrefillItem prefill_item(const PrefillArgs& a, int re
     it.ql = a.q_lens ? clamp_len(scalar_load(a.q_lens, it.b), a.Sq) : a.Sq;
   } else {
     const int lane = threadIdx.x & 63;
-    int before = 0;
+    int before = 0, highest = 0;
     it.b = -1;
     for (int b0 = 0; b0 < a.B + 2; b0 += 64) {
       const int b = b0 + lane;
-      TokenSpan t{0, 0};
-      if (b < a.B + 2) t = packed_span(a.starts, b, a.B, a.Sq);
+      TokenSpan t = packed_span(a.starts, imin(b, a.B + 1), a.B, a.Sq);
+      if (b > a.B + 1) t = TokenSpan{0, 0};
+      const int high = imax(wave_max_scan(b <= a.B ? t.s : 0), highest);
+      highest = __builtin_amdgcn_readlane(high, 63);
+      if (b <= a.B) t = span_behind(t, high);
       const int n = row_tiles(t.e - t.s, a.g);
       const int end = before + wave_scan(n);
       const unsigned long long mine = __ballot(rest >= end - n && rest < end);

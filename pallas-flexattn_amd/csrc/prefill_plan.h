@@ -40,8 +40,16 @@ struct TokenSpan {
 };
 FA_HD TokenSpan packed_span(const int* starts, int b, int B, int total) {
   TokenSpan t;
-  t.s = b <= B ? clamp_len(starts[b], total) : 0;
-  t.e = b < B ? clamp_len(starts[b + 1], total) : b == B ? total : clamp_len(starts[0], total);
+  const int first = starts[b < B ? b : B], next = starts[b < B ? b + 1 : 0];  // (both at once, in no branch)
+  t.s = b <= B ? clamp_len(first, total) : 0;
+  t.e = b == B ? total : clamp_len(next, total);
+  if (t.e < t.s) t.e = t.s;
+  return t;
+}
+// A start below an earlier one counts as the highest before it (of row b: `before`), so that every token is in one span and
+// the call writes all results, whatever the starts are.
+FA_HD TokenSpan span_behind(TokenSpan t, int before) {
+  if (t.s < before) t.s = before;
   if (t.e < t.s) t.e = t.s;
   return t;
 }

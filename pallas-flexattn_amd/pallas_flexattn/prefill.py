@@ -25,7 +25,8 @@ def flex_prefill(query, cache, kv_lens=None, page_table=None, mask_mod=None, sco
 
     The new tokens, bf16, are padded or packed. Padded: ``query`` (B, Hq, T, D), of which row b has
     ``query_lens[b]`` (None: T). Packed: ``query`` (1, Hq, tokens, D) and ``query_starts`` (B + 1,): row b has tokens
-    ``query_starts[b]`` .. ``query_starts[b + 1] - 1``; it starts with 0 and does not fall.  Query i of a row's n sits at
+    ``query_starts[b]`` .. ``query_starts[b + 1] - 1``; it starts with 0 and does not fall (a start below an earlier one counts
+    as the highest before it).  Query i of a row's n sits at
     position ``kv_lens[b] - n + i``; ``mask_mod`` (``causal_mask``, ``sliding_window_mask`` or another
     window :class:`MaskSpec` without documents; None: every key) and ``score_mod`` (the built-in ALiBi and soft-cap descriptors)
     refer to it.  Padded tokens, packed ones behind the last row's, and queries that see no key return O = 0 and
