@@ -705,16 +705,16 @@ int fa_fwd_kvcache_fp8(const fa_params* p, const fa_fp8_cache* kv, const fa_stri
 
 size_t fa_prefill_workspace_bytes(const fa_prefill_call* c) {
   fa::PrefillArgs a;
-  PrefillLayout L;
-  return prefill_args(c, device_cus(), &a, &L) == FA_OK ? L.bytes : 0;
+  size_t bytes;
+  return prefill_args(c, device_cus(), &a, &bytes) == FA_OK ? bytes : 0;
 }
 
 int fa_prefill(const fa_prefill_call* c, void* workspace, size_t workspace_bytes, void* stream) {
   fa::PrefillArgs a;
-  PrefillLayout L;
-  const int rc = prefill_args(c, device_cus(), &a, &L);
+  size_t bytes;
+  const int rc = prefill_args(c, device_cus(), &a, &bytes);
   if (rc) return rc;
-  if (L.bytes && (!workspace || workspace_bytes < L.bytes || !aligned16({workspace}))) return FA_ERR_WORKSPACE;
+  if (bytes && (!workspace || workspace_bytes < bytes || !aligned16({workspace}))) return FA_ERR_WORKSPACE;
   a.part = static_cast<float*>(workspace);
   const bool fp8 = c->cache_dtype == FA_DTYPE_FP8_E4M3, mods = c->alibi_slopes || c->softcap > 0.f;
   const hipStream_t s = static_cast<hipStream_t>(stream);

@@ -90,16 +90,16 @@ FA_HD TileSpan tile_span(int have, int ql, int i0, int i1, int left, int right) 
 constexpr long long kMergeWide = 1 << 17;
 
 // Ranges of keys that an item is cut into where there are fewer items than `want`, the workgroups that run at a time: each at least
-// kPrefillLeast tiles of the longest row, at most kPrefillSplits.  If the items are `even`, the last of them get one range more, so
+// a tile of the longest row, at most kPrefillSplits.  If the items are `even`, the last of them get one range more, so
 // that `want` workgroups come out: 375 of 512 in one range each leave half the compute units with one workgroup and
 // half with two (8192 keys, D = 128: 237 us, 257 whole, 245 all in two).
-constexpr int kPrefillSplits = 32, kPrefillLeast = 1;
+constexpr int kPrefillSplits = 32;
 struct PrefillCut {
   int n, few;  // ranges; the first `few` items have one less
 };
 FA_HD PrefillCut prefill_cut(long long items, int most_tiles, int want, bool even) {
   if (items >= want) return PrefillCut{1, 0};
-  const int most = most_tiles / kPrefillLeast < kPrefillSplits ? most_tiles / kPrefillLeast : kPrefillSplits;
+  const int most = most_tiles < kPrefillSplits ? most_tiles : kPrefillSplits;
   const long long n = want / items;
   if (n >= most) return PrefillCut{most < 1 ? 1 : most, 0};
   if (!even || items * n == want) return PrefillCut{(int)n, 0};

@@ -8,10 +8,8 @@ int paged_ok(int B, int page_size, int max_pages, int num_pages, const int32_t* 
 }
 bool normal_or_zero(float x) { return x == 0.f || (x >= FLT_MIN && x <= FLT_MAX); }
 
-struct PrefillLayout {
-  size_t bytes;
-};
-int prefill_args(const fa_prefill_call* c, int cus, fa::PrefillArgs* a, PrefillLayout* L) {
+// (*workspace: its bytes)
+int prefill_args(const fa_prefill_call* c, int cus, fa::PrefillArgs* a, size_t* workspace) {
   if (!c) return FA_ERR_NULL;
   if (c->abi_version != FA_ABI_VERSION) return FA_ERR_VERSION;
   if (c->cache_dtype != FA_DTYPE_BF16 && c->cache_dtype != FA_DTYPE_FP8_E4M3) return FA_ERR_DTYPE;
@@ -79,7 +77,7 @@ int prefill_args(const fa_prefill_call* c, int cus, fa::PrefillArgs* a, PrefillL
   a->few = fits ? cut.few : 0;
   const size_t rows = (size_t)(packed ? 1 : c->B) * Hq * c->T;
   if (rows > 0x7fffffffull) return FA_ERR_SHAPE;
-  L->bytes = a->n_splits > 1 ? rows * a->n_splits * (c->D + 2) * sizeof(float) : 0;
+  *workspace = a->n_splits > 1 ? rows * a->n_splits * (c->D + 2) * sizeof(float) : 0;
   return FA_OK;
 }
 
