@@ -9,7 +9,9 @@
 // id), a mark per page, and ranks of the free pages.  Where marks and rows fit in LDS one
 // workgroup does all of it in one launch; else the marks lie in the workspace and three
 // launches (a compaction: four) follow each other.  A mark is the smallest claim on its page, so no result
-// depends on the order of the atomics.
+// depends on the order of the atomics.  In the larger plans, too, one workgroup ranks all pages, which is most of their time:
+// a fork / a compaction of 8 rows of 100 pages among 24000 16 / 34 us (one launch), among 50000 36 / 76, among 500000 229 / 559;
+// 64 rows of 4096 among 300000 192 / 682 (pages of 128 bytes, so that the copies take little).
 #pragma once
 #include "common.h"
 #include "page_plan.h"

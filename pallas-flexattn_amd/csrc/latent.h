@@ -9,7 +9,7 @@
 // queries), and the 64 keys of a tile serve both products from LDS:
 //   * S^T = K Q^T (v_mfma_f32_16x16x32_bf16): a wave takes 16 of the tile's keys and all rows, whose Q
 //     stays in registers (4 of them per 32 of L + R and 16 rows);
-//   * the waves' P meet in LDS (bf16, 2^-9 relative as c is; sums take the unrounded values), against maxima that
+//   * the waves' P meet in LDS (bf16, half a step 2^-8 as for c; sums take the unrounded values), against maxima that
 //     they settle together when one of them has grown;
 //   * O^T += C^T P^T: a wave takes L / waves of the elements of all rows, so that each value of the
 //     tile is read from LDS once for all rows, by transposing reads; O stays in registers.
@@ -19,7 +19,9 @@
 // Measured at L + R = 576: 16 rows of 16 or 64 heads 5.2 TB/s of keys in the walk (a copy: 4.9); 24 ragged rows of 128 heads, 4500 keys
 // on average, 54 us and 9 for the join, of the 54 about 5 launch and search, 5 Q and the first tile, 5 the partial O
 // (33 MB), 38 the walk: 2.8 us a tile for both blocks of rows, 2.4 with a quarter of the products and 2.1 without the
-// copies, so both paths are nearly full.  S a tile ahead of O, in tiles of 32 keys, four of them in LDS: the same within 2 %.
+// copies.  By the counters no unit is busy for a third of the walk (matrix cores 12 us, VALU 10, LDS 8, reads 2.7 TB/s): a SIMD
+// has one wave, whose S, exponentials, two barriers and O follow one another with nothing beside them.  S a tile ahead of O,
+// in tiles of 32 keys, four of them in LDS: the same within 2 %.
 #pragma once
 #include "dma.h"
 #include "latent_args.h"

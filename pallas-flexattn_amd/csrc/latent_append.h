@@ -1,7 +1,8 @@
 // New tokens' latent vectors and rotary parts into a paged cache of them, the rotary parts turned to
 // their positions on the way (rotary.h); the launch's further workgroups turn the queries' rotary parts.
-// A thread takes 16 elements of a token.  Bound by the launch, for prompts by HBM (2 bytes read and
-// 2 written an element).
+// A thread takes 16 elements of a token.  Bound by the launch (a few tokens 6 us), for prompts by HBM (2 bytes read and
+// 2 written an element): 8 x 4096 tokens of 512 + 64 with 16 heads' queries 43 us, 4.9 TB/s, with 128 heads' 244, 4.7; without
+// queries 24, 3.2 TB/s; 1024 tokens 11 and 13.
 #pragma once
 #include "latent_args.h"
 

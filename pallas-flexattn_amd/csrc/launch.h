@@ -49,7 +49,7 @@ struct PrefillArgs;
 
 // Chunks of new tokens over a paged cache (kernels_prefill.hip: D = 32, 64 or 128; mods: ALiBi or a soft-cap), rows
 // over a cache of latent vectors (kernels_latent.hip: L = 128, 256 or 512, R = 32 or 64; nb: 16-row blocks per
-// work item, 1, 2 or 4), appends to it, and pages (kernels_pages.hip; marks null: the plan of one workgroup)
+// work item, 1 to 4), appends to it, and pages (kernels_pages.hip; marks null: the plan of one workgroup)
 template <int D>
 int launch_prefill(const PrefillArgs& a, bool fp8, bool mods, hipStream_t s);
 template <int L>

@@ -13,15 +13,17 @@
 //     tile leaves [0, 2^16] (or that has seen no key) takes the tile's maximum and rescales. What
 //     reference is used does not change O / l;
 //   * O^T += V^T P^T, V^T by transposing LDS reads, P straight from S's registers, rounded to bf16 there
-//     (2^-9 relative, as V and O are; l sums the unrounded values).
+//     (half a step, 2^-8, as for V and O; l sums the unrounded values).
 // A wave brings 16 of a tile's 64 keys, which lie in one run of 32 tokens and so in one page of any
 // size: bf16 by LDS DMA, out-of-range rows as zeros; 8-bit codes through registers, converted once per
 // workgroup (bf16 holds code x scale exactly) and written to the same layout: the products do not
 // know which cache they read.
 // Measured, 32 heads on 8 of D = 128: 4096 queries behind 28672 keys 1.90 ms, 1080 TFLOP/s, the matrix cores busy half
-// the cycles (a library product of 8192^3 1300); 1024 behind 16384 e4m3 keys 285 us and 11 for the join of two ranges, 960: converting
-// takes a fifth more VALU instructions and 8 stores to LDS a wave and tile.  16 heads of D = 64, 8 ragged rows, window of 1500, ALiBi and
-// soft-cap: 90 us, bound by the VALU (40 of its instructions per MFMA), 12 for the join.
+// the cycles (a library product of 8192^3 1300); 1024 behind 16384 e4m3 keys 285 us and 11 for the join of two ranges, 960: converting, once
+// per 128 rows, takes a fifth more VALU instructions and 8 stores to LDS a wave and tile (LDS cycles per product twice those of bf16).  16 heads
+// of D = 64, 8 ragged rows, window of 1500, ALiBi and soft-cap: 90 us and 12 for the join; its VALU instructions (39 per MFMA) are
+// 36 us of them, the matrix cores' 7: the units idle where a row is shorter than the padded tokens, of whose items half are taken to be
+// there and each is cut into as many ranges.
 #pragma once
 #include "decode_fp8.h"
 #include "dma.h"

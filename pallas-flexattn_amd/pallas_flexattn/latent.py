@@ -86,8 +86,9 @@ def flex_decode_latent(query, query_rope, cache: LatentKVCache, scale: float, kv
     are cut to it, and the work is divided by it.
 
     Made for decoding and short chunks: each key is read once for up to 64 rows (heads x queries), and long rows' keys
-    are split over as many workgroups as the batch needs.  (A long prompt takes fewer operations with its heads' keys
-    and values written out.)  Page ids outside the cache read as zero keys; what no query of a row sees
+    are split over as many workgroups as the batch needs.  (A prompt takes three times the operations that it
+    would take with its heads' keys and values written out, which are of two lengths, so that no other call here takes them; and
+    its blocks of rows walk all tiles that the batch row sees.)  Page ids outside the cache read as zero keys; what no query of a row sees
     may be anything."""
     _check_cache(cache)
     left, right, _ = _window(mask_mod, None, "flex_decode_latent")
